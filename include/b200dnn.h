@@ -424,6 +424,107 @@ typedef struct b200dnn_sdpa_t {
 } b200dnn_sdpa_t;
 B200DNN_API int32_t b200dnn_sdpa(const b200dnn_sdpa_t *desc, void *stream);
 
+/* ---- Serving: a paged key/value cache, the call that appends to it and the attention of one new token over it.  No
+ * counterpart in the reference, whose sdpa_direct takes keys and values as dense tensors of one length; here every sequence
+ * has a length and pages of its own, and query heads may share a key head.
+ * Index arrays (slots, positions, page tables, lengths) are read on the device.  An entry that is out of range is met by no
+ * access: the call leaves that token out (kv_append) or reads page 0 in its place (paged_attention: that sequence's output is
+ * unspecified), and b200dnn_stream_status reports it. ---- */
+
+/* A cache of num_pages pages of page_size tokens.  Element (page, token, head, d) of the keys lies at key[page * key_stride[0] +
+ * token * key_stride[1] + head * key_stride[2] + d], of the values likewise: [page][token][head][dim] and [page][head][token][dim]
+ * are both storage orders of it.  s8: x = code * scale with one f32 scale for each (page, token, head), scale_stride for both
+ * arrays.  Device memory. */
+typedef struct b200dnn_kv_cache_t {
+  int32_t dt;                     /* bf16 | s8 */
+  int32_t page_size;              /* any, >= 1 */
+  int32_t kv_heads, head_dim;     /* head_dim <= 256 */
+  int64_t num_pages;
+  void *key, *value;
+  float *key_scale, *value_scale; /* s8 only */
+  int64_t key_stride[3], value_stride[3], scale_stride[3];   /* elements: page, token, head */
+} b200dnn_kv_cache_t;
+
+/* Appends num_tokens tokens, of any number of sequences: the rows of k (rotated) and v go to the cache slots, the rows of q
+ * (rotated) to q_out.  Rotation of a row at position p, for i < rotary_dim / 2 with c = cos_table[p][i], s = sin_table[p][i]:
+ *   (a, b) -> (a c - b s, b c + a s),  a = x[i], b = x[i + rotary_dim / 2]   (interleaved: a = x[2 i], b = x[2 i + 1])
+ * in f32; elements from rotary_dim on stay as they are.  s8 cache: a row's codes and scale are those of
+ * b200dnn_quant_per_token on the rotated f32 row.  A token whose slot is negative is padding: nothing of it is written.  The slots of a call are
+ * distinct; where two tokens name one slot, its row afterwards is unspecified (no other row is touched). */
+typedef struct b200dnn_kv_append_t {
+  b200dnn_kv_cache_t cache;
+  int64_t num_tokens;             /* 0 allowed: nothing is done */
+  int32_t q_heads;                /* 0: no queries */
+  int32_t dt;                     /* bf16 | f32, of q, k, v and q_out */
+  int32_t rotary_dim;             /* even, <= head_dim; 0: no rotation (positions and tables are not read) */
+  int32_t interleaved;
+  int64_t q_stride[2], k_stride[2], v_stride[2], q_out_stride[2];   /* elements: token, head */
+  const void *q, *k, *v;
+  void *q_out;                    /* may be q itself, with the same strides */
+  const int32_t *positions;       /* [num_tokens], rows of the tables */
+  const float *cos_table, *sin_table;   /* [table_rows][table_ld >= rotary_dim / 2] */
+  int64_t table_rows, table_ld;
+  const int64_t *slots;           /* [num_tokens]: page * page_size + token in the page */
+} b200dnn_kv_append_t;
+B200DNN_API int32_t b200dnn_kv_append(const b200dnn_kv_append_t *desc, void *stream);
+
+/* Attention of one new token per sequence over the cache: sequence i sees the keys at its positions [max(0, n - window), n), n =
+ * seq_lens[i], position j on page page_table[i][j / page_size].  With z_j = scale (q . k_j), capped as softcap tanh(z_j /
+ * softcap) when softcap > 0, and m the largest:
+ *   out = sum_j exp(z_j - m) v_j / (sum_j exp(z_j - m) + exp(sink - m)),   lse = log of that denominator + m
+ * (the sink's term only with sinks, one logit per query head).  Query head h reads key head h / (q_heads / kv_heads).  n == 0
+ * gives zeros and an lse of minus infinity; n < 0 is a row of padding: nothing of it is written.  Sums and softmax in f32. */
+typedef struct b200dnn_paged_attention_t {
+  b200dnn_kv_cache_t cache;
+  int32_t num_seqs;               /* 0 allowed: nothing is done */
+  int32_t q_heads;                /* a multiple of kv_heads */
+  int32_t q_dt, out_dt;           /* bf16; bf16 | f32 */
+  int64_t q_stride[2], out_stride[2];   /* elements: sequence, head */
+  const void *q;
+  void *out;                      /* does not overlap q */
+  float *lse;                     /* [num_seqs][q_heads], may be NULL */
+  const int32_t *page_table;      /* [num_seqs][page_table_ld]; entries behind a sequence's last page are not used */
+  int64_t page_table_ld;
+  int32_t max_pages;              /* pages of the longest sequence that the table has room for, <= page_table_ld */
+  int32_t window;                 /* 0: all keys */
+  const int32_t *seq_lens;        /* [num_seqs], including the new token */
+  const float *sinks;             /* [q_heads], may be NULL */
+  double scale;                   /* 0 = 1 / sqrt(head_dim) */
+  float softcap;                  /* 0: off */
+  int32_t reserved;
+} b200dnn_paged_attention_t;
+B200DNN_API int32_t b200dnn_paged_attention(const b200dnn_paged_attention_t *desc, void *stream);
+
+/* Routing with the forms that b200dnn_moe_route does not have.  No counterpart in the reference (see there).  Per token:
+ *   s = softmax | sigmoid of the logits;  c = s + bias (the bias chooses, it does not weigh);
+ *   the experts lie in num_groups groups of equal size; a group's score is its largest c, or the sum of its two largest;
+ *   of the topk_groups groups with the highest scores, the topk experts with the largest c, in descending order;
+ *   weights = s of the chosen, divided by their sum with renorm, times scale.
+ * Ties go to the lower index; scores are told apart as 64-bit values are.  A NaN ranks behind everything else (ids stay distinct
+ * and in range) and makes the token's weights NaN where it enters them.  ids [T][topk] (required) and weights as
+ * b200dnn_moe_route's, expert_counts and slot_to_row too. */
+enum { B200DNN_GATE_SOFTMAX = 0, B200DNN_GATE_SIGMOID = 1 };
+enum { B200DNN_GROUP_MAX = 0, B200DNN_GROUP_TOP2 = 1 };
+typedef struct b200dnn_moe_gate_t {
+  int32_t num_tokens;             /* 0 allowed: the counts are zero */
+  int32_t num_experts;            /* <= 1024 */
+  int32_t topk;                   /* <= 32 and <= the experts of topk_groups groups */
+  int32_t score;                  /* B200DNN_GATE_* */
+  int32_t num_groups, topk_groups;   /* 1, 1: no groups; num_groups <= 32 divides num_experts */
+  int32_t group_score;            /* B200DNN_GROUP_* */
+  int32_t renorm;
+  float scale;
+  int32_t logits_dt;              /* f32 | bf16 */
+  int64_t ld;                     /* of the logits, >= num_experts */
+  const void *logits;             /* [num_tokens][ld] */
+  const float *bias;              /* [num_experts], may be NULL */
+  int32_t *ids;
+  float *weights;                 /* may be NULL */
+  int32_t *expert_counts;         /* [num_experts], may be NULL */
+  int32_t *slot_to_row;           /* [num_tokens][topk], may be NULL */
+} b200dnn_moe_gate_t;
+B200DNN_API int32_t b200dnn_moe_gate(const b200dnn_moe_gate_t *desc, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -76,6 +76,38 @@ class SdpaDesc(C.Structure):
                 ("query", C.c_void_p), ("key", C.c_void_p), ("value", C.c_void_p), ("attn_mask", C.c_void_p), ("output", C.c_void_p)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("dt", C.c_int32), ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("num_pages", C.c_int64),
+                ("key", C.c_void_p), ("value", C.c_void_p), ("key_scale", C.c_void_p), ("value_scale", C.c_void_p),
+                ("key_stride", C.c_int64 * 3), ("value_stride", C.c_int64 * 3), ("scale_stride", C.c_int64 * 3)]
+
+
+class KvAppendDesc(C.Structure):
+    _fields_ = [("cache", KvCache), ("num_tokens", C.c_int64), ("q_heads", C.c_int32), ("dt", C.c_int32), ("rotary_dim", C.c_int32),
+                ("interleaved", C.c_int32), ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2),
+                ("q_out_stride", C.c_int64 * 2), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p),
+                ("positions", C.c_void_p), ("cos_table", C.c_void_p), ("sin_table", C.c_void_p), ("table_rows", C.c_int64),
+                ("table_ld", C.c_int64), ("slots", C.c_void_p)]
+
+
+class PagedAttentionDesc(C.Structure):
+    _fields_ = [("cache", KvCache), ("num_seqs", C.c_int32), ("q_heads", C.c_int32), ("q_dt", C.c_int32), ("out_dt", C.c_int32),
+                ("q_stride", C.c_int64 * 2), ("out_stride", C.c_int64 * 2), ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+                ("page_table", C.c_void_p), ("page_table_ld", C.c_int64), ("max_pages", C.c_int32), ("window", C.c_int32),
+                ("seq_lens", C.c_void_p), ("sinks", C.c_void_p), ("scale", C.c_double), ("softcap", C.c_float), ("reserved", C.c_int32)]
+
+
+GATE_SCORE = dict(softmax=0, sigmoid=1)
+GROUP_SCORE = dict(max=0, top2=1)
+
+
+class MoeGateDesc(C.Structure):
+    _fields_ = [("num_tokens", C.c_int32), ("num_experts", C.c_int32), ("topk", C.c_int32), ("score", C.c_int32), ("num_groups", C.c_int32),
+                ("topk_groups", C.c_int32), ("group_score", C.c_int32), ("renorm", C.c_int32), ("scale", C.c_float), ("logits_dt", C.c_int32),
+                ("ld", C.c_int64), ("logits", C.c_void_p), ("bias", C.c_void_p), ("ids", C.c_void_p), ("weights", C.c_void_p),
+                ("expert_counts", C.c_void_p), ("slot_to_row", C.c_void_p)]
+
+
 class EpConfig(C.Structure):
     _fields_ = [("world", C.c_int32), ("rank", C.c_int32), ("num_experts", C.c_int32), ("num_shared", C.c_int32),
                 ("topk", C.c_int32), ("max_tokens", C.c_int32), ("K", C.c_int32), ("I", C.c_int32), ("H", C.c_int32),
@@ -95,7 +127,8 @@ EXPORTS = ["b200dnn_last_error", "b200dnn_version", "b200dnn_device_count", "b20
            "b200dnn_moe_weighted_reduce_rows", "b200dnn_ep_create", "b200dnn_ep_destroy", "b200dnn_ep_local_expert_count",
            "b200dnn_ep_set_experts", "b200dnn_ep_nccl_unique_id", "b200dnn_ep_connect_nccl", "b200dnn_ep_connect_local",
            "b200dnn_moe_layer_ep", "b200dnn_moe_layer_ep_local", "b200dnn_ep_rows_per_rank", "b200dnn_ep_status",
-           "b200dnn_phase_timing", "b200dnn_phase_times", "b200dnn_measure_int8_peak", "b200dnn_normalization", "b200dnn_sdpa"]
+           "b200dnn_phase_timing", "b200dnn_phase_times", "b200dnn_measure_int8_peak", "b200dnn_normalization", "b200dnn_sdpa",
+           "b200dnn_kv_append", "b200dnn_paged_attention", "b200dnn_moe_gate"]
 
 if not os.path.exists(LIB_PATH):
     raise ImportError(
@@ -123,6 +156,9 @@ lib.b200dnn_moe_weighted_reduce.argtypes = [vp, vp, i32, i32, i32, i32, i32, vp,
 lib.b200dnn_quant_per_token_asym.argtypes = [vp, i32, i64, i64, i64, vp, i64, vp, vp, vp]
 lib.b200dnn_normalization.argtypes = [C.POINTER(NormDesc), C.c_void_p]
 lib.b200dnn_sdpa.argtypes = [C.POINTER(SdpaDesc), C.c_void_p]
+lib.b200dnn_kv_append.argtypes = [C.POINTER(KvAppendDesc), C.c_void_p]
+lib.b200dnn_paged_attention.argtypes = [C.POINTER(PagedAttentionDesc), C.c_void_p]
+lib.b200dnn_moe_gate.argtypes = [C.POINTER(MoeGateDesc), C.c_void_p]
 lib.b200dnn_nshard_range.argtypes = [i64, i32, i32, C.POINTER(i64), C.POINTER(i64), C.POINTER(i32)]
 lib.b200dnn_nshard_create.argtypes = [i32, i32, vp, vp, C.POINTER(vp)]
 lib.b200dnn_nshard_destroy.argtypes = [vp]
@@ -258,3 +294,123 @@ def make_matmul(M, N, K, src, weight, dst, *, src_dt, dst_dt, lda=None, ldb=None
 
 def matmul(desc, stream=None):
     return lib.b200dnn_matmul(C.byref(desc), stream)
+
+
+def strides(buf):
+    """Strides of a numpy array or torch tensor, in elements."""
+    return tuple(buf.stride()) if hasattr(buf, "stride") else tuple(s // buf.itemsize for s in buf.strides)
+
+
+def _dense(what, buf, axis=-1):
+    if buf.shape[axis] > 1 and strides(buf)[axis] != 1:
+        raise ValueError("%s: the last dimension must be dense" % what)
+
+
+def make_kv_cache(key, value, key_scale=None, value_scale=None):
+    """Descriptor of a paged cache from views [page, token, head, dim] of its keys and values in any storage order (bf16, or s8 with
+    scales [page, token, head], both scale arrays laid out alike)."""
+    if tuple(key.shape) != tuple(value.shape) or len(key.shape) != 4 or dt_of(key) != dt_of(value):
+        raise ValueError("kv cache: keys and values must be [page, token, head, dim] arrays of one shape and type")
+    c = KvCache()
+    c.keep = (key, value, key_scale, value_scale)      # (a descriptor holds addresses: its buffers live as long as it does)
+    c.dt = dt_of(key)
+    c.num_pages, c.page_size, c.kv_heads, c.head_dim = key.shape
+    for name, buf in (("key", key), ("value", value)):
+        _dense("kv cache", buf)
+        setattr(c, name, ptr(buf))
+        setattr(c, name + "_stride", (C.c_int64 * 3)(*strides(buf)[:3]))
+    if key_scale is not None or value_scale is not None:
+        for buf in (key_scale, value_scale):
+            if buf is None or tuple(buf.shape) != tuple(key.shape[:3]) or dt_of(buf) != DT["f32"] or strides(buf) != strides(key_scale):
+                raise ValueError("kv cache: scales must be two f32 [page, token, head] arrays with the same strides")
+        c.key_scale, c.value_scale = ptr(key_scale), ptr(value_scale)
+        c.scale_stride = (C.c_int64 * 3)(*strides(key_scale))
+    return c
+
+
+def _index(what, buf, dt, shape):
+    name = str(buf.dtype).replace("torch.", "")
+    if name != dt or tuple(buf.shape) != tuple(shape) or (len(shape) and buf.shape[-1] > 1 and strides(buf)[-1] != 1):
+        raise ValueError("%s must be a dense %s array of shape %s" % (what, dt, tuple(shape)))
+    return ptr(buf)
+
+
+def _ld(buf):
+    return strides(buf)[0] if buf.shape[0] > 1 else buf.shape[1]
+
+
+def make_kv_append(cache, k, v, slots, q=None, q_out=None, positions=None, cos=None, sin=None, interleaved=False):
+    """k, v [token, kv head, dim], q and q_out [token, query head, dim] (q_out defaults to q: rotated in place), slots int64 [token];
+    positions int32 [token] and cos, sin f32 [row, rotary_dim / 2] where the rows are rotated."""
+    T = int(k.shape[0])
+    d = KvAppendDesc()
+    d.keep = (cache, k, v, slots, q, q_out, positions, cos, sin)
+    d.cache, d.num_tokens, d.dt, d.interleaved = cache, T, dt_of(k), int(interleaved)
+    heads = [("k", k), ("v", v)]
+    if q is not None:
+        d.q_heads = q.shape[1]
+        heads += [("q", q), ("q_out", q if q_out is None else q_out)]
+    for name, buf in heads:
+        want = (T, cache.kv_heads if name in "kv" else d.q_heads, cache.head_dim)
+        if tuple(buf.shape) != want or dt_of(buf) != d.dt:
+            raise ValueError("kv append: %s must be a %s array of k's type" % (name, want))
+        _dense("kv append: " + name, buf)
+        setattr(d, name, ptr(buf))
+        setattr(d, name + "_stride", (C.c_int64 * 2)(*strides(buf)[:2]))
+    d.slots = _index("kv append: slots", slots, "int64", (T,))
+    if positions is not None:
+        if cos is None or sin is None or tuple(cos.shape) != tuple(sin.shape) or strides(cos) != strides(sin) or dt_of(cos) != DT["f32"] or dt_of(sin) != DT["f32"]:
+            raise ValueError("kv append: cos and sin must be f32 arrays of one layout")
+        _dense("kv append: cos", cos)
+        d.positions = _index("kv append: positions", positions, "int32", (T,))
+        d.rotary_dim, d.table_rows, d.table_ld = 2 * cos.shape[1], cos.shape[0], _ld(cos)
+        d.cos_table, d.sin_table = ptr(cos), ptr(sin)
+    return d
+
+
+def make_paged_attention(cache, q, out, page_table, seq_lens, scale=0.0, window=0, softcap=0.0, sinks=None, lse=None):
+    """q, out [sequence, query head, dim], page_table int32 [sequence, pages], seq_lens int32 [sequence]; sinks f32 [query head], lse f32
+    [sequence, query head]."""
+    B, H = int(q.shape[0]), int(q.shape[1])
+    d = PagedAttentionDesc()
+    d.keep = (cache, q, out, page_table, seq_lens, sinks, lse)
+    d.cache, d.num_seqs, d.q_heads = cache, B, H
+    for name, buf in (("q", q), ("out", out)):
+        if tuple(buf.shape) != (B, H, cache.head_dim):
+            raise ValueError("paged attention: %s must be %s" % (name, (B, H, cache.head_dim)))
+        _dense("paged attention: " + name, buf)
+        setattr(d, name, ptr(buf))
+        setattr(d, name + "_dt", dt_of(buf))
+        setattr(d, name + "_stride", (C.c_int64 * 2)(*strides(buf)[:2]))
+    d.page_table = _index("paged attention: page_table", page_table, "int32", (B, page_table.shape[1]))
+    d.max_pages, d.page_table_ld = page_table.shape[1], _ld(page_table)
+    d.seq_lens = _index("paged attention: seq_lens", seq_lens, "int32", (B,))
+    d.scale, d.window, d.softcap = scale, window, softcap
+    if sinks is not None:
+        d.sinks = _index("paged attention: sinks", sinks, "float32", (H,))
+    if lse is not None:
+        if strides(lse)[0] != H and B > 1:
+            raise ValueError("paged attention: lse must be dense")
+        d.lse = _index("paged attention: lse", lse, "float32", (B, H))
+    return d
+
+
+def make_moe_gate(logits, topk, ids, weights=None, *, bias=None, score="softmax", num_groups=1, topk_groups=1, group_score="max", renorm=True,
+                  scale=1.0, expert_counts=None, slot_to_row=None):
+    """logits [token, expert] f32 or bf16; ids int32 and weights f32 [token, topk], bias f32 and expert_counts int32 [expert],
+    slot_to_row int32 [token, topk]."""
+    T, E = logits.shape
+    d = MoeGateDesc()
+    d.keep = (logits, ids, weights, bias, expert_counts, slot_to_row)
+    d.num_tokens, d.num_experts, d.topk = T, E, topk
+    d.score, d.num_groups, d.topk_groups, d.group_score = GATE_SCORE[score], num_groups, topk_groups, GROUP_SCORE[group_score]
+    d.renorm, d.scale, d.logits_dt = int(renorm), scale, dt_of(logits)
+    _dense("moe gate: logits", logits)
+    d.ld, d.logits = _ld(logits), ptr(logits)
+    for name, buf, dt, shape in (("ids", ids, "int32", (T, topk)), ("weights", weights, "float32", (T, topk)), ("bias", bias, "float32", (E,)),
+                                 ("expert_counts", expert_counts, "int32", (E,)), ("slot_to_row", slot_to_row, "int32", (T, topk))):
+        if buf is not None:
+            if len(shape) == 2 and T > 1 and strides(buf)[0] != topk:
+                raise ValueError("moe gate: %s must be dense" % name)
+            setattr(d, name, _index("moe gate: " + name, buf, dt, shape))
+    return d

@@ -1,0 +1,173 @@
+// Entry points of the paged key/value cache: b200dnn_kv_append and b200dnn_paged_attention (checks, staging, launches).
+#include <cmath>
+#include <cuda_bf16.h>
+#include "runtime.cuh"
+#include "paged_append.cuh"
+#include "paged_attention.cuh"
+
+namespace b200 {
+
+namespace {
+
+template <typename... P>
+int32_t launch(void (*kern)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st, const P &...args) {
+  if (smem > 48 * 1024) B2_TRY(ensure_max_smem((const void *)kern, (int)smem));
+  B2_TRY(launch_pdl(kern, grid, threads, smem, st, true, args...));
+  B2_LAUNCHED();
+  return B200DNN_SUCCESS;
+}
+
+// Bytes from the first element to behind the last one of rows [n0][n1][dim]
+size_t span2(int64_t n0, int64_t n1, int64_t dim, const int64_t (&s)[2], int32_t dt) {
+  return n0 <= 0 || n1 <= 0 ? 0 : (size_t)((n0 - 1) * s[0] + (n1 - 1) * s[1] + dim) * dt_size(dt);
+}
+// Strides of one row from the next: rows do not overlap (an extent of one takes any stride)
+bool rows_apart(int64_t n0, int64_t n1, int64_t dim, const int64_t (&s)[2]) {
+  return (n0 <= 1 || s[0] >= dim) && (n1 <= 1 || s[1] >= dim) && s[0] < (1ll << 40) && s[1] < (1ll << 40);
+}
+
+int32_t check_cache(const char *who, const b200dnn_kv_cache_t &c) {
+  B2_CHECK(c.dt == B200DNN_BF16 || c.dt == B200DNN_S8, B200DNN_UNIMPLEMENTED, "%s: the cache is bf16 or s8 (dt %d)", who, c.dt);
+  B2_CHECK(c.page_size > 0 && c.kv_heads > 0 && c.head_dim > 0 && c.num_pages > 0, B200DNN_FAILURE, "%s: page_size, kv_heads, head_dim and num_pages must be > 0", who);
+  B2_CHECK(c.head_dim <= 256, B200DNN_UNIMPLEMENTED, "%s: head_dim up to 256 (%d)", who, c.head_dim);
+  B2_CHECK(c.page_size < (1 << 20) && c.num_pages < (1ll << 31) && c.kv_heads < (1 << 16), B200DNN_UNIMPLEMENTED, "%s: sizes beyond the cache's limits", who);
+  B2_CHECK(c.key && c.value, B200DNN_FAILURE, "%s: the cache's key or value pointer is null", who);
+  const int64_t n[3] = {c.num_pages, c.page_size, c.kv_heads};
+  for (int i = 0; i < 3; ++i) {
+    B2_CHECK(n[i] == 1 || (c.key_stride[i] >= c.head_dim && c.value_stride[i] >= c.head_dim), B200DNN_FAILURE, "%s: the cache's rows overlap (stride %d)", who, i);
+    B2_CHECK(c.key_stride[i] < (1ll << 31) && c.value_stride[i] < (1ll << 31) && c.key_stride[i] >= 0 && c.value_stride[i] >= 0, B200DNN_UNIMPLEMENTED,
+             "%s: cache strides are below 2^31 elements", who);
+  }
+  if (c.dt == B200DNN_S8) {
+    B2_CHECK(c.key_scale && c.value_scale, B200DNN_FAILURE, "%s: an s8 cache needs key_scale and value_scale", who);
+    for (int i = 0; i < 3; ++i)
+      B2_CHECK((n[i] == 1 || c.scale_stride[i] >= 1) && c.scale_stride[i] >= 0 && c.scale_stride[i] < (1ll << 31), B200DNN_FAILURE, "%s: bad scale stride %d", who, i);
+  }
+  return B200DNN_SUCCESS;
+}
+
+// The kernels write to the cache where it lies, and memory of another device may be out of their reach.
+int32_t check_here(const char *who, const char *what, const void *p) {
+  cudaPointerAttributes at;
+  if (cudaPointerGetAttributes(&at, p) != cudaSuccess) { cudaGetLastError(); at.type = cudaMemoryTypeUnregistered; }
+  B2_CHECK(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, B200DNN_UNIMPLEMENTED, "%s: %s must be device memory", who, what);
+  B2_CHECK(at.type == cudaMemoryTypeManaged || at.device == rt().shared->dev, B200DNN_FAILURE, "%s: %s lies on device %d, the current one is %d", who, what, at.device,
+           rt().shared->dev);
+  return B200DNN_SUCCESS;
+}
+int32_t check_cache_here(const char *who, const b200dnn_kv_cache_t &c) {
+  B2_TRY(check_here(who, "the cache", c.key));
+  B2_TRY(check_here(who, "the cache", c.value));
+  if (c.dt == B200DNN_S8) {
+    B2_TRY(check_here(who, "the cache's scales", c.key_scale));
+    B2_TRY(check_here(who, "the cache's scales", c.value_scale));
+  }
+  return B200DNN_SUCCESS;
+}
+
+}  // namespace
+
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int32_t b200dnn_kv_append(const b200dnn_kv_append_t *d, void *stream) {
+  const char *who = "kv append";
+  B2_CHECK(d, B200DNN_FAILURE, "null descriptor");
+  const b200dnn_kv_cache_t &c = d->cache;
+  B2_TRY(check_cache(who, c));
+  const int64_t T = d->num_tokens;
+  B2_CHECK(T >= 0 && d->q_heads >= 0, B200DNN_FAILURE, "%s: num_tokens and q_heads must be >= 0", who);
+  B2_CHECK(d->dt == B200DNN_BF16 || d->dt == B200DNN_F32, B200DNN_UNIMPLEMENTED, "%s: q, k and v are bf16 or f32 (dt %d)", who, d->dt);
+  B2_CHECK(d->rotary_dim >= 0 && d->rotary_dim % 2 == 0 && d->rotary_dim <= c.head_dim, B200DNN_FAILURE, "%s: rotary_dim must be even and at most head_dim (%d)", who, d->rotary_dim);
+  if (T == 0) return B200DNN_SUCCESS;
+  const int R = d->q_heads + 2 * c.kv_heads;
+  B2_CHECK(T < (1ll << 31) && d->q_heads < (1 << 16) && T * R < (1ll << 34), B200DNN_UNIMPLEMENTED, "%s: too many rows in one call", who);
+  B2_CHECK(d->k && d->v && d->slots, B200DNN_FAILURE, "%s: k, v or slots is null", who);
+  B2_CHECK(d->q_heads == 0 || (d->q && d->q_out), B200DNN_FAILURE, "%s: q or q_out is null", who);
+  B2_CHECK(rows_apart(T, c.kv_heads, c.head_dim, d->k_stride) && rows_apart(T, c.kv_heads, c.head_dim, d->v_stride) &&
+               (d->q_heads == 0 || (rows_apart(T, d->q_heads, c.head_dim, d->q_stride) && rows_apart(T, d->q_heads, c.head_dim, d->q_out_stride))),
+           B200DNN_FAILURE, "%s: token and head strides must be at least head_dim", who);
+  B2_CHECK(d->q_heads == 0 || d->q != d->q_out || ((T == 1 || d->q_stride[0] == d->q_out_stride[0]) && (d->q_heads == 1 || d->q_stride[1] == d->q_out_stride[1])), B200DNN_FAILURE,
+           "%s: q rotated in place must keep its strides", who);
+  if (d->rotary_dim > 0)
+    B2_CHECK(d->positions && d->cos_table && d->sin_table && d->table_rows > 0 && d->table_ld >= d->rotary_dim / 2 && d->table_ld < (1ll << 31), B200DNN_FAILURE,
+             "%s: a rotation needs positions and tables of at least rotary_dim / 2 columns", who);
+  B2_ENTER(stream);
+  B2_TRY(check_cache_here(who, c));
+  AppendArgs a{};
+  const size_t table_bytes = d->rotary_dim ? (size_t)((d->table_rows - 1) * d->table_ld + d->rotary_dim / 2) * 4 : 0;
+  Staged q_out{};
+  const void *p;
+  B2_TRY(stage_in(d->k, span2(T, c.kv_heads, c.head_dim, d->k_stride, d->dt), st, &a.k));
+  B2_TRY(stage_in(d->v, span2(T, c.kv_heads, c.head_dim, d->v_stride, d->dt), st, &a.v));
+  B2_TRY(stage_in(d->slots, (size_t)T * 8, st, &p)); a.slots = (const int64_t *)p;
+  if (d->q_heads) {
+    B2_TRY(stage_in(d->q, span2(T, d->q_heads, c.head_dim, d->q_stride, d->dt), st, &a.q));
+    B2_TRY(stage_out(d->q_out, span2(T, d->q_heads, c.head_dim, d->q_out_stride, d->dt), st, &q_out, true));
+    a.q_out = q_out.dev;
+  }
+  if (d->rotary_dim) {
+    B2_TRY(stage_in(d->positions, (size_t)T * 4, st, &p)); a.positions = (const int32_t *)p;
+    B2_TRY(stage_in(d->cos_table, table_bytes, st, &p)); a.cos_t = (const float *)p;
+    B2_TRY(stage_in(d->sin_table, table_bytes, st, &p)); a.sin_t = (const float *)p;
+  }
+  for (int i = 0; i < 2; ++i) { a.qs[i] = d->q_stride[i]; a.ks[i] = d->k_stride[i]; a.vs[i] = d->v_stride[i]; a.os[i] = d->q_out_stride[i]; }
+  for (int i = 0; i < 3; ++i) { a.ck[i] = c.key_stride[i]; a.cv[i] = c.value_stride[i]; a.cs[i] = c.scale_stride[i]; }
+  a.key = c.key; a.value = c.value; a.key_scale = c.key_scale; a.value_scale = c.value_scale;
+  a.table_rows = d->table_rows; a.table_ld = d->table_ld;
+  a.n_slots = c.num_pages * c.page_size; a.T = T;
+  a.page_size = c.page_size; a.q_heads = d->q_heads; a.kv_heads = c.kv_heads; a.dim = c.head_dim; a.rot = d->rotary_dim; a.interleaved = d->interleaved ? 1 : 0;
+  a.status = rt().status;
+  const unsigned grid = (unsigned)((T * R + 7) / 8);
+  const bool f32 = d->dt == B200DNN_F32, s8 = c.dt == B200DNN_S8;
+  B2_TRY(f32 ? (s8 ? launch(append_rows_kernel<float, true>, grid, 256, 0, st, a) : launch(append_rows_kernel<float, false>, grid, 256, 0, st, a))
+             : (s8 ? launch(append_rows_kernel<__nv_bfloat16, true>, grid, 256, 0, st, a) : launch(append_rows_kernel<__nv_bfloat16, false>, grid, 256, 0, st, a)));
+  return finish_out({&q_out}, st);
+}
+
+extern "C" int32_t b200dnn_paged_attention(const b200dnn_paged_attention_t *d, void *stream) {
+  const char *who = "paged attention";
+  B2_CHECK(d, B200DNN_FAILURE, "null descriptor");
+  const b200dnn_kv_cache_t &c = d->cache;
+  B2_TRY(check_cache(who, c));
+  B2_CHECK(d->num_seqs >= 0, B200DNN_FAILURE, "%s: num_seqs must be >= 0", who);
+  B2_CHECK(d->q_heads > 0 && d->q_heads % c.kv_heads == 0, B200DNN_FAILURE, "%s: q_heads (%d) must be a multiple of kv_heads (%d)", who, d->q_heads, c.kv_heads);
+  B2_CHECK(d->q_dt == B200DNN_BF16, B200DNN_UNIMPLEMENTED, "%s: queries are bf16 (dt %d)", who, d->q_dt);
+  B2_CHECK(d->out_dt == B200DNN_BF16 || d->out_dt == B200DNN_F32, B200DNN_UNIMPLEMENTED, "%s: the output is bf16 or f32 (dt %d)", who, d->out_dt);
+  B2_CHECK(d->window >= 0, B200DNN_FAILURE, "%s: window must be >= 0", who);
+  B2_CHECK(d->softcap >= 0.f && std::isfinite(d->softcap), B200DNN_FAILURE, "%s: softcap must be finite and >= 0", who);
+  B2_CHECK(std::isfinite(d->scale), B200DNN_FAILURE, "%s: scale must be finite", who);
+  if (d->num_seqs == 0) return B200DNN_SUCCESS;
+  B2_CHECK(d->max_pages > 0 && d->page_table_ld >= d->max_pages && d->page_table_ld < (1ll << 31), B200DNN_FAILURE, "%s: page_table_ld must be at least max_pages > 0", who);
+  B2_CHECK(d->q && d->out && d->page_table && d->seq_lens, B200DNN_FAILURE, "%s: q, out, page_table or seq_lens is null", who);
+  const int64_t B = d->num_seqs;
+  B2_CHECK(rows_apart(B, d->q_heads, c.head_dim, d->q_stride) && rows_apart(B, d->q_heads, c.head_dim, d->out_stride), B200DNN_FAILURE,
+           "%s: sequence and head strides must be at least head_dim", who);
+  B2_CHECK(B * d->q_heads < (1ll << 31), B200DNN_UNIMPLEMENTED, "%s: too many rows in one call", who);
+  B2_CHECK(d->q != d->out, B200DNN_FAILURE, "%s: out must not overlap q", who);
+  B2_ENTER(stream);
+  B2_TRY(check_cache_here(who, c));
+  PagedArgs a{};
+  const void *p;
+  Staged out{}, lse{};
+  B2_TRY(stage_in(d->q, span2(B, d->q_heads, c.head_dim, d->q_stride, d->q_dt), st, &p)); a.q = (const uint16_t *)p;
+  B2_TRY(stage_in(d->page_table, (size_t)((B - 1) * d->page_table_ld + d->max_pages) * 4, st, &p)); a.table = (const int32_t *)p;
+  B2_TRY(stage_in(d->seq_lens, (size_t)B * 4, st, &p)); a.lens = (const int32_t *)p;
+  if (d->sinks) { B2_TRY(stage_in(d->sinks, (size_t)d->q_heads * 4, st, &p)); a.sinks = (const float *)p; }
+  B2_TRY(stage_out(d->out, span2(B, d->q_heads, c.head_dim, d->out_stride, d->out_dt), st, &out, true));
+  if (d->lse) B2_TRY(stage_out(d->lse, (size_t)B * d->q_heads * 4, st, &lse, true));
+  a.out = out.dev; a.lse = d->lse ? (float *)lse.dev : nullptr;
+  for (int i = 0; i < 2; ++i) { a.qs[i] = d->q_stride[i]; a.os[i] = d->out_stride[i]; }
+  for (int i = 0; i < 3; ++i) { a.ck[i] = c.key_stride[i]; a.cv[i] = c.value_stride[i]; a.cs[i] = c.scale_stride[i]; }
+  a.key = c.key; a.value = c.value; a.key_scale = c.key_scale; a.value_scale = c.value_scale;
+  a.table_ld = d->page_table_ld; a.n_pages = c.num_pages; a.n_keys = (int64_t)d->max_pages * c.page_size;
+  a.B = (int)B; a.q_heads = d->q_heads; a.kv_heads = c.kv_heads; a.group = d->q_heads / c.kv_heads; a.dim = c.head_dim; a.page_size = c.page_size; a.window = d->window;
+  a.scale = d->scale == 0.0 ? 1.0f / std::sqrt((float)c.head_dim) : (float)d->scale;
+  a.softcap = d->softcap;
+  a.status = rt().status;
+  const int f32 = d->out_dt == B200DNN_F32;
+  const unsigned grid = (unsigned)(B * d->q_heads);
+  B2_TRY(c.dt == B200DNN_S8 ? launch(paged_rows_kernel<true>, grid, 32 * kPagedRowWarps, 0, st, a, f32) : launch(paged_rows_kernel<false>, grid, 32 * kPagedRowWarps, 0, st, a, f32));
+  return finish_out({&out, &lse}, st);
+}

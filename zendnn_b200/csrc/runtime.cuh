@@ -376,6 +376,9 @@ struct CallGuard {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream_ptr);    \
   B2_TRY(guard__.enter(st))
 
+// Not a wait: a slot, position, page or length that a kernel of the paged cache met and made no access with.
+constexpr int32_t kStatusIndex = 41;
+
 // After the stream has been drained: did a kernel of this context give up on one of its bounded waits since the last
 // check?  The kernels write the code into mapped pinned memory, so the check is one host load.
 inline int32_t read_status() {
@@ -383,6 +386,7 @@ inline int32_t read_status() {
   const int32_t code = *R.status_host;
   if (code != 0) {
     *R.status_host = 0;
+    if (code == kStatusIndex) return fail(B200DNN_FAILURE, "an index array on the device held an entry out of range (code %d)", code);
     return fail(B200DNN_FAILURE, "a GEMM kernel gave up waiting on a barrier (code %d)", code);
   }
   return B200DNN_SUCCESS;
