@@ -1,4 +1,5 @@
 // Entry points of the paged key/value cache: b200dnn_kv_append and b200dnn_paged_attention (checks, staging, launches).
+#include <algorithm>
 #include <cmath>
 #include <cuda_bf16.h>
 #include "runtime.cuh"
@@ -63,6 +64,48 @@ int32_t check_cache_here(const char *who, const b200dnn_kv_cache_t &c) {
     B2_TRY(check_here(who, "the cache's scales", c.value_scale));
   }
   return B200DNN_SUCCESS;
+}
+
+// The split form, where rows are 16-byte vectors: false when the call does not fit.
+template <bool S8, int DP, int NT>
+int32_t launch_split(PagedSplitArgs &s, cudaStream_t st) {
+  auto kern = paged_split_kernel<S8, DP, NT>;
+  constexpr size_t smem = paged_smem<S8, DP, NT>();
+  const int resident = (int)std::min<size_t>(DP <= 128 ? 3 : 1, (size_t)(227 * 1024) / (smem + 2048));
+  const int64_t most = (int64_t)s.a.B * s.rows * ((s.a.n_keys + kPagedUnit - 1) / kPagedUnit);
+  if (most >= (1ll << 31)) return B200DNN_UNIMPLEMENTED;
+  const unsigned grid = (unsigned)std::min<int64_t>(most, (int64_t)resident * rt().sm_count);
+  s.part_o = (float *)rt().ws.alloc((size_t)grid * 2 * 8 * NT * DP * 4);
+  s.part_ml = (float2 *)rt().ws.alloc((size_t)grid * 2 * 8 * NT * 8);
+  B2_CHECK(s.part_o && s.part_ml, B200DNN_FAILURE, "workspace allocation failed");
+  s.counters = rt().counters;
+  return launch(kern, grid, 32 * kPagedWarps, smem, st, s);
+}
+template <bool S8, int DP>
+int32_t launch_split_heads(PagedSplitArgs &s, cudaStream_t st) {
+  const bool two = s.a.group > 8;
+  s.tiles = (s.a.group + (two ? 16 : 8) - 1) / (two ? 16 : 8);
+  s.rows = s.a.kv_heads * s.tiles;
+  return two ? launch_split<S8, DP, 2>(s, st) : launch_split<S8, DP, 1>(s, st);
+}
+template <bool S8>
+int32_t paged_split(const PagedArgs &a, int out_f32, cudaStream_t st) {
+  const int vec = S8 ? 16 : 8;          // elements of 16 bytes
+  auto rows_vec = [&](const void *p, const int64_t (&s)[3]) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s[0] % vec == 0 && (a.page_size == 1 || s[1] % vec == 0) && (a.kv_heads == 1 || s[2] % vec == 0);
+  };
+  if (a.dim % vec != 0 || !rows_vec(a.key, a.ck) || !rows_vec(a.value, a.cv)) return B200DNN_UNIMPLEMENTED;
+  PagedSplitArgs s{};
+  s.a = a;
+  s.out_f32 = out_f32;
+  s.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.qs[0] % 8 == 0 && a.qs[1] % 8 == 0;
+  const int ov = out_f32 ? 4 : 8;
+  s.out_vec = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.os[0] % ov == 0 && a.os[1] % ov == 0;
+  s.min_units = 1;
+  if (a.dim <= 64) return launch_split_heads<S8, 64>(s, st);
+  if (a.dim <= 128) return launch_split_heads<S8, 128>(s, st);
+  if (a.dim <= 192) return launch_split_heads<S8, 192>(s, st);
+  return launch_split_heads<S8, 256>(s, st);
 }
 
 }  // namespace
@@ -167,6 +210,8 @@ extern "C" int32_t b200dnn_paged_attention(const b200dnn_paged_attention_t *d, v
   a.softcap = d->softcap;
   a.status = rt().status;
   const int f32 = d->out_dt == B200DNN_F32;
+  const int32_t rc = c.dt == B200DNN_S8 ? paged_split<true>(a, f32, st) : paged_split<false>(a, f32, st);
+  if (rc != B200DNN_UNIMPLEMENTED) { B2_TRY(rc); return finish_out({&out, &lse}, st); }
   const unsigned grid = (unsigned)(B * d->q_heads);
   B2_TRY(c.dt == B200DNN_S8 ? launch(paged_rows_kernel<true>, grid, 32 * kPagedRowWarps, 0, st, a, f32) : launch(paged_rows_kernel<false>, grid, 32 * kPagedRowWarps, 0, st, a, f32));
   return finish_out({&out, &lse}, st);

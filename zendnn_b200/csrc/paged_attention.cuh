@@ -94,4 +94,595 @@ __global__ void __launch_bounds__(32 * kPagedRowWarps) paged_rows_kernel(const P
   if (a.lse && threadIdx.x == 0) a.lse[(int64_t)i * a.q_heads + h] = frame + logf(total);
 }
 
+
+// ---------------------------------------------------------------------------------------------------------------------------------------------
+// The split form: rows of 16-byte vectors.
+//
+// Work.  A row is one sequence and one tile of up to 8 NT query heads of a key head; its visible keys come in units of 64.  The units of all rows, one row after the other, are
+// dealt out evenly: CTA c takes units [c per, (c + 1) per) of a grid that fills the device once, whatever the lengths are (they are on the device).  A row that lies in one CTA is finished
+// there; of the others every CTA leaves a partial result (maximum, sum, unnormalised output), and the last one to arrive joins them, in order.
+//
+// A warp takes 16 keys of a unit at a time, by itself: every lane copies the 16-byte pieces of keys and values that it will multiply (cp.async, `ST` steps ahead,
+// across the ends of rows), and reads back nothing but these, so the ring needs no barrier and no swizzle.  The products run on mma.m16n8k16 with the keys as the 16 rows:
+//   S^T[key][head] = K Q^T     lane (r, c) = (lane / 4, lane % 4) holds pieces of the keys r and r + 8; which element of the head dimension is which index
+//                              of the product does not matter as long as Q agrees, so a piece of 8 elements is the operand of two products as it lies
+//   O^T[dim][head] = V^T P^T   lane (r, c) holds the same 8 (s8: 16) dims of the keys 2c, 2c + 1, 2c + 8, 2c + 9: a byte permutation pairs two keys of one dim
+// P^T comes from S^T by transposing 8 x 8 blocks (movmatrix).  Statistics of heads 2c and 2c + 1 and their columns of O^T are in the same lanes.
+// Tensor work is a fifth of what the memory leaves time for, so bf16 tiles of 16 x 8 serve: the call is bound by the bytes of the cache.
+//
+// Probabilities enter the second product as the sum of two bf16 (2^-17 relative): one alone would cost as much again as the rounding of a bf16 output, and an f32
+// output most of its digits.  The row sum has them unrounded.  s8 codes are exact in bf16; a key's scale multiplies its scores, a value's scale its probability.
+// The running maximum moves only when a score passes it by more than 2^8: probabilities are then at most 256, and few steps meet the exchange.
+
+constexpr float kPagedLog2e = 1.44269504088896340736f;
+constexpr int kPagedWarps = 4, kPagedUnit = 16 * kPagedWarps;
+constexpr float kPagedReach = 8.0f;
+
+struct PagedSplitArgs {
+  PagedArgs a;
+  int tiles;                       // head tiles of a key head
+  int rows;                        // rows of a sequence: kv_heads * tiles
+  int out_f32, q_vec, out_vec;     // 16-byte rows of q and out
+  int min_units;                   // fewest units of a CTA
+  float *part_o; float2 *part_ml;  // partial results: two slots a CTA
+  uint32_t *counters;              // one a CTA, zero between launches
+};
+
+__device__ __forceinline__ float paged_exp2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+template <int BYTES>
+__device__ __forceinline__ void paged_copy(uint32_t dst, const void *src, bool take) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(take ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ void paged_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void paged_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 paged_lds16(uint32_t p) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 paged_lds8(uint32_t p) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float paged_lds4(uint32_t p) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void paged_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t paged_transpose(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t paged_pack(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Two codes (the bytes of e that stand in front of 0x43) as bf16: 0x43bb without its sign bit is 128 + (the low seven bits), with nothing else 128 or 256.
+__device__ __forceinline__ uint32_t paged_codes(uint32_t e) {
+  const uint32_t x = e & 0xff7fff7fu, y = e & 0xff80ff80u;
+  uint32_t r;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  return r;
+}
+
+// What a CTA works on, one piece of a row after the other.
+struct PagedPieces {
+  int seq, row, off, n;            // sequence, row of it, first unit in the row, units of the row
+  int left;                        // units that the CTA still has, this piece included
+  int64_t lo, hi;                  // visible keys of the sequence
+  __device__ __forceinline__ int units() const { return min(n - off, left); }
+  __device__ __forceinline__ void sequence(const PagedArgs &a) {
+    if (!paged_range(a, seq, lo, hi)) lo = hi = 0;
+    n = (int)((hi - lo + kPagedUnit - 1) / kPagedUnit);
+  }
+  __device__ __forceinline__ void next(const PagedSplitArgs &s) {
+    const int u = units();
+    left -= u;
+    off += u;
+    if (off < n || left <= 0) return;
+    off = 0;
+    if (++row < s.rows) return;
+    row = 0;
+    for (n = 0; n == 0;) {                             // (there are units left, so there is a sequence with some)
+      if (++seq >= s.a.B) { left = 0; return; }
+      sequence(s.a);
+    }
+  }
+};
+
+template <bool S8, int DP> struct PagedRing {
+  static constexpr int kPieceK = DP * (S8 ? 1 : 2) / 64;                    // 16-byte pieces of a key that a lane copies
+  static constexpr int kWideV = S8 ? (DP % 128 == 0 ? 16 : 8) : 16;          // bytes of a value's pieces
+  static constexpr int kPieceV = DP * (S8 ? 1 : 2) / (8 * kWideV);
+  static constexpr int kK = 2 * kPieceK * 512, kV = 4 * kPieceV * 32 * kWideV, kScales = S8 ? 128 : 0;   // bytes of a step: keys, values, scales
+  static constexpr int kStep = kK + kV + kScales;
+  static constexpr int ST = (S8 ? 1 : 2) * DP <= 64 ? 8 : (S8 ? 1 : 2) * DP <= 128 ? 4 : 2;
+  static constexpr int kBytes = kPagedWarps * ST * kStep;
+};
+template <int DP, int NT> struct PagedJoin {
+  static constexpr int kRegs = NT * DP / 4;                                  // unnormalised outputs of a lane
+  static constexpr int kBytes = 2 * kRegs * 128;                             // two warps' in shared memory
+};
+template <bool S8, int DP, int NT> constexpr size_t paged_smem() { return PagedRing<S8, DP>::kBytes + PagedJoin<DP, NT>::kBytes; }
+
+template <bool S8, int DP, int NT>
+__global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 : 2) paged_split_kernel(const PagedSplitArgs s) {
+  using Ring = PagedRing<S8, DP>;
+  constexpr int ST = Ring::ST, KP = Ring::kPieceK, VP = Ring::kPieceV, VB = Ring::kWideV, REGS = PagedJoin<DP, NT>::kRegs;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float s_m[kPagedWarps][8 * NT], s_l[kPagedWarps][8 * NT];
+  __shared__ int s_scan[kPagedWarps], s_start[4];
+  __shared__ int s_last;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const PagedArgs &a = s.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
+  const float ninf = __int_as_float(0xff800000);
+
+  // ---- sequences without keys: zeros
+  for (int i = blockIdx.x; i < a.B; i += gridDim.x) {
+    if (a.lens[i] != 0) continue;
+    for (int x = tid; x < a.q_heads * a.dim; x += 32 * kPagedWarps) {
+      const int h = x / a.dim, d = x - h * a.dim;
+      const int64_t at = i * a.os[0] + h * a.os[1] + d;
+      if (s.out_f32) reinterpret_cast<float *>(a.out)[at] = 0.f; else reinterpret_cast<uint16_t *>(a.out)[at] = 0;
+    }
+    if (a.lse) for (int h = tid; h < a.q_heads; h += 32 * kPagedWarps) a.lse[(int64_t)i * a.q_heads + h] = ninf;
+  }
+
+  // ---- this CTA's units: every thread adds up the sequences of its stretch
+  PagedPieces ahead;
+  int per, first;
+  {
+    const int stretch = (a.B + 32 * kPagedWarps - 1) / (32 * kPagedWarps), b0 = min(a.B, tid * stretch), b1 = min(a.B, b0 + stretch);
+    int mine = 0;
+    for (ahead.seq = b0; ahead.seq < b1; ++ahead.seq) { ahead.sequence(a); mine += ahead.n * s.rows; }
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += v; }
+    if (lane == 31) s_scan[warp] = sum;
+    __syncthreads();
+    int before = sum - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < kPagedWarps; ++w) { if (w < warp) before += s_scan[w]; total += s_scan[w]; }
+    per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, s.min_units);
+    first = min(total, (int)blockIdx.x * per);
+    const int count = min(per, total - first);
+    if (count <= 0) return;
+    if (before <= first && first < before + mine) {
+      for (ahead.seq = b0; ahead.seq < b1; ++ahead.seq) {
+        ahead.sequence(a);
+        const int units = ahead.n * s.rows;
+        if (first < before + units) break;
+        before += units;
+      }
+      s_start[0] = ahead.seq;
+      s_start[1] = (first - before) / ahead.n;
+      s_start[2] = (first - before) % ahead.n;
+    }
+    __syncthreads();
+    ahead.seq = s_start[0]; ahead.row = s_start[1]; ahead.off = s_start[2]; ahead.left = count;
+    ahead.sequence(a);
+  }
+  PagedPieces now = ahead;
+
+  // ---- copies, ST steps ahead
+  const uint32_t ring = smem_u32(smem) + (uint32_t)warp * (ST * Ring::kStep);
+  int64_t next_key = ahead.lo + (int64_t)ahead.off * kPagedUnit + warp * 16, next_end = min(ahead.hi, ahead.lo + (int64_t)(ahead.off + ahead.units()) * kPagedUnit);
+  int slot_in = 0;
+  int64_t k_at = 0, v_at = 0, s_at = 0;       // of key lane % 16 of the step: where its rows lie
+  bool in_k[2], in_v[4];
+  auto find = [&]() {                         // the next step: its keys' places
+    while (ahead.left > 0 && next_key >= next_end) {
+      ahead.next(s);
+      if (ahead.left <= 0) break;
+      next_key = ahead.lo + (int64_t)ahead.off * kPagedUnit + warp * 16;
+      next_end = min(ahead.hi, ahead.lo + (int64_t)(ahead.off + ahead.units()) * kPagedUnit);
+    }
+    const bool any = ahead.left > 0;
+    const int64_t key = next_key + (lane & 15);
+    const bool take = any && key < next_end;
+    int64_t page = 0, off = 0;
+    if (take) {
+      const uint32_t column = (uint32_t)key / (uint32_t)a.page_size;
+      off = (uint32_t)key - column * (uint32_t)a.page_size;
+      page = paged_page(a, ahead.seq, column);
+    }
+    const int g = any ? ahead.row / s.tiles : 0;
+    k_at = page * a.ck[0] + off * a.ck[1] + g * a.ck[2];
+    v_at = page * a.cv[0] + off * a.cv[1] + g * a.cv[2];
+    if (S8) s_at = page * a.cs[0] + off * a.cs[1] + g * a.cs[2];
+    const unsigned taken = __ballot_sync(0xffffffffu, take);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) in_k[i] = (taken >> (r + 8 * i)) & 1u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) in_v[i] = (taken >> (2 * c + (i & 1) + 8 * (i >> 1))) & 1u;
+    return any;
+  };
+  auto copy_keys = [&]() {
+    const uint32_t to = ring + (uint32_t)slot_in * Ring::kStep + (uint32_t)lane * 16u;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t at = __shfl_sync(0xffffffffu, k_at, r + 8 * i);
+#pragma unroll
+      for (int t = 0; t < KP; ++t) {
+        const int d = S8 ? t * 64 + c * 16 : t * 32 + c * 8;
+        const bool in = in_k[i] && d < a.dim;
+        const uint8_t *p = reinterpret_cast<const uint8_t *>(a.key) + (in ? at + d : 0) * (S8 ? 1 : 2);
+        paged_copy<16>(to + (uint32_t)(i * KP + t) * 512u, p, in);
+      }
+    }
+    if (S8) {
+      const bool in = __shfl_sync(0xffffffffu, (int)(in_k[0] | (in_k[1] << 1)), (lane & 7) * 4) >> ((lane >> 3) & 1) & 1;      // key lane % 16
+      const float *p = (lane < 16 ? a.key_scale : a.value_scale) + (in ? s_at : 0);
+      paged_copy<4>(ring + (uint32_t)slot_in * Ring::kStep + Ring::kK + Ring::kV + (uint32_t)lane * 4u, p, in);
+    }
+  };
+  auto copy_values = [&]() {
+    const uint32_t to = ring + (uint32_t)slot_in * Ring::kStep + Ring::kK + (uint32_t)lane * VB;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t at = __shfl_sync(0xffffffffu, v_at, 2 * c + (i & 1) + 8 * (i >> 1));
+#pragma unroll
+      for (int t = 0; t < VP; ++t) {
+        const int d = t * (S8 ? 8 * VB : 64) + r * (S8 ? VB : 8);
+        const bool in = in_v[i] && d < a.dim;
+        const uint8_t *p = reinterpret_cast<const uint8_t *>(a.value) + (in ? at + d : 0) * (S8 ? 1 : 2);
+        paged_copy<VB>(to + (uint32_t)(t * 4 + i) * (32u * VB), p, in);
+      }
+    }
+  };
+  bool more = true;                           // (of this step: something to copy)
+  auto step_on = [&]() { slot_in = slot_in + 1 == ST ? 0 : slot_in + 1; next_key += kPagedUnit; };
+#pragma unroll 1
+  for (int i = 0; i < ST; ++i) {
+    more = find();
+    if (more) copy_keys();
+    paged_commit();
+    if (more) copy_values();
+    paged_commit();
+    step_on();
+  }
+
+  // ---- piece after piece
+  int slot = 0;
+  int global = first;                         // its first unit among all
+#pragma unroll 1
+  for (; now.left > 0;) {
+    const int units = now.units(), g = now.row / s.tiles, h0 = g * a.group + (now.row - g * s.tiles) * 8 * NT, heads = min(8 * NT, (g + 1) * a.group - h0);
+    // queries: the pieces that match the keys'
+    uint32_t q[NT][DP / 8];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const bool have = n * 8 + r < heads;
+      const uint16_t *qp = a.q + now.seq * a.qs[0] + (int64_t)(have ? h0 + n * 8 + r : h0) * a.qs[1];
+#pragma unroll
+      for (int t = 0; t < DP / 32; ++t) {
+        // eight elements: of piece t for bf16, of half t & 1 of piece t / 2 for s8
+        const int d = S8 ? (t >> 1) * 64 + c * 16 + (t & 1) * 8 : t * 32 + c * 8;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (have && d < a.dim) {
+          if (s.q_vec) v = *reinterpret_cast<const uint4 *>(qp + d);
+          else {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = (uint32_t)qp[d + 2 * e] | ((uint32_t)qp[d + 2 * e + 1] << 16);
+            v = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        q[n][4 * t] = v.x; q[n][4 * t + 1] = v.y; q[n][4 * t + 2] = v.z; q[n][4 * t + 3] = v.w;
+      }
+    }
+    float o[NT][DP / 16][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = ninf; l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.f;
+    }
+    const int64_t end = min(now.hi, now.lo + (int64_t)(now.off + units) * kPagedUnit);
+    const float to_log2 = a.scale * kPagedLog2e, cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f, cap_out = a.softcap * kPagedLog2e;
+#pragma unroll 1
+    for (int64_t key = now.lo + (int64_t)now.off * kPagedUnit + warp * 16; key < end; key += kPagedUnit) {
+      const uint32_t at = ring + (uint32_t)slot * Ring::kStep;
+      slot = slot + 1 == ST ? 0 : slot + 1;
+      // ---- scores
+      paged_wait<2 * ST - 1>();
+      float kscale[2] = {1.f, 1.f}, vscale[2] = {1.f, 1.f};
+      if (S8) {
+        __syncwarp();
+        const uint32_t sc = at + Ring::kK + Ring::kV;
+        kscale[0] = paged_lds4(sc + 4u * r); kscale[1] = paged_lds4(sc + 4u * r + 32u);
+        vscale[0] = paged_lds4(sc + 64u + 4u * r); vscale[1] = paged_lds4(sc + 96u + 4u * r);
+      }
+      float x[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
+#pragma unroll
+      for (int t = 0; t < KP; ++t) {
+        const uint4 k0 = paged_lds16(at + (uint32_t)lane * 16u + (uint32_t)t * 512u), k1 = paged_lds16(at + (uint32_t)lane * 16u + (uint32_t)(KP + t) * 512u);
+        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+        if constexpr (S8) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t a0 = paged_codes(__byte_perm(w0[e], 0x43434343u, 0x4140)), a2 = paged_codes(__byte_perm(w0[e], 0x43434343u, 0x4342));
+            const uint32_t a1 = paged_codes(__byte_perm(w1[e], 0x43434343u, 0x4140)), a3 = paged_codes(__byte_perm(w1[e], 0x43434343u, 0x4342));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) paged_mma(x[n], a0, a1, a2, a3, q[n][8 * t + 2 * e], q[n][8 * t + 2 * e + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; e += 2)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) paged_mma(x[n], w0[e], w1[e], w0[e + 1], w1[e + 1], q[n][4 * t + e], q[n][4 * t + e + 1]);
+        }
+      }
+      if (S8) __syncwarp();                    // (the scales of this slot have been read by all)
+      more = find();
+      if (more) copy_keys();
+      paged_commit();
+      // ---- probabilities
+      const bool cut = key + 16 > end;
+      bool raise = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float z = x[n][e];
+          if (S8) z *= kscale[e >> 1];
+          z = a.softcap > 0.f ? cap_out * tanhf(z * cap_in) : z * to_log2;
+          if (cut && key + r + (e >> 1) * 8 >= end) z = ninf;
+          x[n][e] = z;
+          raise |= z > m[n][e & 1] + kPagedReach;
+        }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(m[n][e], fmaxf(x[n][e], x[n][e + 2]));
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+            const float keep = top == ninf ? 1.f : paged_exp2(m[n][e] - top);
+            m[n][e] = top;
+            l[n][e] *= keep;
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t) { o[n][t][e] *= keep; o[n][t][e + 2] *= keep; }
+          }
+      }
+      uint32_t p[NT][2], pl[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float f0 = m[n][0] == ninf ? 0.f : m[n][0], f1 = m[n][1] == ninf ? 0.f : m[n][1];
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = paged_exp2(x[n][e] - ((e & 1) ? f1 : f0));
+        l[n][0] += y[0] + y[2];
+        l[n][1] += y[1] + y[3];
+        if (S8) { y[0] *= vscale[0]; y[1] *= vscale[0]; y[2] *= vscale[1]; y[3] *= vscale[1]; }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t hi = paged_pack(y[2 * e], y[2 * e + 1]);
+          p[n][e] = paged_transpose(hi);
+          pl[n][e] = paged_transpose(paged_pack(y[2 * e] - __uint_as_float(hi << 16), y[2 * e + 1] - __uint_as_float(hi & 0xffff0000u)));
+        }
+      }
+      // ---- outputs
+      paged_wait<2 * ST - 1>();
+      const uint32_t vat = at + Ring::kK + (uint32_t)lane * VB;
+      auto product = [&](int t, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          paged_mma(o[n][t], a0, a1, a2, a3, p[n][0], p[n][1]);
+          paged_mma(o[n][t], a0, a1, a2, a3, pl[n][0], pl[n][1]);
+        }
+      };
+#pragma unroll
+      for (int t = 0; t < VP; ++t) {
+        constexpr int W = VB / 4;
+        uint32_t v[4][W];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t from = vat + (uint32_t)(t * 4 + i) * (32u * VB);
+          if constexpr (VB == 16) { const uint4 w = paged_lds16(from); v[i][0] = w.x; v[i][1] = w.y; v[i][2] = w.z; v[i][3] = w.w; }
+          else { const uint2 w = paged_lds8(from); v[i][0] = w.x; v[i][1] = w.y; }
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          if constexpr (S8) {
+            const uint32_t x01 = __byte_perm(v[0][w], v[1][w], 0x5140), x23 = __byte_perm(v[0][w], v[1][w], 0x7362);
+            const uint32_t y01 = __byte_perm(v[2][w], v[3][w], 0x5140), y23 = __byte_perm(v[2][w], v[3][w], 0x7362);
+            product((t * W + w) * 2, paged_codes(__byte_perm(x01, 0x43434343u, 0x4140)), paged_codes(__byte_perm(x01, 0x43434343u, 0x4342)),
+                    paged_codes(__byte_perm(y01, 0x43434343u, 0x4140)), paged_codes(__byte_perm(y01, 0x43434343u, 0x4342)));
+            product((t * W + w) * 2 + 1, paged_codes(__byte_perm(x23, 0x43434343u, 0x4140)), paged_codes(__byte_perm(x23, 0x43434343u, 0x4342)),
+                    paged_codes(__byte_perm(y23, 0x43434343u, 0x4140)), paged_codes(__byte_perm(y23, 0x43434343u, 0x4342)));
+          } else {
+            product(t * W + w, __byte_perm(v[0][w], v[1][w], 0x5410), __byte_perm(v[0][w], v[1][w], 0x7632), __byte_perm(v[2][w], v[3][w], 0x5410),
+                    __byte_perm(v[2][w], v[3][w], 0x7632));
+          }
+        }
+      }
+      if (more) copy_values();
+      paged_commit();
+      step_on();
+    }
+
+    // ---- the four warps' results as one, in warp 0: maximum, sum, output of its heads 2c and 2c + 1
+    float4 *box = reinterpret_cast<float4 *>(smem + Ring::kBytes);
+    auto join_warps = [&]() {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], w);
+          if (r == 0) { s_m[warp][n * 8 + 2 * c + e] = m[n][e]; s_l[warp][n * 8 + 2 * c + e] = l[n][e]; }
+        }
+      __syncthreads();
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int h = n * 8 + 2 * c + e;
+          float top = s_m[0][h], sum = 0.f;
+#pragma unroll
+          for (int w = 1; w < kPagedWarps; ++w) top = fmaxf(top, s_m[w][h]);
+          const float f = top == ninf ? 0.f : top;
+#pragma unroll
+          for (int w = 0; w < kPagedWarps; ++w) sum += s_l[w][h] * paged_exp2(s_m[w][h] - f);
+          const float keep = paged_exp2(m[n][e] - f);
+          m[n][e] = top; l[n][e] = sum;
+#pragma unroll
+          for (int t = 0; t < DP / 16; ++t) { o[n][t][e] *= keep; o[n][t][e + 2] *= keep; }
+        }
+      auto put = [&](int b) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int t = 0; t < DP / 16; ++t) box[(b * (REGS / 4) + n * (DP / 16) + t) * 32 + lane] = make_float4(o[n][t][0], o[n][t][1], o[n][t][2], o[n][t][3]);
+      };
+      auto add = [&](int b) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int t = 0; t < DP / 16; ++t) {
+            const float4 v = box[(b * (REGS / 4) + n * (DP / 16) + t) * 32 + lane];
+            o[n][t][0] += v.x; o[n][t][1] += v.y; o[n][t][2] += v.z; o[n][t][3] += v.w;
+          }
+      };
+      if (warp >= 2) put(warp - 2);
+      __syncthreads();
+      if (warp < 2) add(warp);
+      if (warp == 1) put(1);
+      __syncthreads();
+      if (warp == 0) add(1);
+    };
+    // the row's result, in warp 0's registers, to where it belongs
+    auto finish = [&]() {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int hh = n * 8 + 2 * c + e, h = h0 + hh;
+          if (hh >= heads) continue;
+          float top = m[n][e], sum = l[n][e], keep = 1.f;
+          if (a.sinks) {
+            const float sink = a.sinks[h] * kPagedLog2e, to = fmaxf(top, sink), f = to == ninf ? 0.f : to;
+            keep = paged_exp2(top - f);
+            sum = sum * keep + paged_exp2(sink - f);
+            top = to;
+          }
+          const float by = sum == 0.f ? 0.f : keep / sum;
+          if (a.lse && r == 0) a.lse[(int64_t)now.seq * a.q_heads + h] = sum == 0.f ? ninf : (top + log2f(sum)) * 0.693147180559945309417f;
+#pragma unroll
+          for (int t = 0; t < DP / 16; t += (S8 && VB == 16 ? 8 : 4)) {
+            // S8 with 16-byte pieces: sixteen dims of a lane in eight tiles, else eight in four
+            constexpr int TILES = S8 && VB == 16 ? 8 : 4;
+            const int d = t * 16 + r * 2 * TILES;
+            if (d >= a.dim) continue;
+            const int64_t to = now.seq * a.os[0] + h * a.os[1] + d;
+            float y[2 * TILES];
+#pragma unroll
+            for (int w = 0; w < TILES; ++w) { y[2 * w] = o[n][t + w][e] * by; y[2 * w + 1] = o[n][t + w][e + 2] * by; }
+            if (s.out_f32) {
+              float *out = reinterpret_cast<float *>(a.out) + to;
+#pragma unroll
+              for (int w = 0; w < TILES / 2; ++w) {
+                if (s.out_vec) reinterpret_cast<float4 *>(out)[w] = make_float4(y[4 * w], y[4 * w + 1], y[4 * w + 2], y[4 * w + 3]);
+                else for (int i = 0; i < 4; ++i) out[4 * w + i] = y[4 * w + i];
+              }
+            } else {
+              uint16_t *out = reinterpret_cast<uint16_t *>(a.out) + to;
+#pragma unroll
+              for (int w = 0; w < TILES / 4; ++w) {
+                const uint4 v = make_uint4(paged_pack(y[8 * w], y[8 * w + 1]), paged_pack(y[8 * w + 2], y[8 * w + 3]), paged_pack(y[8 * w + 4], y[8 * w + 5]),
+                                           paged_pack(y[8 * w + 6], y[8 * w + 7]));
+                if (s.out_vec) reinterpret_cast<uint4 *>(out)[w] = v;
+                else {
+                  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) { out[8 * w + 2 * i] = (uint16_t)(u[i] & 0xffffu); out[8 * w + 2 * i + 1] = (uint16_t)(u[i] >> 16); }
+                }
+              }
+            }
+          }
+        }
+    };
+    join_warps();
+    if (units == now.n) {
+      if (warp == 0) finish();
+    } else {
+      // a part of a row: slot 1 of the CTA in which the row begins, slot 0 of the others
+      const int begin = global - now.off, c0 = begin / per, c1 = (begin + now.n - 1) / per;
+      auto part = [&](int cta) { return (int64_t)cta * 2 + (cta == c0 ? 1 : 0); };
+      if (warp == 0) {
+        float4 *to = reinterpret_cast<float4 *>(s.part_o) + part(blockIdx.x) * (REGS / 4) * 32;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int t = 0; t < DP / 16; ++t) __stcg(to + (n * (DP / 16) + t) * 32 + lane, make_float4(o[n][t][0], o[n][t][1], o[n][t][2], o[n][t][3]));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) if (r == 0) __stcg(s.part_ml + part(blockIdx.x) * 8 * NT + n * 8 + 2 * c + e, make_float2(m[n][e], l[n][e]));
+        }
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) s_last = atomicAdd(s.counters + c0, 1u) == (uint32_t)(c1 - c0);
+      }
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        if (tid == 0) s.counters[c0] = 0u;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          m[n][0] = m[n][1] = ninf; l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+          for (int t = 0; t < DP / 16; ++t) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.f;
+        }
+#pragma unroll 1
+        for (int i = c0 + warp; i <= c1; i += kPagedWarps) {
+          const float4 *from = reinterpret_cast<const float4 *>(s.part_o) + part(i) * (REGS / 4) * 32;
+          float4 v[NT][DP / 16];
+          float2 ml[NT][2];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) ml[n][e] = __ldcg(s.part_ml + part(i) * 8 * NT + n * 8 + 2 * c + e);
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t) v[n][t] = __ldcg(from + (n * (DP / 16) + t) * 32 + lane);
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float mine[2], theirs[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float top = fmaxf(m[n][e], ml[n][e].x), f = top == ninf ? 0.f : top;
+              mine[e] = paged_exp2(m[n][e] - f);
+              theirs[e] = paged_exp2(ml[n][e].x - f);
+              m[n][e] = top;
+              l[n][e] = l[n][e] * mine[e] + (r == 0 ? ml[n][e].y * theirs[e] : 0.f);
+            }
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t) {
+              o[n][t][0] = o[n][t][0] * mine[0] + v[n][t].x * theirs[0]; o[n][t][1] = o[n][t][1] * mine[1] + v[n][t].y * theirs[1];
+              o[n][t][2] = o[n][t][2] * mine[0] + v[n][t].z * theirs[0]; o[n][t][3] = o[n][t][3] * mine[1] + v[n][t].w * theirs[1];
+            }
+          }
+        }
+        join_warps();
+        if (warp == 0) finish();
+      }
+    }
+    global += units;
+    now.next(s);
+  }
+}
+
 }  // namespace b200
