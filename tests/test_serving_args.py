@@ -121,6 +121,7 @@ def test_attention_refusals(capi):
     bad("null", page_table=None)
     bad("strides", q_stride=(C.c_int64 * 2)(256, 1))
     bad("too many", capi.UNIMPLEMENTED, num_seqs=1 << 30)
+    bad("2^30", capi.UNIMPLEMENTED, max_pages=1 << 26, page_table_ld=1 << 26)
     d = attend(capi)
     d.out = d.q
     refused(capi, "b200dnn_paged_attention", d, "overlap")

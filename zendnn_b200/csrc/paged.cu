@@ -69,10 +69,10 @@ int32_t check_cache_here(const char *who, const b200dnn_kv_cache_t &c) {
 // The split form, where rows are 16-byte vectors: false when the call does not fit.
 template <bool S8, int DP, int NT>
 int32_t launch_split(PagedSplitArgs &s, cudaStream_t st) {
-  auto kern = paged_split_kernel<S8, DP, NT>;
+  auto kern = s.a.page_size % 8 == 0 ? paged_split_kernel<S8, DP, NT, true> : paged_split_kernel<S8, DP, NT, false>;
   constexpr size_t smem = paged_smem<S8, DP, NT>();
   const int resident = (int)std::min<size_t>(DP <= 128 ? 3 : 1, (size_t)(227 * 1024) / (smem + 2048));
-  const int64_t most = (int64_t)s.a.B * s.rows * ((s.a.n_keys + kPagedUnit - 1) / kPagedUnit);
+  const int64_t most = (int64_t)s.a.B * s.rows * ((s.a.n_keys + kPagedUnit - 1) / kPagedUnit + 1);      // (a window may begin inside a unit)
   if (most >= (1ll << 31)) return B200DNN_UNIMPLEMENTED;
   const unsigned grid = (unsigned)std::min<int64_t>(most, (int64_t)resident * rt().sm_count);
   s.part_o = (float *)rt().ws.alloc((size_t)grid * 2 * 8 * NT * DP * 4);
@@ -188,6 +188,7 @@ extern "C" int32_t b200dnn_paged_attention(const b200dnn_paged_attention_t *d, v
   B2_CHECK(rows_apart(B, d->q_heads, c.head_dim, d->q_stride) && rows_apart(B, d->q_heads, c.head_dim, d->out_stride), B200DNN_FAILURE,
            "%s: sequence and head strides must be at least head_dim", who);
   B2_CHECK(B * d->q_heads < (1ll << 31), B200DNN_UNIMPLEMENTED, "%s: too many rows in one call", who);
+  B2_CHECK((int64_t)d->max_pages * c.page_size < (1ll << 30), B200DNN_UNIMPLEMENTED, "%s: sequences have less than 2^30 keys", who);
   B2_CHECK(d->q != d->out, B200DNN_FAILURE, "%s: out must not overlap q", who);
   B2_ENTER(stream);
   B2_TRY(check_cache_here(who, c));

@@ -174,14 +174,19 @@ __device__ __forceinline__ uint32_t paged_codes(uint32_t e) {
 }
 
 // What a CTA works on, one piece of a row after the other.
-struct PagedPieces {
+template <bool P8> struct PagedPieces {
   int seq, row, off, n;            // sequence, row of it, first unit in the row, units of the row
   int left;                        // units that the CTA still has, this piece included
-  int64_t lo, hi;                  // visible keys of the sequence
+  int lo, hi, base;                // visible keys of the sequence; where its units begin
   __device__ __forceinline__ int units() const { return min(n - off, left); }
+  __device__ __forceinline__ int first_key() const { return base + off * kPagedUnit; }
+  __device__ __forceinline__ int end_key() const { return min(hi, base + (off + units()) * kPagedUnit); }
   __device__ __forceinline__ void sequence(const PagedArgs &a) {
-    if (!paged_range(a, seq, lo, hi)) lo = hi = 0;
-    n = (int)((hi - lo + kPagedUnit - 1) / kPagedUnit);
+    int64_t l, h;
+    if (!paged_range(a, seq, l, h)) l = h = 0;
+    lo = (int)l; hi = (int)h;
+    base = P8 ? lo & ~7 : lo;
+    n = hi > lo ? (hi - base + kPagedUnit - 1) / kPagedUnit : 0;
   }
   __device__ __forceinline__ void next(const PagedSplitArgs &s) {
     const int u = units();
@@ -213,7 +218,9 @@ template <int DP, int NT> struct PagedJoin {
 };
 template <bool S8, int DP, int NT> constexpr size_t paged_smem() { return PagedRing<S8, DP>::kBytes + PagedJoin<DP, NT>::kBytes; }
 
-template <bool S8, int DP, int NT>
+// P8: pages of a multiple of eight keys.  Units then begin at a multiple of eight, the eight keys of half a step lie on one page, and their places need no lane's
+// table entry but two that the whole warp knows; otherwise every lane looks up the key lane % 16.
+template <bool S8, int DP, int NT, bool P8>
 __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 : 2) paged_split_kernel(const PagedSplitArgs s) {
   using Ring = PagedRing<S8, DP>;
   constexpr int ST = Ring::ST, KP = Ring::kPieceK, VP = Ring::kPieceV, VB = Ring::kWideV, REGS = PagedJoin<DP, NT>::kRegs;
@@ -239,7 +246,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
   }
 
   // ---- this CTA's units: every thread adds up the sequences of its stretch
-  PagedPieces ahead;
+  PagedPieces<P8> ahead;
   int per, first;
   {
     const int stretch = (a.B + 32 * kPagedWarps - 1) / (32 * kPagedWarps), b0 = min(a.B, tid * stretch), b1 = min(a.B, b0 + stretch);
@@ -272,57 +279,118 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     ahead.seq = s_start[0]; ahead.row = s_start[1]; ahead.off = s_start[2]; ahead.left = count;
     ahead.sequence(a);
   }
-  PagedPieces now = ahead;
+  PagedPieces<P8> now = ahead;
 
   // ---- copies, ST steps ahead
   const uint32_t ring = smem_u32(smem) + (uint32_t)warp * (ST * Ring::kStep);
-  int64_t next_key = ahead.lo + (int64_t)ahead.off * kPagedUnit + warp * 16, next_end = min(ahead.hi, ahead.lo + (int64_t)(ahead.off + ahead.units()) * kPagedUnit);
-  int slot_in = 0;
-  int64_t k_at = 0, v_at = 0, s_at = 0;       // of key lane % 16 of the step: where its rows lie
-  bool in_k[2], in_v[4];
-  auto find = [&]() {                         // the next step: its keys' places
-    while (ahead.left > 0 && next_key >= next_end) {
-      ahead.next(s);
-      if (ahead.left <= 0) break;
-      next_key = ahead.lo + (int64_t)ahead.off * kPagedUnit + warp * 16;
-      next_end = min(ahead.hi, ahead.lo + (int64_t)(ahead.off + ahead.units()) * kPagedUnit);
+  constexpr int ES = S8 ? 1 : 2, NP = P8 ? 2 : 1;
+  const int dim_bytes = a.dim * ES;
+  // pieces behind the head dimension stay zeros: nothing is ever copied there
+  if (a.dim < DP) {
+#pragma unroll 1
+    for (int i = 0; i < ST; ++i) {
+      const uint32_t at = ring + (uint32_t)i * Ring::kStep;
+      for (int t = 0; t < 2 * KP; ++t)
+        if ((t % KP) * 64 + c * 16 >= dim_bytes) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + (uint32_t)lane * 16u + (uint32_t)t * 512u), "r"(0) : "memory");
+      for (int t = 0; t < 4 * VP; ++t)
+        for (int w = 0; w < VB; w += 8)
+          if ((t / 4) * 8 * VB + r * VB >= dim_bytes)
+            asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(at + Ring::kK + (uint32_t)lane * VB + (uint32_t)t * (32u * VB) + (uint32_t)w), "r"(0) : "memory");
     }
-    const bool any = ahead.left > 0;
-    const int64_t key = next_key + (lane & 15);
-    const bool take = any && key < next_end;
-    int64_t page = 0, off = 0;
-    if (take) {
-      const uint32_t column = (uint32_t)key / (uint32_t)a.page_size;
-      off = (uint32_t)key - column * (uint32_t)a.page_size;
-      page = paged_page(a, ahead.seq, column);
+  }
+  // the step that is copied next: its first key, the end of its piece, and the place of key (P8: half a step i; else key lane % 16) in the table and on its page
+  int key_in = 0, end_in = 0, column[NP], off_in[NP], page_in[NP];
+  const int step_columns = kPagedUnit / a.page_size, step_off = kPagedUnit - step_columns * a.page_size;
+  const uint8_t *k_head = nullptr, *v_head = nullptr;
+  int64_t s_head = 0;
+  auto look_up = [&]() {
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int key = key_in + (P8 ? 8 * i : lane & 15);
+      page_in[i] = ahead.left > 0 && key < end_in ? a.table[ahead.seq * a.table_ld + column[i]] : 0;
     }
-    const int g = any ? ahead.row / s.tiles : 0;
-    k_at = page * a.ck[0] + off * a.ck[1] + g * a.ck[2];
-    v_at = page * a.cv[0] + off * a.cv[1] + g * a.cv[2];
-    if (S8) s_at = page * a.cs[0] + off * a.cs[1] + g * a.cs[2];
-    const unsigned taken = __ballot_sync(0xffffffffu, take);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) in_k[i] = (taken >> (r + 8 * i)) & 1u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) in_v[i] = (taken >> (2 * c + (i & 1) + 8 * (i >> 1))) & 1u;
-    return any;
   };
+  auto enter = [&]() {                         // the first step that this warp has in the pieces from here on
+    key_in = end_in = 0;
+    while (ahead.left > 0) {
+      key_in = ahead.first_key() + warp * 16;
+      end_in = ahead.end_key();
+      if (key_in < end_in) break;
+      ahead.next(s);
+    }
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const uint32_t key = (uint32_t)(key_in + (P8 ? 8 * i : lane & 15));
+      column[i] = (int)(key / (uint32_t)a.page_size);
+      off_in[i] = (int)key - column[i] * a.page_size;
+    }
+    const int g = ahead.left > 0 ? ahead.row / s.tiles : 0;
+    k_head = reinterpret_cast<const uint8_t *>(a.key) + g * a.ck[2] * ES;
+    v_head = reinterpret_cast<const uint8_t *>(a.value) + g * a.cv[2] * ES;
+    if (S8) s_head = g * a.cs[2];
+  };
+  enter();
+  look_up();
+  int slot_in = 0;
+  const uint32_t k_page = (uint32_t)(a.ck[0] * ES), k_token = (uint32_t)(a.ck[1] * ES), v_page = (uint32_t)(a.cv[0] * ES), v_token = (uint32_t)(a.cv[1] * ES);
+  // (not P8: one address for the lane's key; P8: one for each half of the step)
+  const uint8_t *k_from[NP], *v_from[NP];
+  int64_t s_from = 0;
+  bool more = false, cut_in = false;
+  unsigned taken = 0;                         // cut steps: keys of the step that are visible
+  // Takes the next step: where its keys and values lie; then moves on and asks for the table's entries of the step behind it.
+  auto take = [&]() {
+    more = ahead.left > 0;
+    if (!more) return;
+    int page[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      page[i] = page_in[i];
+      if ((uint32_t)page[i] >= (uint32_t)a.n_pages) { report_status(a.status, kStatusIndex); page[i] = 0; }
+      const bool in = key_in + (P8 ? 8 * i : lane & 15) < end_in;
+      const uint32_t at = in ? (uint32_t)off_in[i] : 0u;      // (behind the end: page 0, token 0; nothing is read there)
+      k_from[i] = k_head + (uint64_t)(uint32_t)page[i] * k_page + (uint64_t)at * k_token;
+      v_from[i] = v_head + (uint64_t)(uint32_t)page[i] * v_page + (uint64_t)at * v_token;
+    }
+    cut_in = key_in + 16 > end_in || key_in < ahead.lo;
+    if (cut_in) { const int key = key_in + (lane & 15); taken = __ballot_sync(0xffffffffu, key >= ahead.lo && key < end_in); }
+    if (S8) {
+      const int i = P8 ? (lane >> 3) & 1 : 0, in_half = P8 ? lane & 7 : 0;
+      s_from = s_head + (int64_t)(P8 && i ? page[NP - 1] : page[0]) * a.cs[0] + (int64_t)((P8 && i ? off_in[NP - 1] : off_in[0]) + in_half) * a.cs[1];
+    }
+    key_in += kPagedUnit;
+    if (key_in < end_in) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        column[i] += step_columns;
+        off_in[i] += step_off;
+        if (off_in[i] >= a.page_size) { off_in[i] -= a.page_size; ++column[i]; }
+      }
+    } else {
+      ahead.next(s);
+      enter();
+    }
+    look_up();
+  };
+  const uint64_t k_lane = (P8 ? (uint64_t)r * k_token : 0) + c * 16, v_lane = (P8 ? (uint64_t)(2 * c) * v_token : 0) + r * VB;
   auto copy_keys = [&]() {
     const uint32_t to = ring + (uint32_t)slot_in * Ring::kStep + (uint32_t)lane * 16u;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t at = __shfl_sync(0xffffffffu, k_at, r + 8 * i);
+      const uint8_t *p = (P8 ? k_from[P8 ? i : 0] : reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(k_from[0]), r + 8 * i))) + k_lane;
+      if (cut_in) {
+        const bool in = (taken >> (r + 8 * i)) & 1u;
+        if (!in) p = reinterpret_cast<const uint8_t *>(a.key);
 #pragma unroll
-      for (int t = 0; t < KP; ++t) {
-        const int d = S8 ? t * 64 + c * 16 : t * 32 + c * 8;
-        const bool in = in_k[i] && d < a.dim;
-        const uint8_t *p = reinterpret_cast<const uint8_t *>(a.key) + (in ? at + d : 0) * (S8 ? 1 : 2);
-        paged_copy<16>(to + (uint32_t)(i * KP + t) * 512u, p, in);
+        for (int t = 0; t < KP; ++t) if (t * 64 + c * 16 < dim_bytes) paged_copy<16>(to + (uint32_t)(i * KP + t) * 512u, p + t * 64, in);
+      } else {
+#pragma unroll
+        for (int t = 0; t < KP; ++t) if (t * 64 + c * 16 < dim_bytes) paged_copy<16>(to + (uint32_t)(i * KP + t) * 512u, p + t * 64, true);
       }
     }
     if (S8) {
-      const bool in = __shfl_sync(0xffffffffu, (int)(in_k[0] | (in_k[1] << 1)), (lane & 7) * 4) >> ((lane >> 3) & 1) & 1;      // key lane % 16
-      const float *p = (lane < 16 ? a.key_scale : a.value_scale) + (in ? s_at : 0);
+      const bool in = !cut_in || ((taken >> (lane & 15)) & 1u);
+      const float *p = (lane < 16 ? a.key_scale : a.value_scale) + (in ? s_from : 0);
       paged_copy<4>(ring + (uint32_t)slot_in * Ring::kStep + Ring::kK + Ring::kV + (uint32_t)lane * 4u, p, in);
     }
   };
@@ -330,21 +398,24 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     const uint32_t to = ring + (uint32_t)slot_in * Ring::kStep + Ring::kK + (uint32_t)lane * VB;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t at = __shfl_sync(0xffffffffu, v_at, 2 * c + (i & 1) + 8 * (i >> 1));
+      const int key = 2 * c + (i & 1) + 8 * (i >> 1);
+      const uint8_t *p = P8 ? v_from[P8 ? i >> 1 : 0] + v_lane + ((i & 1) ? v_token : 0u)
+                            : reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(v_from[0]), key)) + v_lane;
+      if (cut_in) {
+        const bool in = (taken >> key) & 1u;
+        if (!in) p = reinterpret_cast<const uint8_t *>(a.value);
 #pragma unroll
-      for (int t = 0; t < VP; ++t) {
-        const int d = t * (S8 ? 8 * VB : 64) + r * (S8 ? VB : 8);
-        const bool in = in_v[i] && d < a.dim;
-        const uint8_t *p = reinterpret_cast<const uint8_t *>(a.value) + (in ? at + d : 0) * (S8 ? 1 : 2);
-        paged_copy<VB>(to + (uint32_t)(t * 4 + i) * (32u * VB), p, in);
+        for (int t = 0; t < VP; ++t) if (t * 8 * VB + r * VB < dim_bytes) paged_copy<VB>(to + (uint32_t)(t * 4 + i) * (32u * VB), p + t * 8 * VB, in);
+      } else {
+#pragma unroll
+        for (int t = 0; t < VP; ++t) if (t * 8 * VB + r * VB < dim_bytes) paged_copy<VB>(to + (uint32_t)(t * 4 + i) * (32u * VB), p + t * 8 * VB, true);
       }
     }
   };
-  bool more = true;                           // (of this step: something to copy)
-  auto step_on = [&]() { slot_in = slot_in + 1 == ST ? 0 : slot_in + 1; next_key += kPagedUnit; };
+  auto step_on = [&]() { slot_in = slot_in + 1 == ST ? 0 : slot_in + 1; };
 #pragma unroll 1
   for (int i = 0; i < ST; ++i) {
-    more = find();
+    take();
     if (more) copy_keys();
     paged_commit();
     if (more) copy_values();
@@ -388,10 +459,10 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
 #pragma unroll
       for (int t = 0; t < DP / 16; ++t) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.f;
     }
-    const int64_t end = min(now.hi, now.lo + (int64_t)(now.off + units) * kPagedUnit);
+    const int end = now.end_key();
     const float to_log2 = a.scale * kPagedLog2e, cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f, cap_out = a.softcap * kPagedLog2e;
 #pragma unroll 1
-    for (int64_t key = now.lo + (int64_t)now.off * kPagedUnit + warp * 16; key < end; key += kPagedUnit) {
+    for (int key = now.first_key() + warp * 16; key < end; key += kPagedUnit) {
       const uint32_t at = ring + (uint32_t)slot * Ring::kStep;
       slot = slot + 1 == ST ? 0 : slot + 1;
       // ---- scores
@@ -403,9 +474,11 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
         kscale[0] = paged_lds4(sc + 4u * r); kscale[1] = paged_lds4(sc + 4u * r + 32u);
         vscale[0] = paged_lds4(sc + 64u + 4u * r); vscale[1] = paged_lds4(sc + 96u + 4u * r);
       }
-      float x[NT][4];
+      float x[NT][4], x2[NT][4];                // two chains of products
 #pragma unroll
-      for (int n = 0; n < NT; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[n][e] = x2[n][e] = 0.f;
 #pragma unroll
       for (int t = 0; t < KP; ++t) {
         const uint4 k0 = paged_lds16(at + (uint32_t)lane * 16u + (uint32_t)t * 512u), k1 = paged_lds16(at + (uint32_t)lane * 16u + (uint32_t)(KP + t) * 512u);
@@ -416,30 +489,30 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
             const uint32_t a0 = paged_codes(__byte_perm(w0[e], 0x43434343u, 0x4140)), a2 = paged_codes(__byte_perm(w0[e], 0x43434343u, 0x4342));
             const uint32_t a1 = paged_codes(__byte_perm(w1[e], 0x43434343u, 0x4140)), a3 = paged_codes(__byte_perm(w1[e], 0x43434343u, 0x4342));
 #pragma unroll
-            for (int n = 0; n < NT; ++n) paged_mma(x[n], a0, a1, a2, a3, q[n][8 * t + 2 * e], q[n][8 * t + 2 * e + 1]);
+            for (int n = 0; n < NT; ++n) paged_mma(e & 1 ? x2[n] : x[n], a0, a1, a2, a3, q[n][8 * t + 2 * e], q[n][8 * t + 2 * e + 1]);
           }
         } else {
 #pragma unroll
           for (int e = 0; e < 4; e += 2)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) paged_mma(x[n], w0[e], w1[e], w0[e + 1], w1[e + 1], q[n][4 * t + e], q[n][4 * t + e + 1]);
+            for (int n = 0; n < NT; ++n) paged_mma(e ? x2[n] : x[n], w0[e], w1[e], w0[e + 1], w1[e + 1], q[n][4 * t + e], q[n][4 * t + e + 1]);
         }
       }
       if (S8) __syncwarp();                    // (the scales of this slot have been read by all)
-      more = find();
+      take();
       if (more) copy_keys();
       paged_commit();
       // ---- probabilities
-      const bool cut = key + 16 > end;
+      const bool cut = key + 16 > end || key < now.lo;
       bool raise = false;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float z = x[n][e];
+          float z = x[n][e] + x2[n][e];
           if (S8) z *= kscale[e >> 1];
           z = a.softcap > 0.f ? cap_out * tanhf(z * cap_in) : z * to_log2;
-          if (cut && key + r + (e >> 1) * 8 >= end) z = ninf;
+          if (cut && (key + r + (e >> 1) * 8 >= end || key + r + (e >> 1) * 8 < now.lo)) z = ninf;
           x[n][e] = z;
           raise |= z > m[n][e & 1] + kPagedReach;
         }

@@ -6,6 +6,9 @@
   python -m zendnn_b200.run_case bf16 M K N [--copies C] [--reps R] [--act gelu_tanh] [--bias]
   python -m zendnn_b200.run_case norm <rms|fused_add_rms|layer> ROWS COLS [--quant] [--no-output] [--reps R]
   python -m zendnn_b200.run_case sdpa BATCH HEADS SEQ DIM [--kv KEYS] [--causal] [--reps R]
+  python -m zendnn_b200.run_case paged BATCH HEADS KV_HEADS DIM KEYS [--page P] [--s8] [--by-head] [--ragged] [--reps R]
+  python -m zendnn_b200.run_case append TOKENS HEADS KV_HEADS DIM [--page P] [--s8] [--by-head] [--reps R]
+  python -m zendnn_b200.run_case gate TOKENS EXPERTS TOPK [--score softmax|sigmoid] [--groups G] [--reps R]
 
 matmul: s8 per-token activations x s8 per-channel prepacked weight -> bf16; `--copies` distinct prepacked
 weights are used in turn (pick copies * K * N above the L2 size to keep the weight stream in HBM);
@@ -166,6 +169,86 @@ def _sdpa(args):
     flops = 4.0 * B * H * S * KV * D
     print("sdpa B%d H%d S%d KV%d D%d%s: %.1f us per call, %.0f TFLOP/s of 4*B*H*S*KV*D, %.0f GB/s of Q, K, V and O" %
           (B, H, S, KV, D, " causal" if args.causal else "", us, flops / us / 1e6, 4e-3 * B * H * (S + KV) * D / us))
+
+
+def _report(what, reps, call, nbytes):
+    import torch
+    for _ in range(2):
+        call()
+    torch.cuda.synchronize()
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    e0.record()
+    for _ in range(reps):
+        call()
+    e1.record()
+    torch.cuda.synchronize()
+    us = e0.elapsed_time(e1) * 1e3 / reps
+    print("%s: %.1f us per call, %.0f GB/s" % (what, us, nbytes / us / 1e3))
+
+
+def _paged_cache(args, pages, g):
+    import torch
+    from . import capi
+    H, ps, D = args.kv_heads, args.page, args.dim
+    shape = (pages, H, ps, D) if args.by_head else (pages, ps, H, D)
+    seen = (lambda t: t.transpose(1, 2)) if args.by_head else (lambda t: t)
+    if args.s8:
+        kv = [seen(torch.randint(-127, 128, shape, generator=g, dtype=torch.int8, device="cuda")) for _ in range(2)]
+        return capi.make_kv_cache(*kv, *(seen(torch.rand(shape[:3], generator=g, device="cuda") * 0.02 + 0.005) for _ in range(2)))
+    return capi.make_kv_cache(*(seen(torch.randn(shape, generator=g, dtype=torch.bfloat16, device="cuda")) for _ in range(2)))
+
+
+def _paged(args):
+    import ctypes as C
+    import torch
+    from . import capi
+    g = torch.Generator(device="cuda").manual_seed(0)
+    B, n, ps = args.batch, args.keys, args.page
+    lens = torch.full((B,), n, dtype=torch.int32)
+    if args.ragged:
+        lens = (n * torch.rand(B, generator=torch.Generator().manual_seed(0)).sqrt()).int().clamp(min=1)
+    cols = -(-n // ps)
+    table = torch.randperm(B * cols, generator=g, device="cuda").to(torch.int32).view(B, cols)
+    cache = _paged_cache(args, B * cols, g)
+    q = torch.randn(B, args.heads, args.dim, generator=g, device="cuda").to(torch.bfloat16)
+    out = torch.empty_like(q)
+    d = capi.make_paged_attention(cache, q, out, table, lens.cuda())
+    st = torch.cuda.current_stream().cuda_stream
+    seen = int(lens.sum()) * args.kv_heads * 2 * (args.dim * (1 if args.s8 else 2) + (4 if args.s8 else 0))
+    _report("paged attention B%d H%d/%d D%d keys %d" % (B, args.heads, args.kv_heads, args.dim, n), args.reps,
+            lambda: capi.check(capi.lib.b200dnn_paged_attention(C.byref(d), st)), seen)
+
+
+def _append(args):
+    import ctypes as C
+    import torch
+    from . import capi
+    g = torch.Generator(device="cuda").manual_seed(0)
+    T, H, Hk, D = args.tokens, args.heads, args.kv_heads, args.dim
+    pages = -(-T // args.page)
+    cache = _paged_cache(args, pages, g)
+    qkv = torch.randn(T, H + 2 * Hk, D, generator=g, device="cuda").to(torch.bfloat16)
+    angle = torch.rand(32768, D // 2, generator=g, device="cuda") * 6.28
+    q_out = torch.empty(T, H, D, dtype=torch.bfloat16, device="cuda")
+    d = capi.make_kv_append(cache, qkv[:, H:H + Hk], qkv[:, H + Hk:], torch.randperm(pages * args.page, generator=g, device="cuda")[:T].clone(), q=qkv[:, :H],
+                            q_out=q_out, positions=torch.randint(0, 32768, (T,), generator=g, dtype=torch.int32, device="cuda"), cos=angle.cos(), sin=angle.sin())
+    st = torch.cuda.current_stream().cuda_stream
+    _report("kv append T%d H%d/%d D%d" % (T, H, Hk, D), args.reps, lambda: capi.check(capi.lib.b200dnn_kv_append(C.byref(d), st)),
+            T * D * (4 * H + Hk * (4 + 2 * (1 if args.s8 else 2))))
+
+
+def _gate(args):
+    import ctypes as C
+    import torch
+    from . import capi
+    g = torch.Generator(device="cuda").manual_seed(0)
+    T, E, k = args.tokens, args.experts, args.topk
+    x, ids, w = torch.randn(T, E, generator=g, device="cuda"), torch.empty(T, k, dtype=torch.int32, device="cuda"), torch.empty(T, k, device="cuda")
+    d = capi.make_moe_gate(x, k, ids, w, bias=torch.randn(E, generator=g, device="cuda") * 0.1 if args.score == "sigmoid" else None, score=args.score, num_groups=args.groups,
+                           topk_groups=(args.groups + 1) // 2, group_score="top2", expert_counts=torch.empty(E, dtype=torch.int32, device="cuda"),
+                           slot_to_row=torch.empty(T, k, dtype=torch.int32, device="cuda"))
+    st = torch.cuda.current_stream().cuda_stream
+    _report("moe gate T%d E%d top %d" % (T, E, k), args.reps, lambda: capi.check(capi.lib.b200dnn_moe_gate(C.byref(d), st)), T * E * 4 + T * k * 12)
 
 
 def _gs(args):
@@ -342,6 +425,20 @@ def main():
     sd.add_argument("--kv", type=int, default=0, help="keys (default: as many as queries)")
     sd.add_argument("--causal", action="store_true")
     sd.add_argument("--reps", type=int, default=3)
+    for name, what in (("paged", "batch"), ("append", "tokens")):
+        pg = sub.add_parser(name)
+        for a in (what, "heads", "kv_heads", "dim") + (("keys",) if name == "paged" else ()):
+            pg.add_argument(a, type=int)
+        pg.add_argument("--page", type=int, default=16)
+        pg.add_argument("--s8", action="store_true", help="an s8 cache (default: bf16)")
+        pg.add_argument("--by-head", action="store_true", dest="by_head", help="pages stored head by head (default: token by token)")
+        pg.add_argument("--ragged", action="store_true", help="sequences of up to that many keys")
+        pg.add_argument("--reps", type=int, default=5)
+    gt = sub.add_parser("gate")
+    gt.add_argument("tokens", type=int); gt.add_argument("experts", type=int); gt.add_argument("topk", type=int)
+    gt.add_argument("--score", choices=["softmax", "sigmoid"], default="sigmoid")
+    gt.add_argument("--groups", type=int, default=1)
+    gt.add_argument("--reps", type=int, default=5)
     e = sub.add_parser("moe")
     e.add_argument("config", choices=["c4", "c5"])
     e.add_argument("--reps", type=int, default=3)
@@ -351,7 +448,7 @@ def main():
     wp.add_argument("--transB", action="store_true")
     wp.add_argument("--reps", type=int, default=3)
     args = ap.parse_args()
-    {"wprep": _wprep, "matmul": _matmul, "moe": _moe, "gs": _gs, "bf16": _bf16, "norm": _norm, "sdpa": _sdpa}[args.what](args)
+    {"wprep": _wprep, "matmul": _matmul, "moe": _moe, "gs": _gs, "bf16": _bf16, "norm": _norm, "sdpa": _sdpa, "paged": _paged, "append": _append, "gate": _gate}[args.what](args)
 
 
 if __name__ == "__main__":
