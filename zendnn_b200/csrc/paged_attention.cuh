@@ -102,8 +102,8 @@ __global__ void __launch_bounds__(32 * kPagedRowWarps) paged_rows_kernel(const P
 // dealt out evenly: CTA c takes units [c per, (c + 1) per) of a grid that fills the device once, whatever the lengths are (they are on the device).  A row that lies in one CTA is finished
 // there; of the others every CTA leaves a partial result (maximum, sum, unnormalised output), and the last one to arrive joins them, in order.
 //
-// A warp takes 16 keys of a unit at a time, by itself: every lane copies the 16-byte pieces of keys and values that it will multiply (cp.async, `ST` steps ahead,
-// across the ends of rows), and reads back nothing but these, so the ring needs no barrier and no swizzle.  The products run on mma.m16n8k16 with the keys as the 16 rows:
+// A warp takes 16 keys of a unit at a time, by itself: it copies their rows and those of their values into a ring of its own (cp.async, `ST` steps ahead, across the
+// ends of the work's rows), so that no barrier stands between steps.  The products run on mma.m16n8k16 with the keys as the 16 rows:
 //   S^T[key][head] = K Q^T     lane (r, c) = (lane / 4, lane % 4) holds pieces of the keys r and r + 8; which element of the head dimension is which index
 //                              of the product does not matter as long as Q agrees, so a piece of 8 elements is the operand of two products as it lies
 //   O^T[dim][head] = V^T P^T   lane (r, c) holds the same 8 (s8: 16) dims of the keys 2c, 2c + 1, 2c + 8, 2c + 9: a byte permutation pairs two keys of one dim
@@ -129,10 +129,13 @@ struct PagedSplitArgs {
 };
 
 __device__ __forceinline__ float paged_exp2(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+// BYTES from src, or zeros where size is 0; nothing where go is not set
 template <int BYTES>
-__device__ __forceinline__ void paged_copy(uint32_t dst, const void *src, bool take) {
-  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(take ? BYTES : 0) : "memory");
+__device__ __forceinline__ void paged_copy(uint32_t dst, const void *src, uint32_t size, bool go) {
+  if constexpr (BYTES == 16)
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %3, 0;\n@p cp.async.cg.shared.global [%0], [%1], 16, %2;\n}" ::"r"(dst), "l"(src), "r"(size), "r"((int)go) : "memory");
+  else
+    asm volatile("{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n@p cp.async.ca.shared.global [%0], [%1], %2, %3;\n}" ::"r"(dst), "l"(src), "n"(BYTES), "r"(size), "r"((int)go) : "memory");
 }
 __device__ __forceinline__ void paged_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void paged_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -204,13 +207,19 @@ template <bool P8> struct PagedPieces {
 };
 
 template <bool S8, int DP> struct PagedRing {
-  static constexpr int kPieceK = DP * (S8 ? 1 : 2) / 64;                    // 16-byte pieces of a key that a lane copies
+  static constexpr int kRow = DP * (S8 ? 1 : 2);                             // bytes of a row
+  static constexpr int CH = kRow <= 64 ? 4 : kRow <= 128 ? 8 : kRow <= 256 ? 16 : 32;   // lanes of a row, 16 bytes each
+  static constexpr int RI = 32 / CH, IN = 16 / RI;                           // rows of one copy instruction, instructions of 16 rows
+  static constexpr int kPieceK = kRow / 64;                                  // 16-byte pieces of a key that a lane multiplies
   static constexpr int kWideV = S8 ? (DP % 128 == 0 ? 16 : 8) : 16;          // bytes of a value's pieces
-  static constexpr int kPieceV = DP * (S8 ? 1 : 2) / (8 * kWideV);
-  static constexpr int kK = 2 * kPieceK * 512, kV = 4 * kPieceV * 32 * kWideV, kScales = S8 ? 128 : 0;   // bytes of a step: keys, values, scales
-  static constexpr int kStep = kK + kV + kScales;
-  static constexpr int ST = (S8 ? 1 : 2) * DP <= 64 ? 8 : (S8 ? 1 : 2) * DP <= 128 ? 4 : 2;
+  static constexpr int kPieceV = kRow / (8 * kWideV);
+  static constexpr int kRows = 16 * CH * 16, kScales = S8 ? 128 : 0;         // bytes of a step's keys (values), and scales
+  static constexpr int kStep = 2 * kRows + kScales;
+  static constexpr int ST = kRows <= 1024 ? 8 : kRows <= 2048 ? 4 : 2;
   static constexpr int kBytes = kPagedWarps * ST * kStep;
+  // 16-byte chunk j of row `key`, as an offset: neither the copies' rows nor the pieces that eight lanes read at a time meet in a bank
+  static __device__ __forceinline__ uint32_t at_key(int key, int j) { return (uint32_t)((key * CH + j) ^ (CH >= 8 ? (key & 1) << 2 : 0)) * 16u; }
+  static __device__ __forceinline__ uint32_t at_value(int key, int j) { return (uint32_t)((key * CH + j) ^ (((key >> 1) & 3) << 1)) * 16u; }
 };
 template <int DP, int NT> struct PagedJoin {
   static constexpr int kRegs = NT * DP / 4;                                  // unnormalised outputs of a lane
@@ -223,7 +232,7 @@ template <bool S8, int DP, int NT> constexpr size_t paged_smem() { return PagedR
 template <bool S8, int DP, int NT, bool P8>
 __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 : 2) paged_split_kernel(const PagedSplitArgs s) {
   using Ring = PagedRing<S8, DP>;
-  constexpr int ST = Ring::ST, KP = Ring::kPieceK, VP = Ring::kPieceV, VB = Ring::kWideV, REGS = PagedJoin<DP, NT>::kRegs;
+  constexpr int ST = Ring::ST, CH = Ring::CH, RI = Ring::RI, IN = Ring::IN, KP = Ring::kPieceK, VP = Ring::kPieceV, VB = Ring::kWideV, REGS = PagedJoin<DP, NT>::kRegs;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float s_m[kPagedWarps][8 * NT], s_l[kPagedWarps][8 * NT];
   __shared__ int s_scan[kPagedWarps], s_start[4];
@@ -285,18 +294,11 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
   const uint32_t ring = smem_u32(smem) + (uint32_t)warp * (ST * Ring::kStep);
   constexpr int ES = S8 ? 1 : 2, NP = P8 ? 2 : 1;
   const int dim_bytes = a.dim * ES;
-  // pieces behind the head dimension stay zeros: nothing is ever copied there
-  if (a.dim < DP) {
+  // what lies behind the head dimension stays zeros: nothing is ever copied there
+  if (a.dim < CH * 16 / ES) {
 #pragma unroll 1
-    for (int i = 0; i < ST; ++i) {
-      const uint32_t at = ring + (uint32_t)i * Ring::kStep;
-      for (int t = 0; t < 2 * KP; ++t)
-        if ((t % KP) * 64 + c * 16 >= dim_bytes) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + (uint32_t)lane * 16u + (uint32_t)t * 512u), "r"(0) : "memory");
-      for (int t = 0; t < 4 * VP; ++t)
-        for (int w = 0; w < VB; w += 8)
-          if ((t / 4) * 8 * VB + r * VB >= dim_bytes)
-            asm volatile("st.shared.v2.b32 [%0], {%1, %1};" ::"r"(at + Ring::kK + (uint32_t)lane * VB + (uint32_t)t * (32u * VB) + (uint32_t)w), "r"(0) : "memory");
-    }
+    for (uint32_t i = lane * 16u; i < ST * Ring::kStep; i += 512u) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + i), "r"(0) : "memory");
+    __syncwarp();
   }
   // the step that is copied next: its first key, the end of its piece, and the place of key (P8: half a step i; else key lane % 16) in the table and on its page
   int key_in = 0, end_in = 0, column[NP], off_in[NP], page_in[NP];
@@ -336,28 +338,29 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
   // (not P8: one address for the lane's key; P8: one for each half of the step)
   const uint8_t *k_from[NP], *v_from[NP];
   int64_t s_from = 0;
-  bool more = false, cut_in = false;
-  unsigned taken = 0;                         // cut steps: keys of the step that are visible
+  bool cut_in = false;
+  unsigned taken = 0;                         // keys of the step that are visible
+  int limit = 0;                              // head_dim in bytes; 0 when there is no step left
   // Takes the next step: where its keys and values lie; then moves on and asks for the table's entries of the step behind it.
   auto take = [&]() {
-    more = ahead.left > 0;
-    if (!more) return;
+    limit = ahead.left > 0 ? dim_bytes : 0;
+    if (limit == 0) return;
     int page[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       page[i] = page_in[i];
       if ((uint32_t)page[i] >= (uint32_t)a.n_pages) { report_status(a.status, kStatusIndex); page[i] = 0; }
       const bool in = key_in + (P8 ? 8 * i : lane & 15) < end_in;
-      const uint32_t at = in ? (uint32_t)off_in[i] : 0u;      // (behind the end: page 0, token 0; nothing is read there)
-      k_from[i] = k_head + (uint64_t)(uint32_t)page[i] * k_page + (uint64_t)at * k_token;
-      v_from[i] = v_head + (uint64_t)(uint32_t)page[i] * v_page + (uint64_t)at * v_token;
+      const uint32_t at = in ? (uint32_t)off_in[i] : 0u;      // (behind the end: page 0, token 0)
+      k_from[i] = k_head + ((uint64_t)(uint32_t)page[i] * k_page + (uint64_t)at * k_token);
+      v_from[i] = v_head + ((uint64_t)(uint32_t)page[i] * v_page + (uint64_t)at * v_token);
+      if (S8) {
+        const int64_t s_at = (uint64_t)(uint32_t)page[i] * (uint32_t)a.cs[0] + (uint64_t)(at + (P8 ? lane & 7 : 0)) * (uint32_t)a.cs[1];
+        if (i == 0 || (lane & 8)) s_from = s_head + s_at;
+      }
     }
     cut_in = key_in + 16 > end_in || key_in < ahead.lo;
     if (cut_in) { const int key = key_in + (lane & 15); taken = __ballot_sync(0xffffffffu, key >= ahead.lo && key < end_in); }
-    if (S8) {
-      const int i = P8 ? (lane >> 3) & 1 : 0, in_half = P8 ? lane & 7 : 0;
-      s_from = s_head + (int64_t)(P8 && i ? page[NP - 1] : page[0]) * a.cs[0] + (int64_t)((P8 && i ? off_in[NP - 1] : off_in[0]) + in_half) * a.cs[1];
-    }
     key_in += kPagedUnit;
     if (key_in < end_in) {
 #pragma unroll
@@ -372,53 +375,36 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     }
     look_up();
   };
-  const uint64_t k_lane = (P8 ? (uint64_t)r * k_token : 0) + c * 16, v_lane = (P8 ? (uint64_t)(2 * c) * v_token : 0) + r * VB;
+  // Copies of whole rows, CH lanes each (a key that the step does not see is zeros: its address is that of a token of the same page, or of page 0).  Measured on their own, 256-byte
+  // rows: 6.8 TB/s, with every lane copying the pieces that it multiplies (64 bytes of a row at a time) 4.9.
+  const int sub = lane / CH, chunk = lane % CH;
+  const uint64_t k_lane = (P8 ? (uint64_t)sub * k_token : 0) + chunk * 16, v_lane = (P8 ? (uint64_t)sub * v_token : 0) + chunk * 16;
+  auto copy_rows = [&](const uint8_t *const (&from)[NP], uint64_t mine, uint32_t token, bool value) {
+    const uint32_t to = ring + (uint32_t)slot_in * Ring::kStep + (value ? Ring::kRows : 0);
+    const bool go = chunk * 16 < limit;
+#pragma unroll
+    for (int i = 0; i < IN; ++i) {
+      const int half = i * RI / 8, key = i * RI + sub;
+      const uint8_t *p = (P8 ? from[P8 ? half : 0] + (uint32_t)(i * RI - 8 * half) * (uint64_t)token
+                             : reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(from[0]), key))) + mine;
+      const uint32_t size = cut_in && !((taken >> key) & 1u) ? 0u : 16u;
+      paged_copy<16>(to + (value ? Ring::at_value(key, chunk) : Ring::at_key(key, chunk)), p, size, go);
+    }
+  };
   auto copy_keys = [&]() {
-    const uint32_t to = ring + (uint32_t)slot_in * Ring::kStep + (uint32_t)lane * 16u;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint8_t *p = (P8 ? k_from[P8 ? i : 0] : reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(k_from[0]), r + 8 * i))) + k_lane;
-      if (cut_in) {
-        const bool in = (taken >> (r + 8 * i)) & 1u;
-        if (!in) p = reinterpret_cast<const uint8_t *>(a.key);
-#pragma unroll
-        for (int t = 0; t < KP; ++t) if (t * 64 + c * 16 < dim_bytes) paged_copy<16>(to + (uint32_t)(i * KP + t) * 512u, p + t * 64, in);
-      } else {
-#pragma unroll
-        for (int t = 0; t < KP; ++t) if (t * 64 + c * 16 < dim_bytes) paged_copy<16>(to + (uint32_t)(i * KP + t) * 512u, p + t * 64, true);
-      }
-    }
-    if (S8) {
-      const bool in = !cut_in || ((taken >> (lane & 15)) & 1u);
-      const float *p = (lane < 16 ? a.key_scale : a.value_scale) + (in ? s_from : 0);
-      paged_copy<4>(ring + (uint32_t)slot_in * Ring::kStep + Ring::kK + Ring::kV + (uint32_t)lane * 4u, p, in);
-    }
+    copy_rows(k_from, k_lane, k_token, false);
+    if (S8)
+      paged_copy<4>(ring + (uint32_t)slot_in * Ring::kStep + 2 * Ring::kRows + (uint32_t)lane * 4u, (lane < 16 ? a.key_scale : a.value_scale) + s_from,
+                    !cut_in || ((taken >> (lane & 15)) & 1u) ? 4u : 0u, limit > 0);
   };
-  auto copy_values = [&]() {
-    const uint32_t to = ring + (uint32_t)slot_in * Ring::kStep + Ring::kK + (uint32_t)lane * VB;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int key = 2 * c + (i & 1) + 8 * (i >> 1);
-      const uint8_t *p = P8 ? v_from[P8 ? i >> 1 : 0] + v_lane + ((i & 1) ? v_token : 0u)
-                            : reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(v_from[0]), key)) + v_lane;
-      if (cut_in) {
-        const bool in = (taken >> key) & 1u;
-        if (!in) p = reinterpret_cast<const uint8_t *>(a.value);
-#pragma unroll
-        for (int t = 0; t < VP; ++t) if (t * 8 * VB + r * VB < dim_bytes) paged_copy<VB>(to + (uint32_t)(t * 4 + i) * (32u * VB), p + t * 8 * VB, in);
-      } else {
-#pragma unroll
-        for (int t = 0; t < VP; ++t) if (t * 8 * VB + r * VB < dim_bytes) paged_copy<VB>(to + (uint32_t)(t * 4 + i) * (32u * VB), p + t * 8 * VB, true);
-      }
-    }
-  };
+  auto copy_values = [&]() { copy_rows(v_from, v_lane, v_token, true); };
   auto step_on = [&]() { slot_in = slot_in + 1 == ST ? 0 : slot_in + 1; };
 #pragma unroll 1
   for (int i = 0; i < ST; ++i) {
     take();
-    if (more) copy_keys();
+    copy_keys();
     paged_commit();
-    if (more) copy_values();
+    copy_values();
     paged_commit();
     step_on();
   }
@@ -468,9 +454,9 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
       // ---- scores
       paged_wait<2 * ST - 1>();
       float kscale[2] = {1.f, 1.f}, vscale[2] = {1.f, 1.f};
+      __syncwarp();
       if (S8) {
-        __syncwarp();
-        const uint32_t sc = at + Ring::kK + Ring::kV;
+        const uint32_t sc = at + 2 * Ring::kRows;
         kscale[0] = paged_lds4(sc + 4u * r); kscale[1] = paged_lds4(sc + 4u * r + 32u);
         vscale[0] = paged_lds4(sc + 64u + 4u * r); vscale[1] = paged_lds4(sc + 96u + 4u * r);
       }
@@ -481,7 +467,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
         for (int e = 0; e < 4; ++e) x[n][e] = x2[n][e] = 0.f;
 #pragma unroll
       for (int t = 0; t < KP; ++t) {
-        const uint4 k0 = paged_lds16(at + (uint32_t)lane * 16u + (uint32_t)t * 512u), k1 = paged_lds16(at + (uint32_t)lane * 16u + (uint32_t)(KP + t) * 512u);
+        const uint4 k0 = paged_lds16(at + Ring::at_key(r, t * 4 + c)), k1 = paged_lds16(at + Ring::at_key(r + 8, t * 4 + c));
         const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
         if constexpr (S8) {
 #pragma unroll
@@ -498,9 +484,9 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
             for (int n = 0; n < NT; ++n) paged_mma(e ? x2[n] : x[n], w0[e], w1[e], w0[e + 1], w1[e + 1], q[n][4 * t + e], q[n][4 * t + e + 1]);
         }
       }
-      if (S8) __syncwarp();                    // (the scales of this slot have been read by all)
+      __syncwarp();                            // (all lanes have read the slot's keys)
       take();
-      if (more) copy_keys();
+      copy_keys();
       paged_commit();
       // ---- probabilities
       const bool cut = key + 16 > end || key < now.lo;
@@ -550,7 +536,8 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
       }
       // ---- outputs
       paged_wait<2 * ST - 1>();
-      const uint32_t vat = at + Ring::kK + (uint32_t)lane * VB;
+      __syncwarp();
+      const uint32_t vat = at + Ring::kRows;
       auto product = [&](int t, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -564,7 +551,8 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
         uint32_t v[4][W];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t from = vat + (uint32_t)(t * 4 + i) * (32u * VB);
+          const int key = 2 * c + (i & 1) + 8 * (i >> 1), byte = t * 8 * VB + r * VB;
+          const uint32_t from = vat + Ring::at_value(key, byte >> 4) + (VB == 8 ? (byte & 8) : 0);
           if constexpr (VB == 16) { const uint4 w = paged_lds16(from); v[i][0] = w.x; v[i][1] = w.y; v[i][2] = w.z; v[i][3] = w.w; }
           else { const uint2 w = paged_lds8(from); v[i][0] = w.x; v[i][1] = w.y; }
         }
@@ -583,7 +571,8 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
           }
         }
       }
-      if (more) copy_values();
+      __syncwarp();                            // (and its values)
+      copy_values();
       paged_commit();
       step_on();
     }
