@@ -149,6 +149,11 @@ __device__ __forceinline__ uint2 paged_lds8(uint32_t p) {
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(p) : "memory");
   return v;
 }
+__device__ __forceinline__ uint64_t paged_lds_ptr(uint32_t p) {
+  uint64_t v;
+  asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(p) : "memory");
+  return v;
+}
 __device__ __forceinline__ float paged_lds4(uint32_t p) {
   float v;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(p) : "memory");
@@ -237,6 +242,8 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
   __shared__ float s_m[kPagedWarps][8 * NT], s_l[kPagedWarps][8 * NT];
   __shared__ int s_scan[kPagedWarps], s_start[4];
   __shared__ int s_last;
+  __shared__ uint4 s_plan[kPagedWarps][32];
+  __shared__ uint64_t s_splan[S8 ? kPagedWarps : 1][32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const PagedArgs &a = s.a;
@@ -292,7 +299,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
 
   // ---- copies, ST steps ahead
   const uint32_t ring = smem_u32(smem) + (uint32_t)warp * (ST * Ring::kStep);
-  constexpr int ES = S8 ? 1 : 2, NP = P8 ? 2 : 1;
+  constexpr int ES = S8 ? 1 : 2;
   const int dim_bytes = a.dim * ES;
   // what lies behind the head dimension stays zeros: nothing is ever copied there
   if (a.dim < CH * 16 / ES) {
@@ -300,104 +307,88 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     for (uint32_t i = lane * 16u; i < ST * Ring::kStep; i += 512u) asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(ring + i), "r"(0) : "memory");
     __syncwarp();
   }
-  // the step that is copied next: its first key, the end of its piece, and the place of key (P8: half a step i; else key lane % 16) in the table and on its page
-  int key_in = 0, end_in = 0, column[NP], off_in[NP], page_in[NP];
-  const int step_columns = kPagedUnit / a.page_size, step_off = kPagedUnit - step_columns * a.page_size;
-  const uint8_t *k_head = nullptr, *v_head = nullptr;
-  int64_t s_head = 0;
-  auto look_up = [&]() {
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int key = key_in + (P8 ? 8 * i : lane & 15);
-      page_in[i] = ahead.left > 0 && key < end_in ? a.table[ahead.seq * a.table_ld + column[i]] : 0;
-    }
-  };
-  auto enter = [&]() {                         // the first step that this warp has in the pieces from here on
-    key_in = end_in = 0;
-    while (ahead.left > 0) {
-      key_in = ahead.first_key() + warp * 16;
+  // The plan: where the rows of the next steps lie, one entry for GK keys that follow each other on a page (P8: eight), found by all lanes together, 32 entries at a time.
+  constexpr int GK = P8 ? 8 : 1, EP = 16 / GK, SP = 32 / EP;      // keys of an entry, entries of a step, steps of a plan
+  const uint32_t plan = smem_u32(s_plan[warp]), splan = S8 ? smem_u32(s_splan[warp]) : 0u;
+  const uint32_t k_token = (uint32_t)(a.ck[1] * ES), v_token = (uint32_t)(a.cv[1] * ES);
+  int step_key = 0, end_in = 0, lo_in = 0, plan_at = 0, plan_n = 0;
+  bool fresh = true;
+  auto refill = [&]() {
+    __syncwarp();                              // (nobody reads the old one any more)
+    plan_at = plan_n = 0;
+    while (step_key >= end_in) {               // the next piece in which this warp has steps
+      if (!fresh && ahead.left > 0) ahead.next(s);
+      fresh = false;
+      if (ahead.left <= 0) return;
+      step_key = ahead.first_key() + warp * 16;
       end_in = ahead.end_key();
-      if (key_in < end_in) break;
-      ahead.next(s);
+      lo_in = ahead.lo;
     }
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const uint32_t key = (uint32_t)(key_in + (P8 ? 8 * i : lane & 15));
-      column[i] = (int)(key / (uint32_t)a.page_size);
-      off_in[i] = (int)key - column[i] * a.page_size;
+    const int g = ahead.row / s.tiles, key = step_key + lane / EP * kPagedUnit + lane % EP * GK;
+    uint32_t page = 0, off = 0;                // (behind the end: page 0, token 0; nothing of it is used)
+    if (key < end_in) {
+      const uint32_t column = (uint32_t)key / (uint32_t)a.page_size;
+      off = (uint32_t)key - column * (uint32_t)a.page_size;
+      page = (uint32_t)paged_page(a, ahead.seq, column);
     }
-    const int g = ahead.left > 0 ? ahead.row / s.tiles : 0;
-    k_head = reinterpret_cast<const uint8_t *>(a.key) + g * a.ck[2] * ES;
-    v_head = reinterpret_cast<const uint8_t *>(a.value) + g * a.cv[2] * ES;
-    if (S8) s_head = g * a.cs[2];
+    const uint64_t k = reinterpret_cast<uint64_t>(a.key) + (uint64_t)((int64_t)page * a.ck[0] + (int64_t)off * a.ck[1] + g * a.ck[2]) * ES;
+    const uint64_t v = reinterpret_cast<uint64_t>(a.value) + (uint64_t)((int64_t)page * a.cv[0] + (int64_t)off * a.cv[1] + g * a.cv[2]) * ES;
+    asm volatile("st.shared.v2.b64 [%0], {%1, %2};" ::"r"(plan + (uint32_t)lane * 16u), "l"(k), "l"(v) : "memory");
+    if (S8) asm volatile("st.shared.b64 [%0], %1;" ::"r"(splan + (uint32_t)lane * 8u), "l"((int64_t)page * a.cs[0] + (int64_t)off * a.cs[1] + g * a.cs[2]) : "memory");
+    plan_n = min(SP, (end_in - step_key + kPagedUnit - 1) / kPagedUnit);
+    __syncwarp();
   };
-  enter();
-  look_up();
-  int slot_in = 0;
-  const uint32_t k_page = (uint32_t)(a.ck[0] * ES), k_token = (uint32_t)(a.ck[1] * ES), v_page = (uint32_t)(a.cv[0] * ES), v_token = (uint32_t)(a.cv[1] * ES);
-  // (not P8: one address for the lane's key; P8: one for each half of the step)
-  const uint8_t *k_from[NP], *v_from[NP];
-  int64_t s_from = 0;
+  int slot_in = 0, entry = 0;
   bool cut_in = false;
-  unsigned taken = 0;                         // keys of the step that are visible
-  int limit = 0;                              // head_dim in bytes; 0 when there is no step left
-  // Takes the next step: where its keys and values lie; then moves on and asks for the table's entries of the step behind it.
+  unsigned taken = 0;                          // of a cut step: the keys that are visible
+  int limit = 0;                               // head_dim in bytes; 0 when there is no step left
   auto take = [&]() {
-    limit = ahead.left > 0 ? dim_bytes : 0;
-    if (limit == 0) return;
-    int page[NP];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      page[i] = page_in[i];
-      if ((uint32_t)page[i] >= (uint32_t)a.n_pages) { report_status(a.status, kStatusIndex); page[i] = 0; }
-      const bool in = key_in + (P8 ? 8 * i : lane & 15) < end_in;
-      const uint32_t at = in ? (uint32_t)off_in[i] : 0u;      // (behind the end: page 0, token 0)
-      k_from[i] = k_head + ((uint64_t)(uint32_t)page[i] * k_page + (uint64_t)at * k_token);
-      v_from[i] = v_head + ((uint64_t)(uint32_t)page[i] * v_page + (uint64_t)at * v_token);
-      if (S8) {
-        const int64_t s_at = (uint64_t)(uint32_t)page[i] * (uint32_t)a.cs[0] + (uint64_t)(at + (P8 ? lane & 7 : 0)) * (uint32_t)a.cs[1];
-        if (i == 0 || (lane & 8)) s_from = s_head + s_at;
-      }
-    }
-    cut_in = key_in + 16 > end_in || key_in < ahead.lo;
-    if (cut_in) { const int key = key_in + (lane & 15); taken = __ballot_sync(0xffffffffu, key >= ahead.lo && key < end_in); }
-    key_in += kPagedUnit;
-    if (key_in < end_in) {
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        column[i] += step_columns;
-        off_in[i] += step_off;
-        if (off_in[i] >= a.page_size) { off_in[i] -= a.page_size; ++column[i]; }
-      }
-    } else {
-      ahead.next(s);
-      enter();
-    }
-    look_up();
+    if (plan_at == plan_n) refill();
+    limit = plan_n > 0 ? dim_bytes : 0;
+    entry = plan_at * EP;
+    cut_in = step_key + 16 > end_in || step_key < lo_in;
+    if (cut_in && limit) taken = (0xffffu >> max(0, step_key + 16 - end_in)) & (0xffffu << max(0, lo_in - step_key));
+    if (limit) { ++plan_at; step_key += kPagedUnit; }
   };
   // Copies of whole rows, CH lanes each (a key that the step does not see is zeros: its address is that of a token of the same page, or of page 0).  Measured on their own, 256-byte
   // rows: 6.8 TB/s, with every lane copying the pieces that it multiplies (64 bytes of a row at a time) 4.9.
   const int sub = lane / CH, chunk = lane % CH;
-  const uint64_t k_lane = (P8 ? (uint64_t)sub * k_token : 0) + chunk * 16, v_lane = (P8 ? (uint64_t)sub * v_token : 0) + chunk * 16;
-  auto copy_rows = [&](const uint8_t *const (&from)[NP], uint64_t mine, uint32_t token, bool value) {
-    const uint32_t to = ring + (uint32_t)slot_in * Ring::kStep + (value ? Ring::kRows : 0);
+  auto copy_rows = [&](bool value) {
+    const uint32_t slot_at = ring + (uint32_t)slot_in * Ring::kStep + (value ? Ring::kRows : 0), token = value ? v_token : k_token;
     const bool go = chunk * 16 < limit;
+    auto place = [&](int key) { return slot_at + (value ? Ring::at_value(key, chunk) : Ring::at_key(key, chunk)); };
+    auto from = [&](int e) { return paged_lds_ptr(plan + (uint32_t)(entry + e) * 16u + (value ? 8u : 0u)); };
+    const uint64_t mine = (P8 ? (uint64_t)sub * token : 0) + chunk * 16;
+    if (!cut_in) {
+      constexpr int REP_K = RI >= 2 ? 1 : 2, REP_V = RI >= 8 ? 1 : 8 / RI;      // copies after which the swizzle repeats
+      const int rep = value ? REP_V : REP_K;
+      const uint64_t base[2] = {P8 ? from(0) + mine : 0, P8 ? from(EP > 1 ? 1 : 0) + mine : 0};
 #pragma unroll
-    for (int i = 0; i < IN; ++i) {
-      const int half = i * RI / 8, key = i * RI + sub;
-      const uint8_t *p = (P8 ? from[P8 ? half : 0] + (uint32_t)(i * RI - 8 * half) * (uint64_t)token
-                             : reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(from[0]), key))) + mine;
-      const uint32_t size = cut_in && !((taken >> key) & 1u) ? 0u : 16u;
-      paged_copy<16>(to + (value ? Ring::at_value(key, chunk) : Ring::at_key(key, chunk)), p, size, go);
+      for (int i = 0; i < IN; ++i) {
+        const uint64_t p = P8 ? base[i * RI / 8] + (uint64_t)token * (uint32_t)(i * RI % 8) : from(i * RI + sub) + mine;
+        paged_copy<16>(place(i % rep * RI + sub) + (uint32_t)(i / rep * rep * RI * CH * 16), reinterpret_cast<const void *>(p), 16u, go);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < IN; ++i) {
+        const int key = i * RI + sub;
+        const uint64_t p = P8 ? from(key >> 3) + (uint64_t)token * (uint32_t)(key & 7) + chunk * 16 : from(key) + mine;
+        paged_copy<16>(place(key), reinterpret_cast<const void *>(p), (taken >> key) & 1u ? 16u : 0u, go);
+      }
     }
   };
   auto copy_keys = [&]() {
-    copy_rows(k_from, k_lane, k_token, false);
-    if (S8)
-      paged_copy<4>(ring + (uint32_t)slot_in * Ring::kStep + 2 * Ring::kRows + (uint32_t)lane * 4u, (lane < 16 ? a.key_scale : a.value_scale) + s_from,
-                    !cut_in || ((taken >> (lane & 15)) & 1u) ? 4u : 0u, limit > 0);
+    copy_rows(false);
+    if (S8) {
+      const int key = lane & 15;
+      const int64_t at = (int64_t)paged_lds_ptr(splan + (uint32_t)(entry + key / GK) * 8u) + (int64_t)(key % GK) * a.cs[1];
+      paged_copy<4>(ring + (uint32_t)slot_in * Ring::kStep + 2 * Ring::kRows + (uint32_t)lane * 4u, (lane < 16 ? a.key_scale : a.value_scale) + (limit ? at : 0),
+                    !cut_in || ((taken >> key) & 1u) ? 4u : 0u, limit > 0);
+    }
   };
-  auto copy_values = [&]() { copy_rows(v_from, v_lane, v_token, true); };
+  auto copy_values = [&]() { copy_rows(true); };
+  // where a lane reads: keys r and r + 8 (pieces of an odd t lie 64 bytes from where those of an even t would), values of keys 2c, 2c + 1, 2c + 8, 2c + 9
+  const uint32_t k_read[2] = {ring + Ring::at_key(r, c), ring + (CH >= 8 ? Ring::at_key(r, c + 4) : 0u)}, v_read = ring + Ring::kRows + Ring::at_value(2 * c, r);
   auto step_on = [&]() { slot_in = slot_in + 1 == ST ? 0 : slot_in + 1; };
 #pragma unroll 1
   for (int i = 0; i < ST; ++i) {
@@ -449,14 +440,14 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     const float to_log2 = a.scale * kPagedLog2e, cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f, cap_out = a.softcap * kPagedLog2e;
 #pragma unroll 1
     for (int key = now.first_key() + warp * 16; key < end; key += kPagedUnit) {
-      const uint32_t at = ring + (uint32_t)slot * Ring::kStep;
+      const uint32_t at = (uint32_t)slot * Ring::kStep;
       slot = slot + 1 == ST ? 0 : slot + 1;
       // ---- scores
       paged_wait<2 * ST - 1>();
       float kscale[2] = {1.f, 1.f}, vscale[2] = {1.f, 1.f};
       __syncwarp();
       if (S8) {
-        const uint32_t sc = at + 2 * Ring::kRows;
+        const uint32_t sc = ring + at + 2 * Ring::kRows;
         kscale[0] = paged_lds4(sc + 4u * r); kscale[1] = paged_lds4(sc + 4u * r + 32u);
         vscale[0] = paged_lds4(sc + 64u + 4u * r); vscale[1] = paged_lds4(sc + 96u + 4u * r);
       }
@@ -467,7 +458,8 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
         for (int e = 0; e < 4; ++e) x[n][e] = x2[n][e] = 0.f;
 #pragma unroll
       for (int t = 0; t < KP; ++t) {
-        const uint4 k0 = paged_lds16(at + Ring::at_key(r, t * 4 + c)), k1 = paged_lds16(at + Ring::at_key(r + 8, t * 4 + c));
+        const uint32_t from = at + k_read[t & 1] + (uint32_t)(t >> 1) * 128u;
+        const uint4 k0 = paged_lds16(from), k1 = paged_lds16(from + 8 * CH * 16);
         const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
         if constexpr (S8) {
 #pragma unroll
@@ -537,7 +529,6 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
       // ---- outputs
       paged_wait<2 * ST - 1>();
       __syncwarp();
-      const uint32_t vat = at + Ring::kRows;
       auto product = [&](int t, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -551,10 +542,9 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
         uint32_t v[4][W];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = 2 * c + (i & 1) + 8 * (i >> 1), byte = t * 8 * VB + r * VB;
-          const uint32_t from = vat + Ring::at_value(key, byte >> 4) + (VB == 8 ? (byte & 8) : 0);
-          if constexpr (VB == 16) { const uint4 w = paged_lds16(from); v[i][0] = w.x; v[i][1] = w.y; v[i][2] = w.z; v[i][3] = w.w; }
-          else { const uint2 w = paged_lds8(from); v[i][0] = w.x; v[i][1] = w.y; }
+          const uint32_t row = (uint32_t)(((i & 1) + 8 * (i >> 1)) * CH * 16);
+          if constexpr (VB == 16) { const uint4 w = paged_lds16(at + v_read + row + (uint32_t)t * 128u); v[i][0] = w.x; v[i][1] = w.y; v[i][2] = w.z; v[i][3] = w.w; }
+          else { const uint2 w = paged_lds8(ring + at + Ring::kRows + Ring::at_value(2 * c + (i & 1) + 8 * (i >> 1), t * 4 + (r >> 1)) + (r & 1) * 8); v[i][0] = w.x; v[i][1] = w.y; }
         }
 #pragma unroll
         for (int w = 0; w < W; ++w) {
