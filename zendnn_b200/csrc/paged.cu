@@ -72,7 +72,8 @@ int32_t launch_split(PagedSplitArgs &s, cudaStream_t st) {
   auto kern = s.a.page_size % 8 == 0 ? paged_split_kernel<S8, DP, NT, true> : paged_split_kernel<S8, DP, NT, false>;
   constexpr size_t smem = paged_smem<S8, DP, NT>();
   const int resident = (int)std::min<size_t>(DP <= 128 ? 3 : 1, (size_t)(227 * 1024) / (smem + 2048));
-  const int64_t most = (int64_t)s.a.B * s.rows * ((s.a.n_keys + kPagedUnit - 1) / kPagedUnit + 1);      // (a window may begin inside a unit)
+  constexpr int unit = PagedRing<S8, DP>::KS * kPagedWarps;
+  const int64_t most = (int64_t)s.a.B * s.rows * ((s.a.n_keys + unit - 1) / unit + 1);      // (a window may begin inside a unit)
   if (most >= (1ll << 31)) return B200DNN_UNIMPLEMENTED;
   const unsigned grid = (unsigned)std::min<int64_t>(most, (int64_t)resident * rt().sm_count);
   s.part_o = (float *)rt().ws.alloc((size_t)grid * 2 * 8 * NT * DP * 4);

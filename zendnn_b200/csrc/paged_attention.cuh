@@ -98,11 +98,11 @@ __global__ void __launch_bounds__(32 * kPagedRowWarps) paged_rows_kernel(const P
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 // The split form: rows of 16-byte vectors.
 //
-// Work.  A row is one sequence and one tile of up to 8 NT query heads of a key head; its visible keys come in units of 64.  The units of all rows, one row after the other, are
+// Work.  A row is one sequence and one tile of up to 8 NT query heads of a key head; its visible keys come in units of 64 or 128.  The units of all rows, one row after the other, are
 // dealt out evenly: CTA c takes units [c per, (c + 1) per) of a grid that fills the device once, whatever the lengths are (they are on the device).  A row that lies in one CTA is finished
 // there; of the others every CTA leaves a partial result (maximum, sum, unnormalised output), and the last one to arrive joins them, in order.
 //
-// A warp takes 16 keys of a unit at a time, by itself: it copies their rows and those of their values into a ring of its own (cp.async, `ST` steps ahead, across the
+// A warp takes 32 keys of a unit at a time (16 of more than 256 bytes), by itself: it copies their rows and those of their values into a ring of its own (cp.async, `ST` steps ahead, across the
 // ends of the work's rows), so that no barrier stands between steps.  The products run on mma.m16n8k16 with the keys as the 16 rows:
 //   S^T[key][head] = K Q^T     lane (r, c) = (lane / 4, lane % 4) holds pieces of the keys r and r + 8; which element of the head dimension is which index
 //                              of the product does not matter as long as Q agrees, so a piece of 8 elements is the operand of two products as it lies
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(32 * kPagedRowWarps) paged_rows_kernel(const P
 // The running maximum moves only when a score passes it by more than 2^8: probabilities are then at most 256, and few steps meet the exchange.
 
 constexpr float kPagedLog2e = 1.44269504088896340736f;
-constexpr int kPagedWarps = 4, kPagedUnit = 16 * kPagedWarps;
+constexpr int kPagedWarps = 4;
 constexpr float kPagedReach = 8.0f;
 
 struct PagedSplitArgs {
@@ -182,7 +182,7 @@ __device__ __forceinline__ uint32_t paged_codes(uint32_t e) {
 }
 
 // What a CTA works on, one piece of a row after the other.
-template <bool P8> struct PagedPieces {
+template <bool P8, int kPagedUnit> struct PagedPieces {
   int seq, row, off, n;            // sequence, row of it, first unit in the row, units of the row
   int left;                        // units that the CTA still has, this piece included
   int lo, hi, base;                // visible keys of the sequence; where its units begin
@@ -214,30 +214,33 @@ template <bool P8> struct PagedPieces {
 template <bool S8, int DP> struct PagedRing {
   static constexpr int kRow = DP * (S8 ? 1 : 2);                             // bytes of a row
   static constexpr int CH = kRow <= 64 ? 4 : kRow <= 128 ? 8 : kRow <= 256 ? 16 : 32;   // lanes of a row, 16 bytes each
-  static constexpr int RI = 32 / CH, IN = 16 / RI;                           // rows of one copy instruction, instructions of 16 rows
+  static constexpr int KS = kRow <= 256 ? 32 : 16;                           // keys of a step of one warp
+  static constexpr int RI = 32 / CH, IN = KS / RI;                           // rows of one copy instruction, instructions of a step's rows
   static constexpr int kPieceK = kRow / 64;                                  // 16-byte pieces of a key that a lane multiplies
   static constexpr int kWideV = S8 ? (DP % 128 == 0 ? 16 : 8) : 16;          // bytes of a value's pieces
   static constexpr int kPieceV = kRow / (8 * kWideV);
-  static constexpr int kRows = 16 * CH * 16, kScales = S8 ? 128 : 0;         // bytes of a step's keys (values), and scales
+  static constexpr int kRows = KS * CH * 16, kScales = S8 ? KS * 8 : 0;         // bytes of a step's keys (values), and scales
   static constexpr int kStep = 2 * kRows + kScales;
-  static constexpr int ST = kRows <= 1024 ? 8 : kRows <= 2048 ? 4 : 2;
+  static constexpr int ST = kRows <= 2048 ? 4 : kRows <= 4096 ? 2 : KS == 32 ? 1 : 2;
   static constexpr int kBytes = kPagedWarps * ST * kStep;
   // 16-byte chunk j of row `key`, as an offset: neither the copies' rows nor the pieces that eight lanes read at a time meet in a bank
   static __device__ __forceinline__ uint32_t at_key(int key, int j) { return (uint32_t)((key * CH + j) ^ (CH >= 8 ? (key & 1) << 2 : 0)) * 16u; }
   static __device__ __forceinline__ uint32_t at_value(int key, int j) { return (uint32_t)((key * CH + j) ^ (((key >> 1) & 3) << 1)) * 16u; }
 };
-template <int DP, int NT> struct PagedJoin {
+template <bool S8, int DP, int NT> struct PagedJoin {
   static constexpr int kRegs = NT * DP / 4;                                  // unnormalised outputs of a lane
-  static constexpr int kBytes = 2 * kRegs * 128;                             // two warps' in shared memory
+  static constexpr int kBoxes = S8 ? 1 : 2;                                  // warps' outputs in shared memory at a time (with s8 scales in the ring, two would cost an SM its third CTA)
+  static constexpr int kBytes = kBoxes * kRegs * 128;
 };
-template <bool S8, int DP, int NT> constexpr size_t paged_smem() { return PagedRing<S8, DP>::kBytes + PagedJoin<DP, NT>::kBytes; }
+template <bool S8, int DP, int NT> constexpr size_t paged_smem() { return PagedRing<S8, DP>::kBytes + PagedJoin<S8, DP, NT>::kBytes; }
 
 // P8: pages of a multiple of eight keys.  Units then begin at a multiple of eight, the eight keys of half a step lie on one page, and their places need no lane's
 // table entry but two that the whole warp knows; otherwise every lane looks up the key lane % 16.
 template <bool S8, int DP, int NT, bool P8>
 __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 : 2) paged_split_kernel(const PagedSplitArgs s) {
   using Ring = PagedRing<S8, DP>;
-  constexpr int ST = Ring::ST, CH = Ring::CH, RI = Ring::RI, IN = Ring::IN, KP = Ring::kPieceK, VP = Ring::kPieceV, VB = Ring::kWideV, REGS = PagedJoin<DP, NT>::kRegs;
+  constexpr int KS = Ring::KS, MT = KS / 16, kPagedUnit = KS * kPagedWarps;
+  constexpr int ST = Ring::ST, CH = Ring::CH, RI = Ring::RI, IN = Ring::IN, KP = Ring::kPieceK, VP = Ring::kPieceV, VB = Ring::kWideV, REGS = PagedJoin<S8, DP, NT>::kRegs;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float s_m[kPagedWarps][8 * NT], s_l[kPagedWarps][8 * NT];
   __shared__ int s_scan[kPagedWarps], s_start[4];
@@ -262,7 +265,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
   }
 
   // ---- this CTA's units: every thread adds up the sequences of its stretch
-  PagedPieces<P8> ahead;
+  PagedPieces<P8, kPagedUnit> ahead;
   int per, first;
   {
     const int stretch = (a.B + 32 * kPagedWarps - 1) / (32 * kPagedWarps), b0 = min(a.B, tid * stretch), b1 = min(a.B, b0 + stretch);
@@ -295,7 +298,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     ahead.seq = s_start[0]; ahead.row = s_start[1]; ahead.off = s_start[2]; ahead.left = count;
     ahead.sequence(a);
   }
-  PagedPieces<P8> now = ahead;
+  PagedPieces<P8, kPagedUnit> now = ahead;
 
   // ---- copies, ST steps ahead
   const uint32_t ring = smem_u32(smem) + (uint32_t)warp * (ST * Ring::kStep);
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     __syncwarp();
   }
   // The plan: where the rows of the next steps lie, one entry for GK keys that follow each other on a page (P8: eight), found by all lanes together, 32 entries at a time.
-  constexpr int GK = P8 ? 8 : 1, EP = 16 / GK, SP = 32 / EP;      // keys of an entry, entries of a step, steps of a plan
+  constexpr int GK = P8 ? 8 : 1, EP = KS / GK, SP = 32 / EP;      // keys of an entry, entries of a step, steps of a plan
   const uint32_t plan = smem_u32(s_plan[warp]), splan = S8 ? smem_u32(s_splan[warp]) : 0u;
   const uint32_t k_token = (uint32_t)(a.ck[1] * ES), v_token = (uint32_t)(a.cv[1] * ES);
   int step_key = 0, end_in = 0, lo_in = 0, plan_at = 0, plan_n = 0;
@@ -320,7 +323,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
       if (!fresh && ahead.left > 0) ahead.next(s);
       fresh = false;
       if (ahead.left <= 0) return;
-      step_key = ahead.first_key() + warp * 16;
+      step_key = ahead.first_key() + warp * KS;
       end_in = ahead.end_key();
       lo_in = ahead.lo;
     }
@@ -346,8 +349,8 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     if (plan_at == plan_n) refill();
     limit = plan_n > 0 ? dim_bytes : 0;
     entry = plan_at * EP;
-    cut_in = step_key + 16 > end_in || step_key < lo_in;
-    if (cut_in && limit) taken = (0xffffu >> max(0, step_key + 16 - end_in)) & (0xffffu << max(0, lo_in - step_key));
+    cut_in = step_key + KS > end_in || step_key < lo_in;
+    if (cut_in && limit) taken = (0xffffffffu >> max(0, step_key + 32 - end_in)) & (0xffffffffu << max(0, lo_in - step_key));
     if (limit) { ++plan_at; step_key += kPagedUnit; }
   };
   // Copies of whole rows, CH lanes each (a key that the step does not see is zeros: its address is that of a token of the same page, or of page 0).  Measured on their own, 256-byte
@@ -362,10 +365,14 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     if (!cut_in) {
       constexpr int REP_K = RI >= 2 ? 1 : 2, REP_V = RI >= 8 ? 1 : 8 / RI;      // copies after which the swizzle repeats
       const int rep = value ? REP_V : REP_K;
-      const uint64_t base[2] = {P8 ? from(0) + mine : 0, P8 ? from(EP > 1 ? 1 : 0) + mine : 0};
+      uint64_t base[P8 ? EP : 1];
+      if constexpr (P8) {
+#pragma unroll
+        for (int e = 0; e < EP; ++e) base[e] = from(e) + mine;
+      }
 #pragma unroll
       for (int i = 0; i < IN; ++i) {
-        const uint64_t p = P8 ? base[i * RI / 8] + (uint64_t)token * (uint32_t)(i * RI % 8) : from(i * RI + sub) + mine;
+        const uint64_t p = P8 ? base[P8 ? i * RI / 8 : 0] + (uint64_t)token * (uint32_t)(i * RI % 8) : from(i * RI + sub) + mine;
         paged_copy<16>(place(i % rep * RI + sub) + (uint32_t)(i / rep * rep * RI * CH * 16), reinterpret_cast<const void *>(p), 16u, go);
       }
     } else {
@@ -380,10 +387,15 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
   auto copy_keys = [&]() {
     copy_rows(false);
     if (S8) {
-      const int key = lane & 15;
-      const int64_t at = (int64_t)paged_lds_ptr(splan + (uint32_t)(entry + key / GK) * 8u) + (int64_t)(key % GK) * a.cs[1];
-      paged_copy<4>(ring + (uint32_t)slot_in * Ring::kStep + 2 * Ring::kRows + (uint32_t)lane * 4u, (lane < 16 ? a.key_scale : a.value_scale) + (limit ? at : 0),
-                    !cut_in || ((taken >> key) & 1u) ? 4u : 0u, limit > 0);
+#pragma unroll
+      for (int i = 0; i < (S8 ? MT : 0); ++i) {
+        // keys' scales, then values' (MT 1: sixteen lanes each)
+        const int key = MT == 2 ? lane : lane & 15;
+        const bool value = MT == 2 ? i == 1 : lane >= 16;
+        const int64_t at = (int64_t)paged_lds_ptr(splan + (uint32_t)(entry + key / GK) * 8u) + (int64_t)(key % GK) * a.cs[1];
+        paged_copy<4>(ring + (uint32_t)slot_in * Ring::kStep + 2 * Ring::kRows + (uint32_t)(i * 32 + lane) * 4u, (value ? a.value_scale : a.key_scale) + (limit ? at : 0),
+                      !cut_in || ((taken >> key) & 1u) ? 4u : 0u, limit > 0);
+      }
     }
   };
   auto copy_values = [&]() { copy_rows(true); };
@@ -439,67 +451,74 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     const int end = now.end_key();
     const float to_log2 = a.scale * kPagedLog2e, cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f, cap_out = a.softcap * kPagedLog2e;
 #pragma unroll 1
-    for (int key = now.first_key() + warp * 16; key < end; key += kPagedUnit) {
+    for (int key = now.first_key() + warp * KS; key < end; key += kPagedUnit) {
       const uint32_t at = (uint32_t)slot * Ring::kStep;
       slot = slot + 1 == ST ? 0 : slot + 1;
       // ---- scores
       paged_wait<2 * ST - 1>();
-      float kscale[2] = {1.f, 1.f}, vscale[2] = {1.f, 1.f};
       __syncwarp();
-      if (S8) {
-        const uint32_t sc = ring + at + 2 * Ring::kRows;
-        kscale[0] = paged_lds4(sc + 4u * r); kscale[1] = paged_lds4(sc + 4u * r + 32u);
-        vscale[0] = paged_lds4(sc + 64u + 4u * r); vscale[1] = paged_lds4(sc + 96u + 4u * r);
+      float kscale[MT][2], vscale[MT][2];
+      if constexpr (S8) {
+        const uint32_t sc = ring + at + 2 * Ring::kRows + 4u * r;
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) { kscale[i >> 1][i & 1] = paged_lds4(sc + 32u * i); vscale[i >> 1][i & 1] = paged_lds4(sc + 4u * KS + 32u * i); }
       }
-      float x[NT][4], x2[NT][4];                // two chains of products
+      float x[MT][NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[n][e] = x2[n][e] = 0.f;
+        for (int n = 0; n < NT; ++n) x[i][n][0] = x[i][n][1] = x[i][n][2] = x[i][n][3] = 0.f;
 #pragma unroll
-      for (int t = 0; t < KP; ++t) {
-        const uint32_t from = at + k_read[t & 1] + (uint32_t)(t >> 1) * 128u;
-        const uint4 k0 = paged_lds16(from), k1 = paged_lds16(from + 8 * CH * 16);
-        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
-        if constexpr (S8) {
+      for (int t = 0; t < KP; ++t)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t a0 = paged_codes(__byte_perm(w0[e], 0x43434343u, 0x4140)), a2 = paged_codes(__byte_perm(w0[e], 0x43434343u, 0x4342));
-            const uint32_t a1 = paged_codes(__byte_perm(w1[e], 0x43434343u, 0x4140)), a3 = paged_codes(__byte_perm(w1[e], 0x43434343u, 0x4342));
+        for (int i = 0; i < MT; ++i) {
+          const uint32_t from = at + k_read[t & 1] + (uint32_t)(t >> 1) * 128u + (uint32_t)(i * 16 * CH * 16);
+          const uint4 k0 = paged_lds16(from), k1 = paged_lds16(from + 8 * CH * 16);
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+          if constexpr (S8) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) paged_mma(e & 1 ? x2[n] : x[n], a0, a1, a2, a3, q[n][8 * t + 2 * e], q[n][8 * t + 2 * e + 1]);
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t a0 = paged_codes(__byte_perm(w0[e], 0x43434343u, 0x4140)), a2 = paged_codes(__byte_perm(w0[e], 0x43434343u, 0x4342));
+              const uint32_t a1 = paged_codes(__byte_perm(w1[e], 0x43434343u, 0x4140)), a3 = paged_codes(__byte_perm(w1[e], 0x43434343u, 0x4342));
+#pragma unroll
+              for (int n = 0; n < NT; ++n) paged_mma(x[i][n], a0, a1, a2, a3, q[n][8 * t + 2 * e], q[n][8 * t + 2 * e + 1]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; e += 2)
+#pragma unroll
+              for (int n = 0; n < NT; ++n) paged_mma(x[i][n], w0[e], w1[e], w0[e + 1], w1[e + 1], q[n][4 * t + e], q[n][4 * t + e + 1]);
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; e += 2)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) paged_mma(e ? x2[n] : x[n], w0[e], w1[e], w0[e + 1], w1[e + 1], q[n][4 * t + e], q[n][4 * t + e + 1]);
         }
-      }
       __syncwarp();                            // (all lanes have read the slot's keys)
       take();
       copy_keys();
       paged_commit();
       // ---- probabilities
-      const bool cut = key + 16 > end || key < now.lo;
+      const bool cut = key + KS > end || key < now.lo;
       bool raise = false;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float z = x[n][e] + x2[n][e];
-          if (S8) z *= kscale[e >> 1];
-          z = a.softcap > 0.f ? cap_out * tanhf(z * cap_in) : z * to_log2;
-          if (cut && (key + r + (e >> 1) * 8 >= end || key + r + (e >> 1) * 8 < now.lo)) z = ninf;
-          x[n][e] = z;
-          raise |= z > m[n][e & 1] + kPagedReach;
-        }
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float z = x[i][n][e];
+            if constexpr (S8) z *= kscale[i][e >> 1];
+            z = a.softcap > 0.f ? cap_out * tanhf(z * cap_in) : z * to_log2;
+            const int at_key = key + 16 * i + r + (e >> 1) * 8;
+            if (cut && (at_key >= end || at_key < now.lo)) z = ninf;
+            x[i][n][e] = z;
+            raise |= z > m[n][e & 1] + kPagedReach;
+          }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(m[n][e], fmaxf(x[n][e], x[n][e + 2]));
+            float top = m[n][e];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) top = fmaxf(top, fmaxf(x[i][n][e], x[i][n][e + 2]));
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
             const float keep = top == ninf ? 1.f : paged_exp2(m[n][e] - top);
@@ -509,55 +528,64 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
             for (int t = 0; t < DP / 16; ++t) { o[n][t][e] *= keep; o[n][t][e + 2] *= keep; }
           }
       }
-      uint32_t p[NT][2], pl[NT][2];
+      uint32_t p[MT][NT][2], pl[MT][NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float f0 = m[n][0] == ninf ? 0.f : m[n][0], f1 = m[n][1] == ninf ? 0.f : m[n][1];
-        float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = paged_exp2(x[n][e] - ((e & 1) ? f1 : f0));
-        l[n][0] += y[0] + y[2];
-        l[n][1] += y[1] + y[3];
-        if (S8) { y[0] *= vscale[0]; y[1] *= vscale[0]; y[2] *= vscale[1]; y[3] *= vscale[1]; }
+        for (int i = 0; i < MT; ++i) {
+          float y[4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint32_t hi = paged_pack(y[2 * e], y[2 * e + 1]);
-          p[n][e] = paged_transpose(hi);
-          pl[n][e] = paged_transpose(paged_pack(y[2 * e] - __uint_as_float(hi << 16), y[2 * e + 1] - __uint_as_float(hi & 0xffff0000u)));
+          for (int e = 0; e < 4; ++e) y[e] = paged_exp2(x[i][n][e] - ((e & 1) ? f1 : f0));
+          l[n][0] += y[0] + y[2];
+          l[n][1] += y[1] + y[3];
+          if constexpr (S8) { y[0] *= vscale[i][0]; y[1] *= vscale[i][0]; y[2] *= vscale[i][1]; y[3] *= vscale[i][1]; }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t hi = paged_pack(y[2 * e], y[2 * e + 1]);
+            p[i][n][e] = paged_transpose(hi);
+            pl[i][n][e] = paged_transpose(paged_pack(y[2 * e] - __uint_as_float(hi << 16), y[2 * e + 1] - __uint_as_float(hi & 0xffff0000u)));
+          }
         }
       }
       // ---- outputs
       paged_wait<2 * ST - 1>();
       __syncwarp();
-      auto product = [&](int t, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          paged_mma(o[n][t], a0, a1, a2, a3, p[n][0], p[n][1]);
-          paged_mma(o[n][t], a0, a1, a2, a3, pl[n][0], pl[n][1]);
-        }
-      };
 #pragma unroll
       for (int t = 0; t < VP; ++t) {
         constexpr int W = VB / 4;
-        uint32_t v[4][W];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t row = (uint32_t)(((i & 1) + 8 * (i >> 1)) * CH * 16);
-          if constexpr (VB == 16) { const uint4 w = paged_lds16(at + v_read + row + (uint32_t)t * 128u); v[i][0] = w.x; v[i][1] = w.y; v[i][2] = w.z; v[i][3] = w.w; }
-          else { const uint2 w = paged_lds8(ring + at + Ring::kRows + Ring::at_value(2 * c + (i & 1) + 8 * (i >> 1), t * 4 + (r >> 1)) + (r & 1) * 8); v[i][0] = w.x; v[i][1] = w.y; }
-        }
+        for (int j = 0; j < MT; ++j) {
+          auto product = [&](int d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
 #pragma unroll
-        for (int w = 0; w < W; ++w) {
-          if constexpr (S8) {
-            const uint32_t x01 = __byte_perm(v[0][w], v[1][w], 0x5140), x23 = __byte_perm(v[0][w], v[1][w], 0x7362);
-            const uint32_t y01 = __byte_perm(v[2][w], v[3][w], 0x5140), y23 = __byte_perm(v[2][w], v[3][w], 0x7362);
-            product((t * W + w) * 2, paged_codes(__byte_perm(x01, 0x43434343u, 0x4140)), paged_codes(__byte_perm(x01, 0x43434343u, 0x4342)),
-                    paged_codes(__byte_perm(y01, 0x43434343u, 0x4140)), paged_codes(__byte_perm(y01, 0x43434343u, 0x4342)));
-            product((t * W + w) * 2 + 1, paged_codes(__byte_perm(x23, 0x43434343u, 0x4140)), paged_codes(__byte_perm(x23, 0x43434343u, 0x4342)),
-                    paged_codes(__byte_perm(y23, 0x43434343u, 0x4140)), paged_codes(__byte_perm(y23, 0x43434343u, 0x4342)));
-          } else {
-            product(t * W + w, __byte_perm(v[0][w], v[1][w], 0x5410), __byte_perm(v[0][w], v[1][w], 0x7632), __byte_perm(v[2][w], v[3][w], 0x5410),
-                    __byte_perm(v[2][w], v[3][w], 0x7632));
+            for (int n = 0; n < NT; ++n) {
+              paged_mma(o[n][d], a0, a1, a2, a3, p[j][n][0], p[j][n][1]);
+              paged_mma(o[n][d], a0, a1, a2, a3, pl[j][n][0], pl[j][n][1]);
+            }
+          };
+          uint32_t v[4][W];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t row = (uint32_t)((16 * j + (i & 1) + 8 * (i >> 1)) * CH * 16);
+            if constexpr (VB == 16) { const uint4 w = paged_lds16(at + v_read + row + (uint32_t)t * 128u); v[i][0] = w.x; v[i][1] = w.y; v[i][2] = w.z; v[i][3] = w.w; }
+            else {
+              const uint2 w = paged_lds8(ring + at + Ring::kRows + Ring::at_value(16 * j + 2 * c + (i & 1) + 8 * (i >> 1), t * 4 + (r >> 1)) + (r & 1) * 8);
+              v[i][0] = w.x; v[i][1] = w.y;
+            }
+          }
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            if constexpr (S8) {
+              const uint32_t x01 = __byte_perm(v[0][w], v[1][w], 0x5140), x23 = __byte_perm(v[0][w], v[1][w], 0x7362);
+              const uint32_t y01 = __byte_perm(v[2][w], v[3][w], 0x5140), y23 = __byte_perm(v[2][w], v[3][w], 0x7362);
+              product((t * W + w) * 2, paged_codes(__byte_perm(x01, 0x43434343u, 0x4140)), paged_codes(__byte_perm(x01, 0x43434343u, 0x4342)),
+                      paged_codes(__byte_perm(y01, 0x43434343u, 0x4140)), paged_codes(__byte_perm(y01, 0x43434343u, 0x4342)));
+              product((t * W + w) * 2 + 1, paged_codes(__byte_perm(x23, 0x43434343u, 0x4140)), paged_codes(__byte_perm(x23, 0x43434343u, 0x4342)),
+                      paged_codes(__byte_perm(y23, 0x43434343u, 0x4140)), paged_codes(__byte_perm(y23, 0x43434343u, 0x4342)));
+            } else {
+              product(t * W + w, __byte_perm(v[0][w], v[1][w], 0x5410), __byte_perm(v[0][w], v[1][w], 0x7632), __byte_perm(v[2][w], v[3][w], 0x5410),
+                      __byte_perm(v[2][w], v[3][w], 0x7632));
+            }
           }
         }
       }
@@ -610,12 +638,22 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
             o[n][t][0] += v.x; o[n][t][1] += v.y; o[n][t][2] += v.z; o[n][t][3] += v.w;
           }
       };
-      if (warp >= 2) put(warp - 2);
-      __syncthreads();
-      if (warp < 2) add(warp);
-      if (warp == 1) put(1);
-      __syncthreads();
-      if (warp == 0) add(1);
+      if constexpr (PagedJoin<S8, DP, NT>::kBoxes == 2) {
+        if (warp >= 2) put(warp - 2);
+        __syncthreads();
+        if (warp < 2) add(warp);
+        if (warp == 1) put(1);
+        __syncthreads();
+        if (warp == 0) add(1);
+      } else {
+        if (warp == 3) put(0);
+#pragma unroll 1
+        for (int w = 2; w >= 0; --w) {
+          __syncthreads();
+          if (warp == w) add(0);
+          if (warp == w && w > 0) put(0);
+        }
+      }
     };
     // the row's result, in warp 0's registers, to where it belongs
     auto finish = [&]() {
