@@ -66,6 +66,33 @@ int32_t check_cache_here(const char *who, const b200dnn_kv_cache_t &c) {
   return B200DNN_SUCCESS;
 }
 
+template <typename T, bool S8>
+int32_t launch_append(const AppendArgs &a, cudaStream_t st) {
+  const int R = a.q_heads + 2 * a.kv_heads;
+  // vectors: 16 bytes of every input and of bf16 rows, 8 of s8 rows; a rotary part of whole pairs of pieces
+  auto apart = [](const void *p, uintptr_t bytes, int size, int64_t n0, int64_t s0, int64_t n1, int64_t s1) {
+    return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (n0 <= 1 || s0 * size % (int64_t)bytes == 0) && (n1 <= 1 || s1 * size % (int64_t)bytes == 0);
+  };
+  const int ct = S8 ? 1 : 2, cb = S8 ? 8 : 16, it = sizeof(T) == 4 ? 4 : 2;
+  auto cache = [&](const void *p, const int64_t (&s)[3]) {
+    return apart(p, cb, ct, 2, s[0], a.page_size, s[1]) && apart(p, cb, ct, a.kv_heads, s[2], 1, 0);
+  };
+  const bool vec = a.dim % 8 == 0 && a.rot % 16 == 0 && (!a.interleaved || a.rot == 0 || a.rot % 16 == 0) && cache(a.key, a.ck) && cache(a.value, a.cv) &&
+                   apart(a.k, 16, it, a.T, a.ks[0], a.kv_heads, a.ks[1]) && apart(a.v, 16, it, a.T, a.vs[0], a.kv_heads, a.vs[1]) &&
+                   (a.q_heads == 0 || (apart(a.q, 16, it, a.T, a.qs[0], a.q_heads, a.qs[1]) && apart(a.q_out, 16, it, a.T, a.os[0], a.q_heads, a.os[1]))) &&
+                   (a.rot == 0 || (apart(a.cos_t, 16, 4, a.table_rows, a.table_ld, 1, 0) && apart(a.sin_t, 16, 4, a.table_rows, a.table_ld, 1, 0)));
+  if (!vec) return launch(append_rows_kernel<T, S8>, (unsigned)((a.T * R + 7) / 8), 256, 0, st, a);
+  const int tpr = a.dim <= 32 ? 2 : a.dim <= 64 ? 4 : a.dim <= 128 ? 8 : 16;
+  // a token's rows over as many threads as take kAppendRows of them each
+  const unsigned threads = (unsigned)std::min(256, (int)round_up((int64_t)(R + kAppendRows - 1) / kAppendRows * tpr, 32));
+  switch (tpr) {
+    case 2: return launch(append_token_kernel<T, S8, 2>, (unsigned)a.T, threads, 0, st, a);
+    case 4: return launch(append_token_kernel<T, S8, 4>, (unsigned)a.T, threads, 0, st, a);
+    case 8: return launch(append_token_kernel<T, S8, 8>, (unsigned)a.T, threads, 0, st, a);
+    default: return launch(append_token_kernel<T, S8, 16>, (unsigned)a.T, threads, 0, st, a);
+  }
+}
+
 // The split form, where rows are 16-byte vectors: false when the call does not fit.
 template <bool S8, int DP, int NT>
 int32_t launch_split(PagedSplitArgs &s, cudaStream_t st) {
@@ -163,10 +190,9 @@ extern "C" int32_t b200dnn_kv_append(const b200dnn_kv_append_t *d, void *stream)
   a.n_slots = c.num_pages * c.page_size; a.T = T;
   a.page_size = c.page_size; a.q_heads = d->q_heads; a.kv_heads = c.kv_heads; a.dim = c.head_dim; a.rot = d->rotary_dim; a.interleaved = d->interleaved ? 1 : 0;
   a.status = rt().status;
-  const unsigned grid = (unsigned)((T * R + 7) / 8);
   const bool f32 = d->dt == B200DNN_F32, s8 = c.dt == B200DNN_S8;
-  B2_TRY(f32 ? (s8 ? launch(append_rows_kernel<float, true>, grid, 256, 0, st, a) : launch(append_rows_kernel<float, false>, grid, 256, 0, st, a))
-             : (s8 ? launch(append_rows_kernel<__nv_bfloat16, true>, grid, 256, 0, st, a) : launch(append_rows_kernel<__nv_bfloat16, false>, grid, 256, 0, st, a)));
+  B2_TRY(f32 ? (s8 ? launch_append<float, true>(a, st) : launch_append<float, false>(a, st))
+             : (s8 ? launch_append<__nv_bfloat16, true>(a, st) : launch_append<__nv_bfloat16, false>(a, st)));
   return finish_out({&q_out}, st);
 }
 

@@ -33,9 +33,7 @@ template <typename T> __device__ __forceinline__ void append_store(void *p, int6
 }
 
 // The token's place: false when nothing of it is to be written (padding, or an index out of range, which is reported).
-__device__ __forceinline__ bool append_place(const AppendArgs &a, int64_t t, int64_t &page, int &off, int64_t &pos) {
-  const int64_t slot = a.slots[t];
-  pos = a.rot ? a.positions[t] : 0;
+__device__ __forceinline__ bool append_place(const AppendArgs &a, int64_t slot, int64_t pos, int64_t &page, int &off) {
   if (slot < 0) return false;
   if (slot >= a.n_slots || pos < 0 || (a.rot && pos >= a.table_rows)) {
     report_status(a.status, kStatusIndex);
@@ -63,8 +61,9 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const AppendArgs a) {
   const int64_t t = w / R;
   if (t >= a.T) return;
   int h = (int)(w - t * R);
-  int64_t page, pos; int off;
-  if (!append_place(a, t, page, off, pos)) return;
+  int64_t page; int off;
+  const int64_t pos = a.rot ? a.positions[t] : 0;
+  if (!append_place(a, a.slots[t], pos, page, off)) return;
   const int half = a.rot >> 1, pairs = (a.dim + 1) >> 1;
   const void *src; int64_t at;                      // the row
   void *dst; int64_t to;
@@ -115,6 +114,139 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const AppendArgs a) {
     } else {
       append_store<__nv_bfloat16>(dst, to + i0, x);
       if (i1 < a.dim) append_store<__nv_bfloat16>(dst, to + i1, y);
+    }
+  }
+}
+
+
+// Rows of 16-byte vectors.  A CTA takes one token, TPR threads a row: thread j of a row holds 16 elements in two pieces of eight, those of a rotary pair where the row is
+// rotated (half against half: [8 j, +8) and [rot / 2 + 8 j, +8); interleaved: 16 neighbours), and goes through the token's rows with them, so that a piece of the
+// tables is loaded once for all heads.  All of a thread's rows are loaded before the token's place is known.  s8: the row's largest element by shuffles over its threads.
+constexpr int kAppendRows = 4;                      // rows of a thread in flight
+
+struct Append8 { float v[8]; };
+template <typename T> __device__ __forceinline__ Append8 append_load8(const void *p, int64_t i) {
+  Append8 x;
+  if constexpr (sizeof(T) == 4) {
+    const float4 *q = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + i);
+    const float4 a = q[0], b = q[1];
+    x.v[0] = a.x; x.v[1] = a.y; x.v[2] = a.z; x.v[3] = a.w; x.v[4] = b.x; x.v[5] = b.y; x.v[6] = b.z; x.v[7] = b.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p) + i);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { x.v[2 * e] = __uint_as_float(w[e] << 16); x.v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+  }
+  return x;
+}
+__device__ __forceinline__ uint32_t append_pack(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <typename T> __device__ __forceinline__ void append_store8(void *p, int64_t i, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    float4 *q = reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + i);
+    q[0] = make_float4(v[0], v[1], v[2], v[3]);
+    q[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(p) + i) = make_uint4(append_pack(v[0], v[1]), append_pack(v[2], v[3]), append_pack(v[4], v[5]), append_pack(v[6], v[7]));
+  }
+}
+
+// TPR: threads of a row, a power of two
+template <typename T, bool S8, int TPR>
+__global__ void __launch_bounds__(256) append_token_kernel(const AppendArgs a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t t = blockIdx.x;
+  const int R = a.q_heads + 2 * a.kv_heads, j = threadIdx.x % TPR, row0 = threadIdx.x / TPR, rows = blockDim.x / TPR;
+  const int half = a.rot >> 1, turned_threads = a.rot >> 4;
+  const bool turns = j < turned_threads;
+  // the two pieces: of a rotated row, and of a row of v
+  const int c0 = turns && !a.interleaved ? 8 * j : 16 * j, c1 = turns && !a.interleaved ? half + 8 * j : 16 * j + 8;
+  const int64_t slot = a.slots[t], pos = a.rot ? a.positions[t] : 0;
+  int64_t page = 0; int off = 0;
+  Append8 cs, sn;
+  bool placed = false;
+  for (int first = row0; first < R; first += rows * kAppendRows) {
+    Append8 x[kAppendRows][2];
+    auto source = [&](int row, const void *&p, int64_t &at) {
+      if (row < a.q_heads) { p = a.q; at = t * a.qs[0] + row * a.qs[1]; }
+      else if (row < a.q_heads + a.kv_heads) { p = a.k; at = t * a.ks[0] + (row - a.q_heads) * a.ks[1]; }
+      else { p = a.v; at = t * a.vs[0] + (row - a.q_heads - a.kv_heads) * a.vs[1]; }
+    };
+#pragma unroll
+    for (int i = 0; i < kAppendRows; ++i) {
+      const int row = first + i * rows;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i][0].v[e] = x[i][1].v[e] = 0.f;
+      if (row >= R) continue;
+      const void *p; int64_t at;
+      source(row, p, at);
+      const int o0 = row < a.q_heads + a.kv_heads ? c0 : 16 * j, o1 = row < a.q_heads + a.kv_heads ? c1 : 16 * j + 8;
+      if (o0 < a.dim) x[i][0] = append_load8<T>(p, at + o0);
+      if (o1 < a.dim) x[i][1] = append_load8<T>(p, at + o1);
+    }
+    if (!placed) {
+      if (!append_place(a, slot, pos, page, off)) return;
+      if (turns) {
+        cs = append_load8<float>(a.cos_t, pos * a.table_ld + 8 * j);
+        sn = append_load8<float>(a.sin_t, pos * a.table_ld + 8 * j);
+      }
+      placed = true;
+    }
+#pragma unroll
+    for (int i = 0; i < kAppendRows; ++i) {
+      const int row = first + i * rows;
+      const bool on = row < R;
+      const bool key = row >= a.q_heads && row < a.q_heads + a.kv_heads, value = row >= a.q_heads + a.kv_heads;
+      float (&u)[8] = x[i][0].v, (&w)[8] = x[i][1].v;
+      if (turns && !value) {
+        if (a.interleaved) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { append_turn(u[2 * e], u[2 * e + 1], cs.v[e], sn.v[e]); append_turn(w[2 * e], w[2 * e + 1], cs.v[4 + e], sn.v[4 + e]); }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) append_turn(u[e], w[e], cs.v[e], sn.v[e]);
+        }
+      }
+      const int o0 = value ? 16 * j : c0, o1 = value ? 16 * j + 8 : c1, h = row - a.q_heads - (value ? a.kv_heads : 0);
+      if (!key && !value) {
+        if (!on) continue;
+        const int64_t to = t * a.os[0] + row * a.os[1];
+        if (o0 < a.dim) append_store8<T>(a.q_out, to + o0, u);
+        if (o1 < a.dim) append_store8<T>(a.q_out, to + o1, w);
+        continue;
+      }
+      void *dst = value ? a.value : a.key;
+      const int64_t to = page * (value ? a.cv[0] : a.ck[0]) + off * (value ? a.cv[1] : a.ck[1]) + h * (value ? a.cv[2] : a.ck[2]);
+      if constexpr (S8) {
+        float most = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (finite_f32(u[e])) most = fmaxf(most, fabsf(u[e]));
+          if (finite_f32(w[e])) most = fmaxf(most, fabsf(w[e]));
+        }
+        const unsigned lanes = TPR == 32 ? 0xffffffffu : ((1u << TPR) - 1u) << ((threadIdx.x & 31) / TPR * TPR);
+#pragma unroll
+        for (int o = TPR / 2; o; o >>= 1) most = fmaxf(most, __shfl_xor_sync(lanes, most, o));
+        if (!on) continue;
+        const float scale = scale_from_absmax(most), rinv = __frcp_rn(scale);
+        auto codes = [&](const float (&v)[8]) {
+          uint32_t c[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) c[e] = (uint32_t)(uint8_t)quant_sym_r<float>(v[e], scale, rinv);
+          return make_uint2(low_bytes4(c[0], c[1], c[2], c[3]), low_bytes4(c[4], c[5], c[6], c[7]));
+        };
+        if (o0 < a.dim) *reinterpret_cast<uint2 *>(reinterpret_cast<int8_t *>(dst) + to + o0) = codes(u);
+        if (o1 < a.dim) *reinterpret_cast<uint2 *>(reinterpret_cast<int8_t *>(dst) + to + o1) = codes(w);
+        if (j == 0) (value ? a.value_scale : a.key_scale)[page * a.cs[0] + off * a.cs[1] + h * a.cs[2]] = scale;
+      } else {
+        if (!on) continue;
+        if (o0 < a.dim) append_store8<__nv_bfloat16>(dst, to + o0, u);
+        if (o1 < a.dim) append_store8<__nv_bfloat16>(dst, to + o1, w);
+      }
     }
   }
 }
