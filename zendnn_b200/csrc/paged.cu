@@ -84,7 +84,7 @@ int32_t launch_append(const AppendArgs &a, cudaStream_t st) {
   if (!vec) return launch(append_rows_kernel<T, S8>, (unsigned)((a.T * R + 7) / 8), 256, 0, st, a);
   const int tpr = a.dim <= 32 ? 2 : a.dim <= 64 ? 4 : a.dim <= 128 ? 8 : 16;
   // a token's rows over as many threads as take kAppendRows of them each
-  const unsigned threads = (unsigned)std::min(256, (int)round_up((int64_t)(R + kAppendRows - 1) / kAppendRows * tpr, 32));
+  const unsigned threads = (unsigned)std::min(256, (int)round_up((int64_t)(R + kAppendRows<T> - 1) / kAppendRows<T> * tpr, 32));
   switch (tpr) {
     case 2: return launch(append_token_kernel<T, S8, 2>, (unsigned)a.T, threads, 0, st, a);
     case 4: return launch(append_token_kernel<T, S8, 4>, (unsigned)a.T, threads, 0, st, a);

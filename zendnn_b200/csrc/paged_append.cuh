@@ -122,22 +122,28 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const AppendArgs a) {
 // Rows of 16-byte vectors.  A CTA takes one token, TPR threads a row: thread j of a row holds 16 elements in two pieces of eight, those of a rotary pair where the row is
 // rotated (half against half: [8 j, +8) and [rot / 2 + 8 j, +8); interleaved: 16 neighbours), and goes through the token's rows with them, so that a piece of the
 // tables is loaded once for all heads.  All of a thread's rows are loaded before the token's place is known.  s8: the row's largest element by shuffles over its threads.
-constexpr int kAppendRows = 4;                      // rows of a thread in flight
-
 struct Append8 { float v[8]; };
-template <typename T> __device__ __forceinline__ Append8 append_load8(const void *p, int64_t i) {
-  Append8 x;
-  if constexpr (sizeof(T) == 4) {
-    const float4 *q = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + i);
-    const float4 a = q[0], b = q[1];
-    x.v[0] = a.x; x.v[1] = a.y; x.v[2] = a.z; x.v[3] = a.w; x.v[4] = b.x; x.v[5] = b.y; x.v[6] = b.z; x.v[7] = b.w;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p) + i);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// eight elements as they lie in memory
+template <typename T> struct AppendRaw { uint4 w[sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ AppendRaw<T> append_raw(const void *p, int64_t i) {
+  const uint4 *q = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(p) + i * (int64_t)sizeof(T));
+  AppendRaw<T> x;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { x.v[2 * e] = __uint_as_float(w[e] << 16); x.v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
-  }
+  for (int e = 0; e < (int)sizeof(T) / 2; ++e) x.w[e] = __ldg(q + e);
   return x;
+}
+template <typename T> __device__ __forceinline__ Append8 append_floats(const AppendRaw<T> &x) {
+  Append8 y;
+#pragma unroll
+  for (int e = 0; e < (int)sizeof(T) / 2; ++e) {
+    const uint32_t w[4] = {x.w[e].x, x.w[e].y, x.w[e].z, x.w[e].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) y.v[4 * e + i] = __uint_as_float(w[i]);
+      else { y.v[2 * i] = __uint_as_float(w[i] << 16); y.v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+  }
+  return y;
 }
 __device__ __forceinline__ uint32_t append_pack(float lo, float hi) {
   uint32_t r;
@@ -154,9 +160,11 @@ template <typename T> __device__ __forceinline__ void append_store8(void *p, int
   }
 }
 
+// Rows of a thread in flight: 128 bytes (their registers decide how many CTAs an SM holds, and the call is bound by how much is in flight).
+template <typename T> constexpr int kAppendRows = sizeof(T) == 4 ? 2 : 4;
 // TPR: threads of a row, a power of two
 template <typename T, bool S8, int TPR>
-__global__ void __launch_bounds__(256) append_token_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(256, 3) append_token_kernel(const AppendArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int64_t t = blockIdx.x;
@@ -169,39 +177,39 @@ __global__ void __launch_bounds__(256) append_token_kernel(const AppendArgs a) {
   int64_t page = 0; int off = 0;
   Append8 cs, sn;
   bool placed = false;
-  for (int first = row0; first < R; first += rows * kAppendRows) {
-    Append8 x[kAppendRows][2];
+  for (int first = row0; first < R; first += rows * kAppendRows<T>) {
+    AppendRaw<T> x[kAppendRows<T>][2];
     auto source = [&](int row, const void *&p, int64_t &at) {
       if (row < a.q_heads) { p = a.q; at = t * a.qs[0] + row * a.qs[1]; }
       else if (row < a.q_heads + a.kv_heads) { p = a.k; at = t * a.ks[0] + (row - a.q_heads) * a.ks[1]; }
       else { p = a.v; at = t * a.vs[0] + (row - a.q_heads - a.kv_heads) * a.vs[1]; }
     };
 #pragma unroll
-    for (int i = 0; i < kAppendRows; ++i) {
+    for (int i = 0; i < kAppendRows<T>; ++i) {
       const int row = first + i * rows;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][0].v[e] = x[i][1].v[e] = 0.f;
+      x[i][0] = x[i][1] = AppendRaw<T>{};
       if (row >= R) continue;
       const void *p; int64_t at;
       source(row, p, at);
       const int o0 = row < a.q_heads + a.kv_heads ? c0 : 16 * j, o1 = row < a.q_heads + a.kv_heads ? c1 : 16 * j + 8;
-      if (o0 < a.dim) x[i][0] = append_load8<T>(p, at + o0);
-      if (o1 < a.dim) x[i][1] = append_load8<T>(p, at + o1);
+      if (o0 < a.dim) x[i][0] = append_raw<T>(p, at + o0);
+      if (o1 < a.dim) x[i][1] = append_raw<T>(p, at + o1);
     }
     if (!placed) {
       if (!append_place(a, slot, pos, page, off)) return;
       if (turns) {
-        cs = append_load8<float>(a.cos_t, pos * a.table_ld + 8 * j);
-        sn = append_load8<float>(a.sin_t, pos * a.table_ld + 8 * j);
+        cs = append_floats<float>(append_raw<float>(a.cos_t, pos * a.table_ld + 8 * j));
+        sn = append_floats<float>(append_raw<float>(a.sin_t, pos * a.table_ld + 8 * j));
       }
       placed = true;
     }
 #pragma unroll
-    for (int i = 0; i < kAppendRows; ++i) {
+    for (int i = 0; i < kAppendRows<T>; ++i) {
       const int row = first + i * rows;
       const bool on = row < R;
       const bool key = row >= a.q_heads && row < a.q_heads + a.kv_heads, value = row >= a.q_heads + a.kv_heads;
-      float (&u)[8] = x[i][0].v, (&w)[8] = x[i][1].v;
+      Append8 x0 = append_floats<T>(x[i][0]), x1 = append_floats<T>(x[i][1]);
+      float (&u)[8] = x0.v, (&w)[8] = x1.v;
       if (turns && !value) {
         if (a.interleaved) {
 #pragma unroll
