@@ -465,6 +465,7 @@ typedef struct b200dnn_kv_append_t {
   const float *cos_table, *sin_table;   /* [table_rows][table_ld >= rotary_dim / 2] */
   int64_t table_rows, table_ld;
   const int64_t *slots;           /* [num_tokens]: page * page_size + token in the page */
+  int32_t device, reserved;
 } b200dnn_kv_append_t;
 B200DNN_API int32_t b200dnn_kv_append(const b200dnn_kv_append_t *desc, void *stream);
 
@@ -491,7 +492,7 @@ typedef struct b200dnn_paged_attention_t {
   const float *sinks;             /* [q_heads], may be NULL */
   double scale;                   /* 0 = 1 / sqrt(head_dim) */
   float softcap;                  /* 0: off */
-  int32_t reserved;
+  int32_t device;
 } b200dnn_paged_attention_t;
 B200DNN_API int32_t b200dnn_paged_attention(const b200dnn_paged_attention_t *desc, void *stream);
 
@@ -522,6 +523,7 @@ typedef struct b200dnn_moe_gate_t {
   float *weights;                 /* may be NULL */
   int32_t *expert_counts;         /* [num_experts], may be NULL */
   int32_t *slot_to_row;           /* [num_tokens][topk], may be NULL */
+  int32_t device, reserved;
 } b200dnn_moe_gate_t;
 B200DNN_API int32_t b200dnn_moe_gate(const b200dnn_moe_gate_t *desc, void *stream);
 

@@ -42,9 +42,9 @@ def refused(capi, entry, desc, text, status=None):
 
 def test_struct_layout_matches_header(capi):
     assert C.sizeof(capi.KvCache) == 4 * 4 + 8 + 4 * 8 + 9 * 8
-    assert C.sizeof(capi.KvAppendDesc) == C.sizeof(capi.KvCache) + 8 + 4 * 4 + 8 * 8 + 7 * 8 + 2 * 8 + 8
+    assert C.sizeof(capi.KvAppendDesc) == C.sizeof(capi.KvCache) + 8 + 4 * 4 + 8 * 8 + 7 * 8 + 2 * 8 + 8 + 2 * 4
     assert C.sizeof(capi.PagedAttentionDesc) == C.sizeof(capi.KvCache) + 4 * 4 + 4 * 8 + 4 * 8 + 8 + 2 * 4 + 2 * 8 + 8 + 2 * 4
-    assert C.sizeof(capi.MoeGateDesc) == 10 * 4 + 8 + 6 * 8
+    assert C.sizeof(capi.MoeGateDesc) == 10 * 4 + 8 + 6 * 8 + 2 * 4
 
 
 def test_null_descriptors(capi):

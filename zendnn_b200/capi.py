@@ -87,14 +87,14 @@ class KvAppendDesc(C.Structure):
                 ("interleaved", C.c_int32), ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2),
                 ("q_out_stride", C.c_int64 * 2), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p),
                 ("positions", C.c_void_p), ("cos_table", C.c_void_p), ("sin_table", C.c_void_p), ("table_rows", C.c_int64),
-                ("table_ld", C.c_int64), ("slots", C.c_void_p)]
+                ("table_ld", C.c_int64), ("slots", C.c_void_p), ("device", C.c_int32), ("reserved", C.c_int32)]
 
 
 class PagedAttentionDesc(C.Structure):
     _fields_ = [("cache", KvCache), ("num_seqs", C.c_int32), ("q_heads", C.c_int32), ("q_dt", C.c_int32), ("out_dt", C.c_int32),
                 ("q_stride", C.c_int64 * 2), ("out_stride", C.c_int64 * 2), ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
                 ("page_table", C.c_void_p), ("page_table_ld", C.c_int64), ("max_pages", C.c_int32), ("window", C.c_int32),
-                ("seq_lens", C.c_void_p), ("sinks", C.c_void_p), ("scale", C.c_double), ("softcap", C.c_float), ("reserved", C.c_int32)]
+                ("seq_lens", C.c_void_p), ("sinks", C.c_void_p), ("scale", C.c_double), ("softcap", C.c_float), ("device", C.c_int32)]
 
 
 GATE_SCORE = dict(softmax=0, sigmoid=1)
@@ -105,7 +105,7 @@ class MoeGateDesc(C.Structure):
     _fields_ = [("num_tokens", C.c_int32), ("num_experts", C.c_int32), ("topk", C.c_int32), ("score", C.c_int32), ("num_groups", C.c_int32),
                 ("topk_groups", C.c_int32), ("group_score", C.c_int32), ("renorm", C.c_int32), ("scale", C.c_float), ("logits_dt", C.c_int32),
                 ("ld", C.c_int64), ("logits", C.c_void_p), ("bias", C.c_void_p), ("ids", C.c_void_p), ("weights", C.c_void_p),
-                ("expert_counts", C.c_void_p), ("slot_to_row", C.c_void_p)]
+                ("expert_counts", C.c_void_p), ("slot_to_row", C.c_void_p), ("device", C.c_int32), ("reserved", C.c_int32)]
 
 
 class EpConfig(C.Structure):
@@ -306,6 +306,13 @@ def _dense(what, buf, axis=-1):
         raise ValueError("%s: the last dimension must be dense" % what)
 
 
+def _device(*bufs):
+    """The `device` field of a descriptor: set when all buffers are CUDA tensors of one device."""
+    found = {buf.device.index if getattr(buf, "is_cuda", False) else None for buf in bufs if buf is not None}
+    only = found.pop() if len(found) == 1 else None
+    return 0 if only is None else only + 1
+
+
 def make_kv_cache(key, value, key_scale=None, value_scale=None):
     """Descriptor of a paged cache from views [page, token, head, dim] of its keys and values in any storage order (bf16, or s8 with
     scales [page, token, head], both scale arrays laid out alike)."""
@@ -345,6 +352,7 @@ def make_kv_append(cache, k, v, slots, q=None, q_out=None, positions=None, cos=N
     T = int(k.shape[0])
     d = KvAppendDesc()
     d.keep = (cache, k, v, slots, q, q_out, positions, cos, sin)
+    d.device = _device(*getattr(cache, "keep", (0,)), *d.keep[1:])
     d.cache, d.num_tokens, d.dt, d.interleaved = cache, T, dt_of(k), int(interleaved)
     heads = [("k", k), ("v", v)]
     if q is not None:
@@ -374,6 +382,7 @@ def make_paged_attention(cache, q, out, page_table, seq_lens, scale=0.0, window=
     B, H = int(q.shape[0]), int(q.shape[1])
     d = PagedAttentionDesc()
     d.keep = (cache, q, out, page_table, seq_lens, sinks, lse)
+    d.device = _device(*getattr(cache, "keep", (0,)), *d.keep[1:])
     d.cache, d.num_seqs, d.q_heads = cache, B, H
     for name, buf in (("q", q), ("out", out)):
         if tuple(buf.shape) != (B, H, cache.head_dim):
@@ -402,6 +411,7 @@ def make_moe_gate(logits, topk, ids, weights=None, *, bias=None, score="softmax"
     T, E = logits.shape
     d = MoeGateDesc()
     d.keep = (logits, ids, weights, bias, expert_counts, slot_to_row)
+    d.device = _device(*d.keep)
     d.num_tokens, d.num_experts, d.topk = T, E, topk
     d.score, d.num_groups, d.topk_groups, d.group_score = GATE_SCORE[score], num_groups, topk_groups, GROUP_SCORE[group_score]
     d.renorm, d.scale, d.logits_dt = int(renorm), scale, dt_of(logits)

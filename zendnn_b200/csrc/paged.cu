@@ -47,21 +47,13 @@ int32_t check_cache(const char *who, const b200dnn_kv_cache_t &c) {
   return B200DNN_SUCCESS;
 }
 
-// The kernels write to the cache where it lies, and memory of another device may be out of their reach.
-int32_t check_here(const char *who, const char *what, const void *p) {
-  cudaPointerAttributes at;
-  if (cudaPointerGetAttributes(&at, p) != cudaSuccess) { cudaGetLastError(); at.type = cudaMemoryTypeUnregistered; }
-  B2_CHECK(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, B200DNN_UNIMPLEMENTED, "%s: %s must be device memory", who, what);
-  B2_CHECK(at.type == cudaMemoryTypeManaged || at.device == rt().shared->dev, B200DNN_FAILURE, "%s: %s lies on device %d, the current one is %d", who, what, at.device,
-           rt().shared->dev);
-  return B200DNN_SUCCESS;
-}
-int32_t check_cache_here(const char *who, const b200dnn_kv_cache_t &c) {
-  B2_TRY(check_here(who, "the cache", c.key));
-  B2_TRY(check_here(who, "the cache", c.value));
+// The kernels use the cache where it lies.
+int32_t check_cache_here(const Staging &g, const b200dnn_kv_cache_t &c) {
+  B2_TRY(g.here("the cache", c.key));
+  B2_TRY(g.here("the cache", c.value));
   if (c.dt == B200DNN_S8) {
-    B2_TRY(check_here(who, "the cache's scales", c.key_scale));
-    B2_TRY(check_here(who, "the cache's scales", c.value_scale));
+    B2_TRY(g.here("the cache's scales", c.key_scale));
+    B2_TRY(g.here("the cache's scales", c.value_scale));
   }
   return B200DNN_SUCCESS;
 }
@@ -165,23 +157,24 @@ extern "C" int32_t b200dnn_kv_append(const b200dnn_kv_append_t *d, void *stream)
     B2_CHECK(d->positions && d->cos_table && d->sin_table && d->table_rows > 0 && d->table_ld >= d->rotary_dim / 2 && d->table_ld < (1ll << 31), B200DNN_FAILURE,
              "%s: a rotation needs positions and tables of at least rotary_dim / 2 columns", who);
   B2_ENTER(stream);
-  B2_TRY(check_cache_here(who, c));
+  const Staging g{d->device, st, who};
+  B2_TRY(g.check());
+  B2_TRY(check_cache_here(g, c));
   AppendArgs a{};
   const size_t table_bytes = d->rotary_dim ? (size_t)((d->table_rows - 1) * d->table_ld + d->rotary_dim / 2) * 4 : 0;
   Staged q_out{};
-  const void *p;
-  B2_TRY(stage_in(d->k, span2(T, c.kv_heads, c.head_dim, d->k_stride, d->dt), st, &a.k));
-  B2_TRY(stage_in(d->v, span2(T, c.kv_heads, c.head_dim, d->v_stride, d->dt), st, &a.v));
-  B2_TRY(stage_in(d->slots, (size_t)T * 8, st, &p)); a.slots = (const int64_t *)p;
+  B2_TRY(g.in(d->k, span2(T, c.kv_heads, c.head_dim, d->k_stride, d->dt), &a.k));
+  B2_TRY(g.in(d->v, span2(T, c.kv_heads, c.head_dim, d->v_stride, d->dt), &a.v));
+  B2_TRY(g.in(d->slots, (size_t)T * 8, &a.slots));
   if (d->q_heads) {
-    B2_TRY(stage_in(d->q, span2(T, d->q_heads, c.head_dim, d->q_stride, d->dt), st, &a.q));
-    B2_TRY(stage_out(d->q_out, span2(T, d->q_heads, c.head_dim, d->q_out_stride, d->dt), st, &q_out, true));
+    B2_TRY(g.in(d->q, span2(T, d->q_heads, c.head_dim, d->q_stride, d->dt), &a.q));
+    B2_TRY(g.out(d->q_out, span2(T, d->q_heads, c.head_dim, d->q_out_stride, d->dt), &q_out, true));
     a.q_out = q_out.dev;
   }
   if (d->rotary_dim) {
-    B2_TRY(stage_in(d->positions, (size_t)T * 4, st, &p)); a.positions = (const int32_t *)p;
-    B2_TRY(stage_in(d->cos_table, table_bytes, st, &p)); a.cos_t = (const float *)p;
-    B2_TRY(stage_in(d->sin_table, table_bytes, st, &p)); a.sin_t = (const float *)p;
+    B2_TRY(g.in(d->positions, (size_t)T * 4, &a.positions));
+    B2_TRY(g.in(d->cos_table, table_bytes, &a.cos_t));
+    B2_TRY(g.in(d->sin_table, table_bytes, &a.sin_t));
   }
   for (int i = 0; i < 2; ++i) { a.qs[i] = d->q_stride[i]; a.ks[i] = d->k_stride[i]; a.vs[i] = d->v_stride[i]; a.os[i] = d->q_out_stride[i]; }
   for (int i = 0; i < 3; ++i) { a.ck[i] = c.key_stride[i]; a.cv[i] = c.value_stride[i]; a.cs[i] = c.scale_stride[i]; }
@@ -218,16 +211,17 @@ extern "C" int32_t b200dnn_paged_attention(const b200dnn_paged_attention_t *d, v
   B2_CHECK((int64_t)d->max_pages * c.page_size < (1ll << 30), B200DNN_UNIMPLEMENTED, "%s: sequences have less than 2^30 keys", who);
   B2_CHECK(d->q != d->out, B200DNN_FAILURE, "%s: out must not overlap q", who);
   B2_ENTER(stream);
-  B2_TRY(check_cache_here(who, c));
+  const Staging g{d->device, st, who};
+  B2_TRY(g.check());
+  B2_TRY(check_cache_here(g, c));
   PagedArgs a{};
-  const void *p;
   Staged out{}, lse{};
-  B2_TRY(stage_in(d->q, span2(B, d->q_heads, c.head_dim, d->q_stride, d->q_dt), st, &p)); a.q = (const uint16_t *)p;
-  B2_TRY(stage_in(d->page_table, (size_t)((B - 1) * d->page_table_ld + d->max_pages) * 4, st, &p)); a.table = (const int32_t *)p;
-  B2_TRY(stage_in(d->seq_lens, (size_t)B * 4, st, &p)); a.lens = (const int32_t *)p;
-  if (d->sinks) { B2_TRY(stage_in(d->sinks, (size_t)d->q_heads * 4, st, &p)); a.sinks = (const float *)p; }
-  B2_TRY(stage_out(d->out, span2(B, d->q_heads, c.head_dim, d->out_stride, d->out_dt), st, &out, true));
-  if (d->lse) B2_TRY(stage_out(d->lse, (size_t)B * d->q_heads * 4, st, &lse, true));
+  B2_TRY(g.in((const uint16_t *)d->q, span2(B, d->q_heads, c.head_dim, d->q_stride, d->q_dt), &a.q));
+  B2_TRY(g.in(d->page_table, (size_t)((B - 1) * d->page_table_ld + d->max_pages) * 4, &a.table));
+  B2_TRY(g.in(d->seq_lens, (size_t)B * 4, &a.lens));
+  if (d->sinks) B2_TRY(g.in(d->sinks, (size_t)d->q_heads * 4, &a.sinks));
+  B2_TRY(g.out(d->out, span2(B, d->q_heads, c.head_dim, d->out_stride, d->out_dt), &out, true));
+  if (d->lse) B2_TRY(g.out(d->lse, (size_t)B * d->q_heads * 4, &lse, true));
   a.out = out.dev; a.lse = d->lse ? (float *)lse.dev : nullptr;
   for (int i = 0; i < 2; ++i) { a.qs[i] = d->q_stride[i]; a.os[i] = d->out_stride[i]; }
   for (int i = 0; i < 3; ++i) { a.ck[i] = c.key_stride[i]; a.cv[i] = c.value_stride[i]; a.cs[i] = c.scale_stride[i]; }

@@ -555,6 +555,38 @@ inline int32_t finish_out(std::initializer_list<Staged *> outs, cudaStream_t st)
   return B200DNN_SUCCESS;
 }
 
+// The buffers of a call whose caller may vouch for where they lie (`device` of its descriptor: 0, or ordinal + 1).
+struct Staging {
+  int32_t device; cudaStream_t st; const char *who;
+  int32_t check() const {
+    B2_CHECK(device >= 0 && (device == 0 || device - 1 == rt().shared->dev), B200DNN_FAILURE, "%s: the descriptor is one of device %d, the current one is %d", who, device - 1,
+             rt().shared->dev);
+    return B200DNN_SUCCESS;
+  }
+  template <typename T> int32_t in(const T *p, size_t bytes, const T **out) const {
+    if (device) { *out = p; return B200DNN_SUCCESS; }
+    const void *d = nullptr;
+    B2_TRY(stage_in(p, bytes, st, &d));
+    *out = static_cast<const T *>(d);
+    return B200DNN_SUCCESS;
+  }
+  int32_t out(void *p, size_t bytes, Staged *s, bool preload = false) const {
+    if (!device) return stage_out(p, bytes, st, s, preload);
+    *s = Staged{};
+    s->dev = p;
+    return B200DNN_SUCCESS;
+  }
+  // buffers that are used where they lie
+  int32_t here(const char *what, const void *p) const {
+    if (device) return B200DNN_SUCCESS;
+    cudaPointerAttributes at;
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) { cudaGetLastError(); at.type = cudaMemoryTypeUnregistered; }
+    B2_CHECK(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, B200DNN_UNIMPLEMENTED, "%s: %s must be device memory", who, what);
+    B2_CHECK(at.type == cudaMemoryTypeManaged || at.device == rt().shared->dev, B200DNN_FAILURE, "%s: %s lies on device %d, the current one is %d", who, what, at.device, rt().shared->dev);
+    return B200DNN_SUCCESS;
+  }
+};
+
 inline size_t dt_size(int32_t dt) {
   switch (dt) { case B200DNN_F32: case B200DNN_S32: return 4; case B200DNN_BF16: return 2; case B200DNN_S8: case B200DNN_U8: return 1; default: return 0; }
 }
