@@ -192,3 +192,17 @@ def test_host_arrays(capi):
     host = Cache(2, 16, 2, dim, "bf16", device="cpu")
     rc = run(capi, capi.lib.b200dnn_kv_append, capi.make_kv_append(host.desc(capi), k, v, slots))
     assert rc == capi.UNIMPLEMENTED and "device memory" in capi.last_error()
+
+
+def test_a_descriptor_of_another_device_is_refused(capi):
+    k = torch.zeros(2, 1, 64, dtype=torch.bfloat16, device="cuda")
+    cache, slots = Cache(1, 16, 1, 64, "bf16"), torch.arange(2, device="cuda")
+    d = capi.make_kv_append(cache.desc(capi), k, k, slots)
+    assert d.device == torch.cuda.current_device() + 1
+    assert capi.make_kv_append(cache.desc(capi), k, k, slots.cpu()).device == 0
+    d.device += 1
+    assert run(capi, capi.lib.b200dnn_kv_append, d) == capi.FAILURE and "current one" in capi.last_error()
+    d.device = -3
+    assert run(capi, capi.lib.b200dnn_kv_append, d) == capi.FAILURE
+    d.device = 0
+    capi.check(run(capi, capi.lib.b200dnn_kv_append, d))

@@ -15,13 +15,17 @@ int32_t launch(void (*kern)(P...), unsigned grid, unsigned threads, size_t smem,
   return B200DNN_SUCCESS;
 }
 
-int32_t launch_gate(const GateArgs &a, unsigned grid, cudaStream_t st) {
-  if (a.E <= 32) return launch(gate_kernel<1>, grid, kGateThreads, 0, st, a);
-  if (a.E <= 64) return launch(gate_kernel<2>, grid, kGateThreads, 0, st, a);
-  if (a.E <= 128) return launch(gate_kernel<4>, grid, kGateThreads, 0, st, a);
-  if (a.E <= 256) return launch(gate_kernel<8>, grid, kGateThreads, 0, st, a);
-  if (a.E <= 512) return launch(gate_kernel<16>, grid, kGateThreads, 0, st, a);
-  return launch(gate_kernel<32>, grid, kGateThreads, 0, st, a);
+// Tokens of a CTA: one CTA up to 128 of them, else 32 and as many more as keep the chunks (whose counts every CTA of the second launch adds up) to 128.
+constexpr int kGateOneCta = 128, kGateChunks = 128;
+int32_t launch_gate(const GateArgs &a, const GateRowsArgs &r, unsigned grid, cudaStream_t st) {
+  const unsigned threads = (unsigned)std::min(kGateThreads, 32 * a.chunk);
+  const size_t smem = (size_t)a.E * 8 + (size_t)(threads / 32) * a.E;
+  if (a.E <= 32) return launch(gate_kernel<1>, grid, threads, smem, st, a, r);
+  if (a.E <= 64) return launch(gate_kernel<2>, grid, threads, smem, st, a, r);
+  if (a.E <= 128) return launch(gate_kernel<4>, grid, threads, smem, st, a, r);
+  if (a.E <= 256) return launch(gate_kernel<8>, grid, threads, smem, st, a, r);
+  if (a.E <= 512) return launch(gate_kernel<16>, grid, threads, smem, st, a, r);
+  return launch(gate_kernel<32>, grid, threads, smem, st, a, r);
 }
 
 }  // namespace
@@ -68,17 +72,16 @@ extern "C" int32_t b200dnn_moe_gate(const b200dnn_moe_gate_t *d, void *stream) {
   a.T = T; a.E = E; a.k = k; a.sigmoid = d->score == B200DNN_GATE_SIGMOID; a.groups = G; a.top_groups = d->topk_groups; a.per_group = E / G;
   a.top2 = d->group_score == B200DNN_GROUP_TOP2; a.renorm = d->renorm ? 1 : 0; a.scale = d->scale;
   a.ids = (int32_t *)ids.dev; a.weights = (float *)weights.dev;
-  a.chunk = std::max(8, (T + 2 * rt().sm_count - 1) / (2 * rt().sm_count));
+  a.chunk = T <= kGateOneCta ? T : std::max(32, (T + kGateChunks - 1) / kGateChunks);
   const unsigned grid = (unsigned)((T + a.chunk - 1) / a.chunk);
-  const bool want_rows = d->expert_counts || d->slot_to_row;
-  if (want_rows) {
+  GateRowsArgs r{a.ids, nullptr, T, E, k, a.chunk, (int32_t *)counts.dev, (int32_t *)rows.dev};
+  const bool second = grid > 1 && (d->expert_counts || d->slot_to_row);
+  if (second) {
     a.counts = (int32_t *)rt().ws.alloc((size_t)grid * E * 4);
     B2_CHECK(a.counts, B200DNN_FAILURE, "workspace allocation failed");
+    r.counts = a.counts;
   }
-  B2_TRY(launch_gate(a, grid, st));
-  if (want_rows) {
-    GateRowsArgs r{a.ids, a.counts, T, E, k, a.chunk, (int32_t *)counts.dev, (int32_t *)rows.dev};
-    B2_TRY(launch(gate_rows_kernel, grid, kGateRowsThreads, (size_t)34 * E * 4, st, r));
-  }
+  B2_TRY(launch_gate(a, grid > 1 ? GateRowsArgs{} : r, grid, st));
+  if (second) B2_TRY(launch(gate_rows_kernel, grid, kGateThreads, (size_t)E * (8 + 32), st, r));
   return finish_out({&ids, &weights, &counts, &rows}, st);
 }

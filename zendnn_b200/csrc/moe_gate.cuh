@@ -39,9 +39,16 @@ __device__ __forceinline__ GateTop gate_best(GateTop t) {
   return t;
 }
 
-// A warp's token in 64 bits.  x[j]: logit of expert 32 j + lane.  Lane i < k returns the i-th choice and its score.
+__device__ __forceinline__ float gate_logit(const GateArgs &a, int64_t at) {
+  return a.logits_bf16 ? bf16_bits_to_f32(__ldg(reinterpret_cast<const uint16_t *>(a.logits) + at)) : __ldg(reinterpret_cast<const float *>(a.logits) + at);
+}
+
+// A warp's token in 64 bits, expert 32 j + lane in element j.  Lane i < k returns the i-th choice and its score.
 template <int PER>
-__device__ __forceinline__ void gate_token(const GateArgs &a, const float (&x)[PER], int lane, int &id, double &score) {
+__device__ __noinline__ void gate_token(const GateArgs &a, int t, int lane, int &id, double &score) {
+  float x[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) x[j] = j * 32 + lane < a.E ? gate_logit(a, t * a.ld + j * 32 + lane) : 0.f;
   double s[PER];
   if (a.sigmoid) {
 #pragma unroll
@@ -111,91 +118,274 @@ __device__ __forceinline__ void gate_token(const GateArgs &a, const float (&x)[P
   }
 }
 
-constexpr int kGateThreads = 256;
+// The same in 32 bits, where these are enough.  f32 scores carry errors of a few steps, and the choice is taken for the one that 64 bits would make when every comparison that decides it is clear
+// by more than these: between neighbours among the chosen, between the last of them and the best that is left, between the last chosen group and the next.
+// (Experts with one logit and one bias have one score in either width, and go by their index.)  False: the token is one for gate_token; about one in 300 over 256 experts
+// with continuous logits.  Returns the weights' scores in f32, and the sum of the chosen is left to the caller.
+__device__ __forceinline__ uint32_t gate_key(float c) {
+  if (c != c) return 1u;
+  const uint32_t b = __float_as_uint(c);
+  return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float gate_value(uint32_t key) {
+  return key <= 1u ? __int_as_float(0x7fc00000) : __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
+}
+template <int N> __device__ __forceinline__ float gate_sum(const float (&v)[N]) {
+  if constexpr (N == 1) return v[0];
+  else {
+    float h[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) h[i] = v[2 * i] + v[2 * i + 1];
+    return gate_sum<N / 2>(h);
+  }
+}
 template <int PER>
-__global__ void __launch_bounds__(kGateThreads) gate_kernel(const GateArgs a) {
-  __shared__ int hist[PER * 32];
+__device__ __forceinline__ bool gate_token_f32(const GateArgs &a, const float (&x)[PER], const float (&bias)[PER], int lane, int &id, float &score) {
+  const unsigned all = 0xffffffffu;
+  float mx = 0.f, sum = 1.f, most = 1.f;       // of the softmax: largest logit, denominator; bound of the scores
+  uint32_t key[PER];
+  {
+    float s[PER];
+    if (a.sigmoid) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) s[j] = __fdividef(1.0f, 1.0f + expf(-x[j]));
+    } else {
+      mx = __int_as_float(0xff800000);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) if (j * 32 + lane < a.E) mx = fmaxf(mx, x[j]);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(all, mx, o));
+#pragma unroll
+      for (int j = 0; j < PER; ++j) s[j] = j * 32 + lane < a.E ? expf(x[j] - mx) : 0.f;
+      sum = gate_sum<PER>(s);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(all, sum, o);
+      most = __fdividef(1.0f, sum);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) s[j] *= most;
+      // (a NaN, an infinity, or minus infinity throughout: there is no softmax)
+      if (!(sum >= 1.0f && sum < 3e38f)) return false;
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) key[j] = j * 32 + lane < a.E ? gate_key(s[j] + bias[j]) : 0u;
+  }
+  // errors: a sigmoid is off by 6e-7 of itself; a softmax by 5e-6 and by 6e-8 for every unit between logit and maximum (the difference's rounding); a sum by its rounding
+  const float off = a.sigmoid ? 7e-7f : 5e-6f;
+  bool clear = true;
+  if (a.groups > 1) {
+    uint32_t mine = 0u;                        // lane g: group g's score
+    const unsigned per = (unsigned)a.per_group;
+    auto best_two = [&](uint32_t t1, uint32_t t2, int g) {      // of a lane's members
+      const uint32_t m1 = __reduce_max_sync(all, t1);
+      uint32_t value = m1;
+      if (a.top2) {
+        const bool first = lane == __ffs(__ballot_sync(all, t1 == m1)) - 1;
+        const uint32_t m2 = __reduce_max_sync(all, first ? t2 : t1);
+        if (m2 != 0u) value = gate_key(gate_value(m1) + gate_value(m2));
+      }
+      if (lane == g) mine = value;
+    };
+    if (per % 32 == 0) {                       // whole elements of all lanes
+      const int elements = (int)per / 32;
+      uint32_t t1 = 0u, t2 = 0u;
+      int left = elements, g = 0;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        if (j * 32 < a.E) {
+          t2 = max(t2, min(t1, key[j]));
+          t1 = max(t1, key[j]);
+          if (--left == 0) { best_two(t1, t2, g++); t1 = t2 = 0u; left = elements; }
+        }
+      }
+    } else {
+      for (int g = 0; g < a.groups; ++g) {
+        uint32_t t1 = 0u, t2 = 0u;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          const uint32_t k = (unsigned)(j * 32 + lane) - (unsigned)g * per < per ? key[j] : 0u;
+          t2 = max(t2, min(t1, k));
+          t1 = max(t1, k);
+        }
+        best_two(t1, t2, g);
+      }
+    }
+    int rank = 0;
+    for (int g = 0; g < a.groups; ++g) {
+      const uint32_t other = __shfl_sync(all, mine, g);
+      rank += other > mine || (other == mine && g < lane);
+    }
+    const unsigned chosen = __ballot_sync(all, lane < a.groups && rank < a.top_groups);
+    if (a.top_groups < a.groups) {
+      const int last = __ffs(__ballot_sync(all, lane < a.groups && rank == a.top_groups - 1)) - 1, next = __ffs(__ballot_sync(all, lane < a.groups && rank == a.top_groups)) - 1;
+      const float u = gate_value(__shfl_sync(all, mine, last)), v = gate_value(__shfl_sync(all, mine, next));
+      clear = u - v > 2.f * (off + 6e-6f * (a.sigmoid ? 0.f : 1.f)) * most + 3e-7f * (fabsf(u) + fabsf(v)) + 1e-36f;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const unsigned e = (unsigned)(j * 32 + lane);
+        const unsigned g = per % 32 == 0 ? (unsigned)j / (per / 32) : e / per;
+        if (!((chosen >> (g & 31)) & 1u)) key[j] = 0u;
+      }
+    }
+  }
+  // the choice, and the best that is left behind it
+  const int rounds = a.k + (a.k < a.top_groups * a.per_group);
+  uint32_t my_key = 0u; int my_id = 0;
+  for (int r = 0; r < rounds; ++r) {
+    uint32_t best = key[0]; int at = 0;
+#pragma unroll
+    for (int j = 1; j < PER; ++j) if (key[j] > best) { best = key[j]; at = j; }
+    const uint32_t top = __reduce_max_sync(all, best);
+    const int e = __reduce_min_sync(all, best == top ? (unsigned)(at * 32 + lane) : 0x7fffffffu);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) if (e == j * 32 + lane) key[j] = 0u;
+    if (lane == r) { my_key = top; my_id = e; }
+  }
+  // logit and bias of my choice
+  float my_x = 0.f, my_b = 0.f;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const float vx = __shfl_sync(all, x[j], my_id & 31), vb = __shfl_sync(all, bias[j], my_id & 31);
+    if (my_id >> 5 == j) { my_x = vx; my_b = vb; }
+  }
+  if (a.sigmoid) score = __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-my_x)));
+  else {
+    // the difference, and what its rounding left out
+    const float d = __fsub_rn(my_x, mx), back = __fsub_rn(d, my_x), rest = __fsub_rn(__fsub_rn(my_x, __fsub_rn(d, back)), __fadd_rn(mx, back));
+    score = __fdiv_rn(expf(d) * (1.0f + rest), sum);
+  }
+  {
+    const float c = gate_value(my_key), c2 = __shfl_down_sync(all, c, 1), x2 = __shfl_down_sync(all, my_x, 1), b2 = __shfl_down_sync(all, my_b, 1), s2 = __shfl_down_sync(all, score, 1);
+    const bool same = my_x == x2 && my_b == b2;
+    const float err = a.sigmoid ? off : off + 6e-8f * fmaxf(mx - my_x, mx - x2);
+    const bool apart = c - c2 > 2.f * err * fmaxf(score, s2) + 3e-7f * (fabsf(c) + fabsf(c2)) + 1e-36f;
+    if (lane + 1 < rounds && !same && !apart) clear = false;
+  }
+  id = my_id;
+  return __all_sync(all, clear);
+}
+
+// Slots' places: rank of each of a chunk's slots inside its expert, behind next[e] rows.  All threads of a CTA of 1024; cnt: [32 warps][E] bytes.
+__device__ __forceinline__ void gate_places(const int32_t *ids, int64_t s0, int64_t s_end, int E, int *next, uint8_t *cnt, int32_t *slot_to_row) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  for (; s0 < s_end; s0 += blockDim.x) {
+    for (int i = tid; i < warps * E; i += blockDim.x) cnt[i] = 0;
+    __syncthreads();
+    const int64_t s = s0 + tid;
+    const int e = s < s_end ? ids[s] : -1;
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    const int before = __popc(same & ((1u << lane) - 1u));
+    if (e >= 0 && before == 0) cnt[warp * E + e] = (uint8_t)__popc(same);
+    __syncthreads();
+    if (e >= 0) {
+      int row = next[e] + before;
+      for (int w = 0; w < warp; ++w) row += cnt[w * E + e];
+      slot_to_row[s] = row;
+    }
+    __syncthreads();
+    for (int i = tid; i < E; i += blockDim.x) { int n = 0; for (int w = 0; w < warps; ++w) n += cnt[w * E + i]; next[i] += n; }
+    __syncthreads();
+  }
+}
+// next[e] += rows of the experts in front of e (one warp)
+__device__ __forceinline__ void gate_offsets(const int *total, int *next, int E) {
+  const int lane = threadIdx.x & 31;
+  int carry = 0;
+  for (int base = 0; base < E; base += 32) {
+    const int e = base + lane, n = e < E ? total[e] : 0;
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += v; }
+    if (e < E) next[e] += carry + sum - n;
+    carry += __shfl_sync(0xffffffffu, sum, 31);
+  }
+}
+
+// A CTA per chunk of tokens, a warp per token.  With a single chunk the places follow at once.
+struct GateRowsArgs { const int32_t *ids, *counts; int T, E, k, chunk; int32_t *expert_counts, *slot_to_row; };
+constexpr int kGateThreads = 1024;
+template <int PER>
+__global__ void __launch_bounds__(kGateThreads) gate_kernel(const GateArgs a, const GateRowsArgs rows) {
+  extern __shared__ int sm[];
+  int *hist = sm, *next = sm + a.E;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t0 = blockIdx.x * a.chunk, t1 = min(a.T, t0 + a.chunk);
-  if (a.counts) {
-    for (int i = threadIdx.x; i < a.E; i += kGateThreads) hist[i] = 0;
+  const bool count = a.counts || rows.expert_counts || rows.slot_to_row;
+  if (count) {
+    for (int i = threadIdx.x; i < a.E; i += blockDim.x) hist[i] = next[i] = 0;
     __syncthreads();
   }
-  for (int t = t0 + warp; t < t1; t += kGateThreads / 32) {
+  float bias[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) bias[j] = a.bias && j * 32 + lane < a.E ? a.bias[j * 32 + lane] : 0.f;
+  for (int t = t0 + warp; t < t1; t += (int)(blockDim.x >> 5)) {
     float x[PER];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const int e = j * 32 + lane;
-      x[j] = e < a.E ? load_as_f32(a.logits, a.logits_bf16 ? DT_BF16 : DT_F32, t * a.ld + e) : 0.f;
+    for (int j = 0; j < PER; ++j) x[j] = j * 32 + lane < a.E ? gate_logit(a, t * a.ld + j * 32 + lane) : 0.f;
+    int id; float w;
+    if (gate_token_f32<PER>(a, x, bias, lane, id, w)) {
+      if (a.renorm) {
+        float sum = lane < a.k ? w : 0.f;
+#pragma unroll
+        for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        w = __fdiv_rn(w, sum);
+      }
+      w *= a.scale;
+    } else {
+      double score, sum = 0.0;
+      gate_token<PER>(a, t, lane, id, score);
+      for (int r = 0; r < a.k; ++r) sum += __shfl_sync(0xffffffffu, score, r);
+      w = (float)((a.renorm ? score / sum : score) * (double)a.scale);
     }
-    int id; double score;
-    gate_token<PER>(a, x, lane, id, score);
-    double sum = 0.0;
-    for (int r = 0; r < a.k; ++r) sum += __shfl_sync(0xffffffffu, score, r);
     if (lane < a.k) {
       a.ids[(int64_t)t * a.k + lane] = id;
-      if (a.weights) a.weights[(int64_t)t * a.k + lane] = (float)((a.renorm ? score / sum : score) * (double)a.scale);
-      if (a.counts) atomicAdd(&hist[id], 1);
+      if (a.weights) a.weights[(int64_t)t * a.k + lane] = w;
+      if (count) atomicAdd(&hist[id], 1);
     }
   }
+  if (!count) return;
+  __syncthreads();
   if (a.counts) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.E; i += kGateThreads) a.counts[(int64_t)blockIdx.x * a.E + i] = hist[i];
+    for (int i = threadIdx.x; i < a.E; i += blockDim.x) a.counts[(int64_t)blockIdx.x * a.E + i] = hist[i];
+    return;
   }
+  if (rows.expert_counts) for (int i = threadIdx.x; i < a.E; i += blockDim.x) rows.expert_counts[i] = hist[i];
+  if (!rows.slot_to_row) return;
+  if (warp == 0) gate_offsets(hist, next, a.E);
+  gate_places(a.ids, 0, (int64_t)a.T * a.k, a.E, next, reinterpret_cast<uint8_t *>(next + a.E), rows.slot_to_row);
 }
 
 // The slots' places in the stable order by expert, from the counts of the chunks: every CTA adds up those of all chunks (first rows of the experts) and of the chunks
 // in front of it, then ranks its own slots inside their experts.
-struct GateRowsArgs { const int32_t *ids, *counts; int T, E, k, chunk; int32_t *expert_counts, *slot_to_row; };
-constexpr int kGateRowsThreads = 1024;
-__global__ void __launch_bounds__(kGateRowsThreads) gate_rows_kernel(const GateRowsArgs a) {
+__global__ void __launch_bounds__(kGateThreads) gate_rows_kernel(const GateRowsArgs a) {
   extern __shared__ int sm[];
-  int *next = sm, *total = sm + a.E, *cnt = sm + 2 * a.E;          // this chunk's next row of each expert; all rows; [32 warps][E]
+  int *next = sm, *total = sm + a.E;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, me = blockIdx.x, chunks = gridDim.x;
-  const int64_t s_end = min((int64_t)a.T, (int64_t)(me + 1) * a.chunk) * a.k;
-  for (int e = tid; e < a.E; e += kGateRowsThreads) { next[e] = 0; total[e] = 0; }
+  const int tid = threadIdx.x, warp = tid >> 5, me = blockIdx.x, chunks = gridDim.x;
+  for (int e = tid; e < a.E; e += kGateThreads) next[e] = total[e] = 0;
   __syncthreads();
-  for (int i = tid; i < chunks * a.E; i += kGateRowsThreads) {
-    const int c = i / a.E, e = i - c * a.E, n = a.counts[i];
-    if (n) { atomicAdd(&total[e], n); if (c < me) atomicAdd(&next[e], n); }
-  }
-  __syncthreads();
-  if (warp == 0) {
-    int carry = 0;
-    for (int base = 0; base < a.E; base += 32) {
-      const int e = base + lane, n = e < a.E ? total[e] : 0;
-      int sum = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += v; }
-      if (e < a.E) next[e] += carry + sum - n;
-      carry += __shfl_sync(0xffffffffu, sum, 31);
+  {
+    // parts of the chunks side by side, a thread per expert in each
+    const int parts = kGateThreads / a.E, e = tid % a.E, part = tid / a.E;      // (E <= 1024)
+    if (part < parts) {
+      int all = 0, before = 0;
+#pragma unroll 8
+      for (int c = part; c < chunks; c += parts) {
+        const int n = a.counts[(int64_t)c * a.E + e];
+        all += n;
+        before += c < me ? n : 0;
+      }
+      if (all) atomicAdd(&total[e], all);
+      if (before) atomicAdd(&next[e], before);
     }
   }
+  __syncthreads();
   if (me == 0 && a.expert_counts)
-    for (int e = tid; e < a.E; e += kGateRowsThreads) a.expert_counts[e] = total[e];
+    for (int e = tid; e < a.E; e += kGateThreads) a.expert_counts[e] = total[e];
   if (!a.slot_to_row) return;
-  __syncthreads();
-  for (int64_t s0 = (int64_t)me * a.chunk * a.k; s0 < s_end; s0 += kGateRowsThreads) {
-    for (int i = tid; i < 32 * a.E; i += kGateRowsThreads) cnt[i] = 0;
-    __syncthreads();
-    const int64_t s = s0 + tid;
-    const int e = s < s_end ? a.ids[s] : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    const int before = __popc(same & ((1u << lane) - 1u));
-    if (e >= 0 && before == 0) cnt[warp * a.E + e] = __popc(same);
-    __syncthreads();
-    if (e >= 0) {
-      int row = next[e] + before;
-      for (int w = 0; w < warp; ++w) row += cnt[w * a.E + e];
-      a.slot_to_row[s] = row;
-    }
-    __syncthreads();
-    for (int i = tid; i < a.E; i += kGateRowsThreads) { int n = 0; for (int w = 0; w < 32; ++w) n += cnt[w * a.E + i]; next[i] += n; }
-    __syncthreads();
-  }
+  if (warp == 0) gate_offsets(total, next, a.E);
+  gate_places(a.ids, (int64_t)me * a.chunk * a.k, min((int64_t)a.T, (int64_t)(me + 1) * a.chunk) * a.k, a.E, next, reinterpret_cast<uint8_t *>(sm + 2 * a.E), a.slot_to_row);
 }
 
 }  // namespace b200
