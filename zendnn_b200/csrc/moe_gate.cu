@@ -15,10 +15,10 @@ int32_t launch(void (*kern)(P...), unsigned grid, unsigned threads, size_t smem,
   return B200DNN_SUCCESS;
 }
 
-// Tokens of a CTA: one CTA up to 128 of them, else 32 and as many more as keep the chunks (whose counts every CTA of the second launch adds up) to 128.
-constexpr int kGateOneCta = 128, kGateChunks = 128;
+// Tokens of a CTA: one CTA up to 128 of them, else 32 and as many more as leave a CTA for every SM (every CTA of the second launch adds up the counts of all).
+constexpr int kGateOneCta = 128;
 int32_t launch_gate(const GateArgs &a, const GateRowsArgs &r, unsigned grid, cudaStream_t st) {
-  const unsigned threads = (unsigned)std::min(kGateThreads, 32 * a.chunk);
+  const unsigned threads = (unsigned)std::min(a.E <= 256 ? kGateTokenThreads<8> : kGateTokenThreads<32>, 32 * a.chunk);
   const size_t smem = (size_t)a.E * 8 + (size_t)(threads / 32) * a.E;
   if (a.E <= 32) return launch(gate_kernel<1>, grid, threads, smem, st, a, r);
   if (a.E <= 64) return launch(gate_kernel<2>, grid, threads, smem, st, a, r);
@@ -72,7 +72,7 @@ extern "C" int32_t b200dnn_moe_gate(const b200dnn_moe_gate_t *d, void *stream) {
   a.T = T; a.E = E; a.k = k; a.sigmoid = d->score == B200DNN_GATE_SIGMOID; a.groups = G; a.top_groups = d->topk_groups; a.per_group = E / G;
   a.top2 = d->group_score == B200DNN_GROUP_TOP2; a.renorm = d->renorm ? 1 : 0; a.scale = d->scale;
   a.ids = (int32_t *)ids.dev; a.weights = (float *)weights.dev;
-  a.chunk = T <= kGateOneCta ? T : std::max(32, (T + kGateChunks - 1) / kGateChunks);
+  a.chunk = T <= kGateOneCta ? T : std::max(32, (T + rt().sm_count - 1) / rt().sm_count);
   const unsigned grid = (unsigned)((T + a.chunk - 1) / a.chunk);
   GateRowsArgs r{a.ids, nullptr, T, E, k, a.chunk, (int32_t *)counts.dev, (int32_t *)rows.dev};
   const bool second = grid > 1 && (d->expert_counts || d->slot_to_row);

@@ -27,16 +27,12 @@ __device__ __forceinline__ unsigned long long gate_key(double c) {
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-struct GateTop { unsigned long long key; int id; };
-// the largest key of the warp, ties to the lower id
-__device__ __forceinline__ GateTop gate_best(GateTop t) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const unsigned long long key = __shfl_xor_sync(0xffffffffu, t.key, o);
-    const int id = __shfl_xor_sync(0xffffffffu, t.id, o);
-    if (key > t.key || (key == t.key && id < t.id)) { t.key = key; t.id = id; }
-  }
-  return t;
+// The largest key of the warp and the lowest of the ids that lanes name for it (the key as two words: each a reduction in hardware).
+__device__ __forceinline__ void gate_best(unsigned long long &key, int &id) {
+  const unsigned all = 0xffffffffu, hi = (unsigned)(key >> 32), lo = (unsigned)key;
+  const unsigned top_hi = __reduce_max_sync(all, hi), top_lo = __reduce_max_sync(all, hi == top_hi ? lo : 0u);
+  id = (int)__reduce_min_sync(all, hi == top_hi && lo == top_lo ? (unsigned)id : 0x7fffffffu);
+  key = (unsigned long long)top_hi << 32 | top_lo;
 }
 
 __device__ __forceinline__ float gate_logit(const GateArgs &a, int64_t at) {
@@ -80,17 +76,16 @@ __device__ __noinline__ void gate_token(const GateArgs &a, int t, int lane, int 
       double total = 0.0;
       int first = -1;
       for (int r = 0; r <= a.top2; ++r) {
-        GateTop t{0ull, 0x7fffffff};
+        unsigned long long top = 0ull; int id_of = 0x7fffffff;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
           const int e = j * 32 + lane;
-          if (e / a.per_group == g && e != first && key[j] > t.key) t = GateTop{key[j], e};
+          if ((unsigned)(e - g * a.per_group) < (unsigned)a.per_group && e != first && key[j] > top) { top = key[j]; id_of = e; }
         }
-        t = gate_best(t);
-        if (t.key == 0ull) break;            // a group of one expert
-        first = t.id;
-        const double c = t.key == 1ull ? __longlong_as_double(0x7ff8000000000000ll)
-                                       : __longlong_as_double((long long)(t.key >> 63 ? t.key & 0x7fffffffffffffffull : ~t.key));
+        gate_best(top, id_of);
+        if (top == 0ull) break;              // a group of one expert
+        first = id_of;
+        const double c = top == 1ull ? __longlong_as_double(0x7ff8000000000000ll) : __longlong_as_double((long long)(top >> 63 ? top & 0x7fffffffffffffffull : ~top));
         total = r == 0 ? c : total + c;
       }
       if (lane == g) mine = gate_key(total);
@@ -106,15 +101,15 @@ __device__ __noinline__ void gate_token(const GateArgs &a, int t, int lane, int 
   }
   id = 0; score = 0.0;
   for (int r = 0; r < a.k; ++r) {
-    GateTop t{0ull, 0x7fffffff};
+    unsigned long long top = 0ull; int id_of = 0x7fffffff;
     double v = 0.0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) if (key[j] > t.key) { t = GateTop{key[j], j * 32 + lane}; v = s[j]; }
-    t = gate_best(t);
-    v = __shfl_sync(0xffffffffu, v, t.id & 31);
+    for (int j = 0; j < PER; ++j) if (key[j] > top) { top = key[j]; id_of = j * 32 + lane; v = s[j]; }
+    gate_best(top, id_of);
+    v = __shfl_sync(0xffffffffu, v, id_of & 31);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) if (t.id == j * 32 + lane) key[j] = 0ull;
-    if (lane == r) { id = t.id; score = v; }
+    for (int j = 0; j < PER; ++j) if (id_of == j * 32 + lane) key[j] = 0ull;
+    if (lane == r) { id = id_of; score = v; }
   }
 }
 
@@ -139,8 +134,26 @@ template <int N> __device__ __forceinline__ float gate_sum(const float (&v)[N]) 
     return gate_sum<N / 2>(h);
   }
 }
+// Sorts PER keys of a lane, largest first (Batcher's odd-even merge sort, 1968; PER a power of two).
+template <int PER> __device__ __forceinline__ void gate_sort(uint32_t (&v)[PER]) {
+#pragma unroll
+  for (int p = 1; p < PER; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < PER; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < PER && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const uint32_t lo = min(v[i + j], v[i + j + k]);
+            v[i + j] = max(v[i + j], v[i + j + k]);
+            v[i + j + k] = lo;
+          }
+}
+
+// group_of: groups of the lane's experts, a byte each
 template <int PER>
-__device__ __forceinline__ bool gate_token_f32(const GateArgs &a, const float (&x)[PER], const float (&bias)[PER], int lane, int &id, float &score) {
+__device__ __forceinline__ bool gate_token_f32(const GateArgs &a, const float (&x)[PER], const float (&bias)[PER], const uint32_t (&group_of)[(PER + 3) / 4], int lane, int &id, float &score) {
   const unsigned all = 0xffffffffu;
   float mx = 0.f, sum = 1.f, most = 1.f;       // of the softmax: largest logit, denominator; bound of the scores
   uint32_t key[PER];
@@ -173,17 +186,16 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, const float (&
   const float off = a.sigmoid ? 7e-7f : 5e-6f;
   bool clear = true;
   if (a.groups > 1) {
-    uint32_t mine = 0u;                        // lane g: group g's score
+    uint32_t first = 0u, second = 0u;          // lane g: the two largest keys of group g
     const unsigned per = (unsigned)a.per_group;
     auto best_two = [&](uint32_t t1, uint32_t t2, int g) {      // of a lane's members
       const uint32_t m1 = __reduce_max_sync(all, t1);
-      uint32_t value = m1;
+      if (lane == g) first = m1;
       if (a.top2) {
-        const bool first = lane == __ffs(__ballot_sync(all, t1 == m1)) - 1;
-        const uint32_t m2 = __reduce_max_sync(all, first ? t2 : t1);
-        if (m2 != 0u) value = gate_key(gate_value(m1) + gate_value(m2));
+        const bool mine = lane == __ffs(__ballot_sync(all, t1 == m1)) - 1;
+        const uint32_t m2 = __reduce_max_sync(all, mine ? t2 : t1);
+        if (lane == g) second = m2;
       }
-      if (lane == g) mine = value;
     };
     if (per % 32 == 0) {                       // whole elements of all lanes
       const int elements = (int)per / 32;
@@ -209,6 +221,8 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, const float (&
         best_two(t1, t2, g);
       }
     }
+    // (a group of one expert has no second)
+    const uint32_t mine = second ? gate_key(gate_value(first) + gate_value(second)) : first;
     int rank = 0;
     for (int g = 0; g < a.groups; ++g) {
       const uint32_t other = __shfl_sync(all, mine, g);
@@ -218,34 +232,55 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, const float (&
     if (a.top_groups < a.groups) {
       const int last = __ffs(__ballot_sync(all, lane < a.groups && rank == a.top_groups - 1)) - 1, next = __ffs(__ballot_sync(all, lane < a.groups && rank == a.top_groups)) - 1;
       const float u = gate_value(__shfl_sync(all, mine, last)), v = gate_value(__shfl_sync(all, mine, next));
-      clear = u - v > 2.f * (off + 6e-6f * (a.sigmoid ? 0.f : 1.f)) * most + 3e-7f * (fabsf(u) + fabsf(v)) + 1e-36f;
+      clear = u - v > 2.f * (off + (a.sigmoid ? 0.f : 6e-6f)) * most + 3e-7f * (fabsf(u) + fabsf(v)) + 1e-36f;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const unsigned e = (unsigned)(j * 32 + lane);
-        const unsigned g = per % 32 == 0 ? (unsigned)j / (per / 32) : e / per;
-        if (!((chosen >> (g & 31)) & 1u)) key[j] = 0u;
-      }
+      for (int j = 0; j < PER; ++j) if (!((chosen >> ((group_of[j / 4] >> (j % 4 * 8)) & 31u)) & 1u)) key[j] = 0u;
     }
   }
-  // the choice, and the best that is left behind it
+  // The choice, and the best that is left behind it: every lane's keys in order, the largest head of all lanes taken again and again.
   const int rounds = a.k + (a.k < a.top_groups * a.per_group);
-  uint32_t my_key = 0u; int my_id = 0;
+  uint32_t head[PER], my_key = 0u;
+  int my_id = 0, my_lane = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) head[j] = key[j];
+  gate_sort<PER>(head);
   for (int r = 0; r < rounds; ++r) {
-    uint32_t best = key[0]; int at = 0;
+    const uint32_t top = __reduce_max_sync(all, head[0]);
+    const int from = __ffs(__ballot_sync(all, head[0] == top)) - 1;
+    if (lane == from) {
 #pragma unroll
-    for (int j = 1; j < PER; ++j) if (key[j] > best) { best = key[j]; at = j; }
-    const uint32_t top = __reduce_max_sync(all, best);
-    const int e = __reduce_min_sync(all, best == top ? (unsigned)(at * 32 + lane) : 0x7fffffffu);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) if (e == j * 32 + lane) key[j] = 0u;
-    if (lane == r) { my_key = top; my_id = e; }
+      for (int j = 0; j + 1 < PER; ++j) head[j] = head[j + 1];
+      head[PER - 1] = 0u;
+    }
+    if (lane == r) { my_key = top; my_lane = from; }
   }
-  // logit and bias of my choice
   float my_x = 0.f, my_b = 0.f;
+  const uint32_t key_behind = __shfl_down_sync(all, my_key, 1);
+  if (!__any_sync(all, lane + 1 < rounds && my_key == key_behind)) {
+    // which of its lane's experts a choice is, with its logit and bias
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const float vx = __shfl_sync(all, x[j], my_id & 31), vb = __shfl_sync(all, bias[j], my_id & 31);
-    if (my_id >> 5 == j) { my_x = vx; my_b = vb; }
+    for (int j = 0; j < PER; ++j) {
+      const uint32_t k = __shfl_sync(all, key[j], my_lane);
+      const float vx = __shfl_sync(all, x[j], my_lane), vb = __shfl_sync(all, bias[j], my_lane);
+      if (k == my_key) { my_id = j * 32 + my_lane; my_x = vx; my_b = vb; }
+    }
+  } else {
+    // equal keys: the lowest index of the largest key, again and again
+    for (int r = 0; r < rounds; ++r) {
+      uint32_t best = key[0]; int at = 0;
+#pragma unroll
+      for (int j = 1; j < PER; ++j) if (key[j] > best) { best = key[j]; at = j; }
+      const uint32_t top = __reduce_max_sync(all, best);
+      const int e = __reduce_min_sync(all, best == top ? (unsigned)(at * 32 + lane) : 0x7fffffffu);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) if (e == j * 32 + lane) key[j] = 0u;
+      if (lane == r) my_id = e;
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const float vx = __shfl_sync(all, x[j], my_id & 31), vb = __shfl_sync(all, bias[j], my_id & 31);
+      if (my_id >> 5 == j) { my_x = vx; my_b = vb; }
+    }
   }
   if (a.sigmoid) score = __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-my_x)));
   else {
@@ -303,8 +338,9 @@ __device__ __forceinline__ void gate_offsets(const int *total, int *next, int E)
 // A CTA per chunk of tokens, a warp per token.  With a single chunk the places follow at once.
 struct GateRowsArgs { const int32_t *ids, *counts; int T, E, k, chunk; int32_t *expert_counts, *slot_to_row; };
 constexpr int kGateThreads = 1024;
+template <int PER> constexpr int kGateTokenThreads = PER <= 8 ? 1024 : 512;      // (registers for PER experts a lane)
 template <int PER>
-__global__ void __launch_bounds__(kGateThreads) gate_kernel(const GateArgs a, const GateRowsArgs rows) {
+__global__ void __launch_bounds__(kGateTokenThreads<PER>) gate_kernel(const GateArgs a, const GateRowsArgs rows) {
   extern __shared__ int sm[];
   int *hist = sm, *next = sm + a.E;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -318,12 +354,22 @@ __global__ void __launch_bounds__(kGateThreads) gate_kernel(const GateArgs a, co
   float bias[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) bias[j] = a.bias && j * 32 + lane < a.E ? a.bias[j * 32 + lane] : 0.f;
+  uint32_t group_of[(PER + 3) / 4] = {};
+#pragma unroll
+  for (int j = 0; j < PER; ++j) group_of[j / 4] |= (uint32_t)(min(j * 32 + lane, a.E - 1) / a.per_group) << (j % 4 * 8);
   for (int t = t0 + warp; t < t1; t += (int)(blockDim.x >> 5)) {
     float x[PER];
+    if (a.logits_bf16) {
+      const uint16_t *p = reinterpret_cast<const uint16_t *>(a.logits) + t * a.ld + lane;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) x[j] = j * 32 + lane < a.E ? gate_logit(a, t * a.ld + j * 32 + lane) : 0.f;
+      for (int j = 0; j < PER; ++j) x[j] = j * 32 + lane < a.E ? bf16_bits_to_f32(__ldg(p + j * 32)) : 0.f;
+    } else {
+      const float *p = reinterpret_cast<const float *>(a.logits) + t * a.ld + lane;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) x[j] = j * 32 + lane < a.E ? __ldg(p + j * 32) : 0.f;
+    }
     int id; float w;
-    if (gate_token_f32<PER>(a, x, bias, lane, id, w)) {
+    if (gate_token_f32<PER>(a, x, bias, group_of, lane, id, w)) {
       if (a.renorm) {
         float sum = lane < a.k ? w : 0.f;
 #pragma unroll
