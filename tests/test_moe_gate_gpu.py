@@ -95,6 +95,17 @@ def test_far_apart_and_infinite_logits(capi, score):
         check(capi, x, 6, b, score, 8, 4, "top2", False, 1.0)
 
 
+@pytest.mark.parametrize("E,k,groups,top", [(33, 11, 3, 1), (33, 3, 11, 1), (40, 8, 1, 1), (45, 15, 3, 1)])
+def test_biases_of_minus_infinity(capi, E, k, groups, top):
+    """Experts that a bias takes out are chosen last, by their index, and nothing behind the last expert is."""
+    x = logits(50, E, seed=4)
+    bias = np.zeros(E, np.float32)
+    bias[E // 2:] = -np.inf
+    for score in ("softmax", "sigmoid"):
+        check(capi, x, k, bias, score, groups, top, "max", False, 1.0)
+        check(capi, x, k, np.full(E, -np.inf, np.float32), score, groups, top, "max", False, 1.0)
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("groups", [1, 4])
 def test_nans_rank_last(capi, score, groups):

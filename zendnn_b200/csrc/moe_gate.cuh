@@ -39,50 +39,59 @@ __device__ __forceinline__ float gate_logit(const GateArgs &a, int64_t at) {
   return a.logits_bf16 ? bf16_bits_to_f32(__ldg(reinterpret_cast<const uint16_t *>(a.logits) + at)) : __ldg(reinterpret_cast<const float *>(a.logits) + at);
 }
 
-// A warp's token in 64 bits, expert 32 j + lane in element j.  Lane i < k returns the i-th choice and its score.
+// A warp's token in 64 bits, expert 32 j + lane in element j.  Lane i < k returns the i-th choice and its score.  Loops, and the elements in local memory: few tokens come here, each finds the
+// code cold, and a CTA waits for it (unrolled, 16384 tokens over 256 experts took 48 us, 10 of them for the nine tokens that did).
 template <int PER>
 __device__ __noinline__ void gate_token(const GateArgs &a, int t, int lane, int &id, double &score) {
-  float x[PER];
-#pragma unroll
-  for (int j = 0; j < PER; ++j) x[j] = j * 32 + lane < a.E ? gate_logit(a, t * a.ld + j * 32 + lane) : 0.f;
   double s[PER];
-  if (a.sigmoid) {
-#pragma unroll
-    for (int j = 0; j < PER; ++j) s[j] = 1.0 / (1.0 + exp(-(double)x[j]));
-  } else {
-    float mx = __int_as_float(0xff800000);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) if (j * 32 + lane < a.E) mx = fmaxf(mx, x[j]);
+  unsigned long long key[PER];
+  const int elements = (a.E - lane + 31) / 32;         // of this lane
+  float mx = __int_as_float(0xff800000);
+  double sum = 1.0;
+  if (!a.sigmoid) {
+    for (int e = lane; e < a.E; e += 32) mx = fmaxf(mx, gate_logit(a, t * a.ld + e));
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    double sum = 0.0;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) { s[j] = j * 32 + lane < a.E ? exp((double)x[j] - (double)mx) : 0.0; sum += s[j]; }
+    sum = 0.0;
+  }
+#pragma unroll 1
+  for (int j = 0; j < elements; ++j) {
+    const double x = (double)gate_logit(a, t * a.ld + j * 32 + lane);
+    const double p = exp(a.sigmoid ? -x : x - (double)mx);
+    s[j] = p;
+    if (!a.sigmoid) sum += p;
+  }
+  if (!a.sigmoid) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) s[j] /= sum;
   }
-  unsigned long long key[PER];
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int e = j * 32 + lane;
-    key[j] = e < a.E ? gate_key(a.bias ? s[j] + (double)a.bias[e] : s[j]) : 0ull;
+#pragma unroll 1
+  for (int j = 0; j < elements; ++j) {
+    s[j] = (a.sigmoid ? 1.0 : s[j]) / (a.sigmoid ? 1.0 + s[j] : sum);
+    key[j] = gate_key(a.bias ? s[j] + (double)a.bias[j * 32 + lane] : s[j]);
   }
+  // the largest key of experts [from, to) but `without`, and its id
+  auto best = [&](int from, int to, int without, unsigned long long &top, int &id_of) {
+    top = 0ull; id_of = 0x7fffffff;
+#pragma unroll 1
+    for (int j = 0; j < elements; ++j) {
+      const int e = j * 32 + lane;
+      if (e >= from && e < to && e != without && key[j] > top) { top = key[j]; id_of = e; }
+    }
+    gate_best(top, id_of);
+  };
+  unsigned long long top;
+  int id_of;
   if (a.groups > 1) {
     // lane g: the score of group g
     unsigned long long mine = 0ull;
+#pragma unroll 1
     for (int g = 0; g < a.groups; ++g) {
       double total = 0.0;
       int first = -1;
+#pragma unroll 1
       for (int r = 0; r <= a.top2; ++r) {
-        unsigned long long top = 0ull; int id_of = 0x7fffffff;
-#pragma unroll
-        for (int j = 0; j < PER; ++j) {
-          const int e = j * 32 + lane;
-          if ((unsigned)(e - g * a.per_group) < (unsigned)a.per_group && e != first && key[j] > top) { top = key[j]; id_of = e; }
-        }
-        gate_best(top, id_of);
+        best(g * a.per_group, (g + 1) * a.per_group, first, top, id_of);
         if (top == 0ull) break;              // a group of one expert
         first = id_of;
         const double c = top == 1ull ? __longlong_as_double(0x7ff8000000000000ll) : __longlong_as_double((long long)(top >> 63 ? top & 0x7fffffffffffffffull : ~top));
@@ -91,39 +100,36 @@ __device__ __noinline__ void gate_token(const GateArgs &a, int t, int lane, int 
       if (lane == g) mine = gate_key(total);
     }
     int rank = 0;
+#pragma unroll 1
     for (int g = 0; g < a.groups; ++g) {
       const unsigned long long other = __shfl_sync(0xffffffffu, mine, g);
       rank += other > mine || (other == mine && g < lane);
     }
     const unsigned chosen = __ballot_sync(0xffffffffu, lane < a.groups && rank < a.top_groups);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) { const int e = j * 32 + lane; if (e < a.E && !((chosen >> (e / a.per_group)) & 1u)) key[j] = 0ull; }
+#pragma unroll 1
+    for (int j = 0; j < elements; ++j) if (!((chosen >> ((j * 32 + lane) / a.per_group)) & 1u)) key[j] = 0ull;
   }
   id = 0; score = 0.0;
+#pragma unroll 1
   for (int r = 0; r < a.k; ++r) {
-    unsigned long long top = 0ull; int id_of = 0x7fffffff;
+    best(0, a.E, -1, top, id_of);
     double v = 0.0;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) if (key[j] > top) { top = key[j]; id_of = j * 32 + lane; v = s[j]; }
-    gate_best(top, id_of);
+    if ((id_of & 31) == lane) { v = s[id_of >> 5]; key[id_of >> 5] = 0ull; }
     v = __shfl_sync(0xffffffffu, v, id_of & 31);
-#pragma unroll
-    for (int j = 0; j < PER; ++j) if (id_of == j * 32 + lane) key[j] = 0ull;
     if (lane == r) { id = id_of; score = v; }
   }
 }
 
 // The same in 32 bits, where these are enough.  f32 scores carry errors of a few steps, and the choice is taken for the one that 64 bits would make when every comparison that decides it is clear
 // by more than these: between neighbours among the chosen, between the last of them and the best that is left, between the last chosen group and the next.
-// (Experts with one logit and one bias have one score in either width, and go by their index.)  False: the token is one for gate_token; about one in 300 over 256 experts
-// with continuous logits.  Returns the weights' scores in f32, and the sum of the chosen is left to the caller.
-__device__ __forceinline__ uint32_t gate_key(float c) {
-  if (c != c) return 1u;
-  const uint32_t b = __float_as_uint(c);
-  return b >> 31 ? ~b : b | 0x80000000u;
+// (Experts with one logit and one bias have one score in either width, and go by their index.)  Choices that are not clear, one token in two thousand over 256 experts with continuous
+// logits, are put in order by the 64-bit scores of these alone.  False: the token is one for gate_token.  Returns the weights' scores in f32; the sum of the chosen is left to the caller.
+__device__ __forceinline__ uint32_t gate_key(float c) {      // (no NaN)
+  const int b = __float_as_int(c);
+  return (uint32_t)(b ^ (b >> 31 | (int)0x80000000));
 }
 __device__ __forceinline__ float gate_value(uint32_t key) {
-  return key <= 1u ? __int_as_float(0x7fc00000) : __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
+  return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
 }
 template <int N> __device__ __forceinline__ float gate_sum(const float (&v)[N]) {
   if constexpr (N == 1) return v[0];
@@ -151,9 +157,10 @@ template <int PER> __device__ __forceinline__ void gate_sort(uint32_t (&v)[PER])
           }
 }
 
-// group_of: groups of the lane's experts, a byte each
+// x, bias: minus infinity behind the last expert.  group_of: groups of the lane's experts, a byte each.
 template <int PER>
-__device__ __forceinline__ bool gate_token_f32(const GateArgs &a, const float (&x)[PER], const float (&bias)[PER], const uint32_t (&group_of)[(PER + 3) / 4], int lane, int &id, float &score) {
+__device__ __forceinline__ bool gate_token_f32(const GateArgs &a, int t, const float (&x)[PER], const float (&bias)[PER], const uint32_t (&group_of)[(PER + 3) / 4], int lane, int &id,
+                                               float &score) {
   const unsigned all = 0xffffffffu;
   float mx = 0.f, sum = 1.f, most = 1.f;       // of the softmax: largest logit, denominator; bound of the scores
   uint32_t key[PER];
@@ -161,15 +168,15 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, const float (&
     float s[PER];
     if (a.sigmoid) {
 #pragma unroll
-      for (int j = 0; j < PER; ++j) s[j] = __fdividef(1.0f, 1.0f + expf(-x[j]));
+      for (int j = 0; j < PER; ++j) s[j] = __fdividef(1.0f, 1.0f + __expf(-x[j]));
     } else {
       mx = __int_as_float(0xff800000);
 #pragma unroll
-      for (int j = 0; j < PER; ++j) if (j * 32 + lane < a.E) mx = fmaxf(mx, x[j]);
+      for (int j = 0; j < PER; ++j) mx = fmaxf(mx, x[j]);
 #pragma unroll
       for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(all, mx, o));
 #pragma unroll
-      for (int j = 0; j < PER; ++j) s[j] = j * 32 + lane < a.E ? expf(x[j] - mx) : 0.f;
+      for (int j = 0; j < PER; ++j) s[j] = __expf(x[j] - mx);
       sum = gate_sum<PER>(s);
 #pragma unroll
       for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(all, sum, o);
@@ -177,13 +184,24 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, const float (&
 #pragma unroll
       for (int j = 0; j < PER; ++j) s[j] *= most;
       // (a NaN, an infinity, or minus infinity throughout: there is no softmax)
-      if (!(sum >= 1.0f && sum < 3e38f)) return false;
+      if (!(sum >= 0.99f && sum < 3e38f)) return false;
     }
+    bool nan = false;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) key[j] = j * 32 + lane < a.E ? gate_key(s[j] + bias[j]) : 0u;
+    for (int j = 0; j < PER; ++j) {
+      const float c = s[j] + bias[j];
+      nan |= c != c;
+      key[j] = gate_key(c);
+    }
+    if (__any_sync(all, nan)) return false;
+    if (a.E != PER * 32) {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) if (j * 32 + lane >= a.E) key[j] = 0u;
+    }
   }
-  // errors: a sigmoid is off by 6e-7 of itself; a softmax by 5e-6 and by 6e-8 for every unit between logit and maximum (the difference's rounding); a sum by its rounding
-  const float off = a.sigmoid ? 7e-7f : 5e-6f;
+  // Errors, relative: the exponential (ex2.approx, 2^-22) with the rounding of its argument, 6e-8 for every unit of it, twice for a softmax (its difference is rounded too); a sum and a quotient: 7e-7 together;
+  // a softmax's denominator up to 4e-6.  A group's two scores, each at most `most`: 1.2e-7 |d| exp(-|d|) of it, which 1e-7 covers.
+  const float off = a.sigmoid ? 8e-7f : 5e-6f;
   bool clear = true;
   if (a.groups > 1) {
     uint32_t first = 0u, second = 0u;          // lane g: the two largest keys of group g
@@ -232,7 +250,7 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, const float (&
     if (a.top_groups < a.groups) {
       const int last = __ffs(__ballot_sync(all, lane < a.groups && rank == a.top_groups - 1)) - 1, next = __ffs(__ballot_sync(all, lane < a.groups && rank == a.top_groups)) - 1;
       const float u = gate_value(__shfl_sync(all, mine, last)), v = gate_value(__shfl_sync(all, mine, next));
-      clear = u - v > 2.f * (off + (a.sigmoid ? 0.f : 6e-6f)) * most + 3e-7f * (fabsf(u) + fabsf(v)) + 1e-36f;
+      clear = u - v > 4.f * (off + 1e-7f) * most + 3e-7f * (fabsf(u) + fabsf(v)) + 1e-36f;
 #pragma unroll
       for (int j = 0; j < PER; ++j) if (!((chosen >> ((group_of[j / 4] >> (j % 4 * 8)) & 31u)) & 1u)) key[j] = 0u;
     }
@@ -254,19 +272,11 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, const float (&
     }
     if (lane == r) { my_key = top; my_lane = from; }
   }
-  float my_x = 0.f, my_b = 0.f;
   const uint32_t key_behind = __shfl_down_sync(all, my_key, 1);
-  if (!__any_sync(all, lane + 1 < rounds && my_key == key_behind)) {
-    // which of its lane's experts a choice is, with its logit and bias
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const uint32_t k = __shfl_sync(all, key[j], my_lane);
-      const float vx = __shfl_sync(all, x[j], my_lane), vb = __shfl_sync(all, bias[j], my_lane);
-      if (k == my_key) { my_id = j * 32 + my_lane; my_x = vx; my_b = vb; }
-    }
-  } else {
-    // equal keys: the lowest index of the largest key, again and again
-    for (int r = 0; r < rounds; ++r) {
+  // the lowest index of the largest key, again and again, from the r0-th choice on (keys of a lane that are chosen become 0)
+  auto choose = [&](int r0, int r1) {
+#pragma unroll 1
+    for (int r = r0; r < r1; ++r) {
       uint32_t best = key[0]; int at = 0;
 #pragma unroll
       for (int j = 1; j < PER; ++j) if (key[j] > best) { best = key[j]; at = j; }
@@ -274,29 +284,61 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, const float (&
       const int e = __reduce_min_sync(all, best == top ? (unsigned)(at * 32 + lane) : 0x7fffffffu);
 #pragma unroll
       for (int j = 0; j < PER; ++j) if (e == j * 32 + lane) key[j] = 0u;
-      if (lane == r) my_id = e;
+      if (lane == r) { my_id = e; my_key = top; }
     }
+  };
+  const bool equal = __any_sync(all, lane + 1 < rounds && my_key == key_behind);
+  if (!equal) {
+    // which of its lane's experts a choice is
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const float vx = __shfl_sync(all, x[j], my_id & 31), vb = __shfl_sync(all, bias[j], my_id & 31);
-      if (my_id >> 5 == j) { my_x = vx; my_b = vb; }
+    for (int j = 0; j < PER; ++j) if (__shfl_sync(all, key[j], my_lane) == my_key) my_id = j * 32 + my_lane;
+  } else choose(0, rounds);
+  float my_x = 0.f, my_b = 0.f;
+  auto look = [&](int r1) {
+    if (lane < r1) {
+      my_x = gate_logit(a, t * a.ld + my_id);
+      my_b = a.bias ? a.bias[my_id] : 0.f;
     }
-  }
-  if (a.sigmoid) score = __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-my_x)));
-  else {
-    // the difference, and what its rounding left out
-    const float d = __fsub_rn(my_x, mx), back = __fsub_rn(d, my_x), rest = __fsub_rn(__fsub_rn(my_x, __fsub_rn(d, back)), __fadd_rn(mx, back));
-    score = __fdiv_rn(expf(d) * (1.0f + rest), sum);
-  }
-  {
+    if (a.sigmoid) score = __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-my_x)));
+    else {
+      // the difference, and what its rounding left out
+      const float d = __fsub_rn(my_x, mx), back = __fsub_rn(d, my_x), rest = __fsub_rn(__fsub_rn(my_x, __fsub_rn(d, back)), __fadd_rn(mx, back));
+      score = __fdiv_rn(expf(d) * (1.0f + rest), sum);
+    }
+  };
+  // is this lane's choice before the next lane's in 64 bits too?
+  bool same = false;                           // one logit and one bias
+  auto before_next = [&]() {
     const float c = gate_value(my_key), c2 = __shfl_down_sync(all, c, 1), x2 = __shfl_down_sync(all, my_x, 1), b2 = __shfl_down_sync(all, my_b, 1), s2 = __shfl_down_sync(all, score, 1);
-    const bool same = my_x == x2 && my_b == b2;
-    const float err = a.sigmoid ? off : off + 6e-8f * fmaxf(mx - my_x, mx - x2);
-    const bool apart = c - c2 > 2.f * err * fmaxf(score, s2) + 3e-7f * (fabsf(c) + fabsf(c2)) + 1e-36f;
-    if (lane + 1 < rounds && !same && !apart) clear = false;
-  }
+    const float err = off + (a.sigmoid ? 6e-8f * fmaxf(fabsf(my_x), fabsf(x2)) : 1.2e-7f * fmaxf(mx - my_x, mx - x2));
+    same = my_x == x2 && my_b == b2;
+    return c - c2 > 2.f * err * fmaxf(score, s2) + 3e-7f * (fabsf(c) + fabsf(c2)) + 1e-36f;
+  };
+  look(rounds);
+  const bool apart = before_next();
   id = my_id;
-  return __all_sync(all, clear);
+  if (__all_sync(all, clear && (lane + 1 >= rounds || apart || same))) return true;
+  // Some neighbours are too close.  Choices up to one that is clearly behind its predecessor, at the k-th or later, hold the right ones: these are put in order by 64-bit scores.
+  if (!__all_sync(all, clear) || (!a.sigmoid && a.bias)) return false;
+  const int candidates = a.top_groups * a.per_group, more = min(min(32, candidates), a.k + 8);
+  choose(equal ? rounds : 0, more);
+  look(more);
+  const unsigned ends = __ballot_sync(all, before_next() && lane + 1 >= a.k && lane + 1 < more) | (more == candidates ? 1u << (more - 1) : 0u);
+  if (ends == 0u) return false;
+  const int p = __ffs(ends);                   // so many of them
+  const double e64 = exp(a.sigmoid ? -(double)my_x : (double)my_x - (double)mx), c64 = a.sigmoid ? 1.0 / (1.0 + e64) + (double)my_b : e64;
+  int rank = 0, from = 0;
+#pragma unroll 1
+  for (int q = 0; q < p; ++q) {
+    const double c2 = __shfl_sync(all, c64, q);
+    const int id2 = __shfl_sync(all, my_id, q);
+    rank += c2 > c64 || (c2 == c64 && id2 < my_id);
+  }
+#pragma unroll 1
+  for (int q = 0; q < p; ++q) if (__shfl_sync(all, rank, q) == lane) from = q;
+  id = __shfl_sync(all, my_id, from);
+  score = __shfl_sync(all, score, from);
+  return true;
 }
 
 // Slots' places: rank of each of a chunk's slots inside its expert, behind next[e] rows.  All threads of a CTA of 1024; cnt: [32 warps][E] bytes.
@@ -353,7 +395,7 @@ __global__ void __launch_bounds__(kGateTokenThreads<PER>) gate_kernel(const Gate
   }
   float bias[PER];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) bias[j] = a.bias && j * 32 + lane < a.E ? a.bias[j * 32 + lane] : 0.f;
+  for (int j = 0; j < PER; ++j) bias[j] = j * 32 + lane >= a.E ? __int_as_float(0xff800000) : a.bias ? a.bias[j * 32 + lane] : 0.f;
   uint32_t group_of[(PER + 3) / 4] = {};
 #pragma unroll
   for (int j = 0; j < PER; ++j) group_of[j / 4] |= (uint32_t)(min(j * 32 + lane, a.E - 1) / a.per_group) << (j % 4 * 8);
@@ -362,14 +404,14 @@ __global__ void __launch_bounds__(kGateTokenThreads<PER>) gate_kernel(const Gate
     if (a.logits_bf16) {
       const uint16_t *p = reinterpret_cast<const uint16_t *>(a.logits) + t * a.ld + lane;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) x[j] = j * 32 + lane < a.E ? bf16_bits_to_f32(__ldg(p + j * 32)) : 0.f;
+      for (int j = 0; j < PER; ++j) x[j] = j * 32 + lane < a.E ? bf16_bits_to_f32(__ldg(p + j * 32)) : __int_as_float(0xff800000);
     } else {
       const float *p = reinterpret_cast<const float *>(a.logits) + t * a.ld + lane;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) x[j] = j * 32 + lane < a.E ? __ldg(p + j * 32) : 0.f;
+      for (int j = 0; j < PER; ++j) x[j] = j * 32 + lane < a.E ? __ldg(p + j * 32) : __int_as_float(0xff800000);
     }
     int id; float w;
-    if (gate_token_f32<PER>(a, x, bias, group_of, lane, id, w)) {
+    if (gate_token_f32<PER>(a, t, x, bias, group_of, lane, id, w)) {
       if (a.renorm) {
         float sum = lane < a.k ? w : 0.f;
 #pragma unroll
