@@ -362,6 +362,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     auto place = [&](int key) { return slot_at + (value ? Ring::at_value(key, chunk) : Ring::at_key(key, chunk)); };
     auto from = [&](int e) { return paged_lds_ptr(plan + (uint32_t)(entry + e) * 16u + (value ? 8u : 0u)); };
     const uint64_t mine = (P8 ? (uint64_t)sub * token : 0) + chunk * 16;
+    if (limit == 0) return;
     if (!cut_in) {
       constexpr int REP_K = RI >= 2 ? 1 : 2, REP_V = RI >= 8 ? 1 : 8 / RI;      // copies after which the swizzle repeats
       const int rep = value ? REP_V : REP_K;
