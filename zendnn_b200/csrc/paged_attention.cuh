@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
   constexpr int ST = Ring::ST, CH = Ring::CH, RI = Ring::RI, IN = Ring::IN, KP = Ring::kPieceK, VP = Ring::kPieceV, VB = Ring::kWideV, REGS = PagedJoin<S8, DP, NT>::kRegs;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float s_m[kPagedWarps][8 * NT], s_l[kPagedWarps][8 * NT];
-  __shared__ int s_scan[kPagedWarps], s_start[4];
+  __shared__ int s_scan[kPagedWarps], s_before[32 * kPagedWarps];
   __shared__ int s_last;
   __shared__ uint4 s_plan[kPagedWarps][32];
   __shared__ uint64_t s_splan[S8 ? kPagedWarps : 1][32];
@@ -275,28 +275,26 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += v; }
     if (lane == 31) s_scan[warp] = sum;
+    s_before[tid] = sum - mine;                // (of this warp's stretches)
     __syncthreads();
-    int before = sum - mine, total = 0;
+    int total = 0;
 #pragma unroll
-    for (int w = 0; w < kPagedWarps; ++w) { if (w < warp) before += s_scan[w]; total += s_scan[w]; }
+    for (int w = 0; w < kPagedWarps; ++w) total += s_scan[w];
     per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, s.min_units);
     first = min(total, (int)blockIdx.x * per);
     const int count = min(per, total - first);
     if (count <= 0) return;
-    if (before <= first && first < before + mine) {
-      for (ahead.seq = b0; ahead.seq < b1; ++ahead.seq) {
-        ahead.sequence(a);
-        const int units = ahead.n * s.rows;
-        if (first < before + units) break;
-        before += units;
-      }
-      s_start[0] = ahead.seq;
-      s_start[1] = (first - before) / ahead.n;
-      s_start[2] = (first - before) % ahead.n;
-    }
-    __syncthreads();
-    ahead.seq = s_start[0]; ahead.row = s_start[1]; ahead.off = s_start[2]; ahead.left = count;
-    ahead.sequence(a);
+    // the stretch: the last one that begins at or before the first unit
+    int w = 0, before = 0;
+#pragma unroll
+    for (int i = 1, begin = 0; i < kPagedWarps; ++i) { begin += s_scan[i - 1]; if (begin <= first) { w = i; before = begin; } }
+    const int at = __popc(__ballot_sync(0xffffffffu, before + s_before[w * 32 + lane] <= first)) - 1;
+    before += s_before[w * 32 + at];
+    ahead.seq = (w * 32 + at) * stretch;
+    for (ahead.sequence(a); before + ahead.n * s.rows <= first && ahead.seq + 1 < a.B; ahead.sequence(a)) { before += ahead.n * s.rows; ++ahead.seq; }
+    ahead.row = (first - before) / ahead.n;
+    ahead.off = (first - before) - ahead.row * ahead.n;
+    ahead.left = count;
   }
   PagedPieces<P8, kPagedUnit> now = ahead;
 
