@@ -19,7 +19,7 @@ int32_t launch(void (*kern)(P...), unsigned grid, unsigned threads, size_t smem,
 constexpr int kGateOneCta = 128;
 int32_t launch_gate(const GateArgs &a, const GateRowsArgs &r, unsigned grid, cudaStream_t st) {
   const unsigned threads = (unsigned)std::min(a.E <= 256 ? kGateTokenThreads<8> : kGateTokenThreads<32>, 32 * a.chunk);
-  const size_t smem = (size_t)a.E * 8 + (size_t)(threads / 32) * a.E;
+  const size_t smem = (size_t)gate_pad(a.E) * 8 + (size_t)a.E * 32;
   if (a.E <= 32) return launch(gate_kernel<1>, grid, threads, smem, st, a, r);
   if (a.E <= 64) return launch(gate_kernel<2>, grid, threads, smem, st, a, r);
   if (a.E <= 128) return launch(gate_kernel<4>, grid, threads, smem, st, a, r);
@@ -77,11 +77,11 @@ extern "C" int32_t b200dnn_moe_gate(const b200dnn_moe_gate_t *d, void *stream) {
   GateRowsArgs r{a.ids, nullptr, T, E, k, a.chunk, (int32_t *)counts.dev, (int32_t *)rows.dev};
   const bool second = grid > 1 && (d->expert_counts || d->slot_to_row);
   if (second) {
-    a.counts = (int32_t *)rt().ws.alloc((size_t)grid * E * 4);
+    a.counts = (int32_t *)rt().ws.alloc((size_t)grid * gate_pad(E) * 4);
     B2_CHECK(a.counts, B200DNN_FAILURE, "workspace allocation failed");
     r.counts = a.counts;
   }
   B2_TRY(launch_gate(a, grid > 1 ? GateRowsArgs{} : r, grid, st));
-  if (second) B2_TRY(launch(gate_rows_kernel, grid, kGateThreads, (size_t)E * (8 + 32), st, r));
+  if (second) B2_TRY(launch(gate_rows_kernel, grid, kGateThreads, (size_t)gate_pad(E) * 8 + (size_t)E * 32, st, r));
   return finish_out({&ids, &weights, &counts, &rows}, st);
 }
