@@ -15,11 +15,14 @@ int32_t launch(void (*kern)(P...), unsigned grid, unsigned threads, size_t smem,
   return B200DNN_SUCCESS;
 }
 
-// Tokens of a CTA: one CTA up to 128 of them, else 32 and as many more as leave a CTA for every SM (every CTA of the second launch adds up the counts of all).
-constexpr int kGateOneCta = 128;
+// Tokens of a CTA: all of a small batch, whose places then need no second launch (us, one CTA and two launches: 32 tokens over 64 experts 5.7, 6.3; 24 over 256 in groups 7.7, 8.5; but 32 over
+// 256 9.1, 8.2; 64 over 64 8.2, 6.5); else 8 and as many more as leave a CTA for every SM (every CTA of the second launch adds up the counts of all), up to 2048 (they may all be on its list
+// of tokens for 64 bits).
+constexpr int kGateMostTokens = 2048;
+bool gate_one_cta(int T, int E) { return T <= 32 && T * E < 8192; }
 int32_t launch_gate(const GateArgs &a, const GateRowsArgs &r, unsigned grid, cudaStream_t st) {
   const unsigned threads = (unsigned)std::min(a.E <= 256 ? kGateTokenThreads<8> : kGateTokenThreads<32>, 32 * a.chunk);
-  const size_t smem = (size_t)gate_pad(a.E) * 8 + (size_t)a.E * 32;
+  const size_t smem = (size_t)gate_pad(a.E) * 8 + (size_t)a.E * 32 + (size_t)a.chunk * 4;
   if (a.E <= 32) return launch(gate_kernel<1>, grid, threads, smem, st, a, r);
   if (a.E <= 64) return launch(gate_kernel<2>, grid, threads, smem, st, a, r);
   if (a.E <= 128) return launch(gate_kernel<4>, grid, threads, smem, st, a, r);
@@ -72,7 +75,7 @@ extern "C" int32_t b200dnn_moe_gate(const b200dnn_moe_gate_t *d, void *stream) {
   a.T = T; a.E = E; a.k = k; a.sigmoid = d->score == B200DNN_GATE_SIGMOID; a.groups = G; a.top_groups = d->topk_groups; a.per_group = E / G;
   a.top2 = d->group_score == B200DNN_GROUP_TOP2; a.renorm = d->renorm ? 1 : 0; a.scale = d->scale;
   a.ids = (int32_t *)ids.dev; a.weights = (float *)weights.dev;
-  a.chunk = T <= kGateOneCta ? T : std::max(32, (T + rt().sm_count - 1) / rt().sm_count);
+  a.chunk = gate_one_cta(T, E) ? T : std::min(kGateMostTokens, std::max(8, (T + rt().sm_count - 1) / rt().sm_count));
   const unsigned grid = (unsigned)((T + a.chunk - 1) / a.chunk);
   GateRowsArgs r{a.ids, nullptr, T, E, k, a.chunk, (int32_t *)counts.dev, (int32_t *)rows.dev};
   const bool second = grid > 1 && (d->expert_counts || d->slot_to_row);

@@ -39,44 +39,32 @@ __device__ __forceinline__ float gate_logit(const GateArgs &a, int64_t at) {
   return a.logits_bf16 ? bf16_bits_to_f32(__ldg(reinterpret_cast<const uint16_t *>(a.logits) + at)) : __ldg(reinterpret_cast<const float *>(a.logits) + at);
 }
 
-// A warp's token in 64 bits, expert 32 j + lane in element j.  Lane i < k returns the i-th choice and its score.  Loops, and the elements in local memory: few tokens come here, each finds the
-// code cold, and a CTA waits for it (unrolled, 16384 tokens over 256 experts took 48 us, 10 of them for the nine tokens that did).
-template <int PER>
-__device__ __noinline__ void gate_token(const GateArgs &a, int t, int lane, int &id, double &score) {
-  double s[PER];
-  unsigned long long key[PER];
-  const int elements = (a.E - lane + 31) / 32;         // of this lane
+// A token in 64 bits, in three parts.  Scores s and keys lie in memory, expert after expert.
+// The softmax's largest logit (a warp's reduction)
+__device__ __forceinline__ float gate_largest(const GateArgs &a, int64_t t, int lane) {
   float mx = __int_as_float(0xff800000);
-  double sum = 1.0;
-  if (!a.sigmoid) {
-    for (int e = lane; e < a.E; e += 32) mx = fmaxf(mx, gate_logit(a, t * a.ld + e));
+  for (int e = lane; e < a.E; e += 32) mx = fmaxf(mx, gate_logit(a, t * a.ld + e));
 #pragma unroll
-    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    sum = 0.0;
-  }
-#pragma unroll 1
-  for (int j = 0; j < elements; ++j) {
-    const double x = (double)gate_logit(a, t * a.ld + j * 32 + lane);
-    const double p = exp(a.sigmoid ? -x : x - (double)mx);
-    s[j] = p;
-    if (!a.sigmoid) sum += p;
-  }
-  if (!a.sigmoid) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  }
-#pragma unroll 1
-  for (int j = 0; j < elements; ++j) {
-    s[j] = (a.sigmoid ? 1.0 : s[j]) / (a.sigmoid ? 1.0 + s[j] : sum);
-    key[j] = gate_key(a.bias ? s[j] + (double)a.bias[j * 32 + lane] : s[j]);
-  }
+  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  return mx;
+}
+// An expert's exponential, and its score and key from it
+__device__ __forceinline__ double gate_exp(const GateArgs &a, int64_t t, int e, float mx) {
+  const double x = (double)gate_logit(a, t * a.ld + e);
+  return exp(a.sigmoid ? -x : x - (double)mx);
+}
+__device__ __forceinline__ unsigned long long gate_score(const GateArgs &a, int e, double sum, double &s) {
+  s = (a.sigmoid ? 1.0 : s) / (a.sigmoid ? 1.0 + s : sum);
+  return gate_key(a.bias ? s + (double)a.bias[e] : s);
+}
+// The choice, by one warp (the keys are used up).  Lane i < k returns the i-th and its score.
+__device__ __noinline__ void gate_choose(const GateArgs &a, const double *s, unsigned long long *key, int lane, int &id, double &score) {
   // the largest key of experts [from, to) but `without`, and its id
   auto best = [&](int from, int to, int without, unsigned long long &top, int &id_of) {
     top = 0ull; id_of = 0x7fffffff;
-#pragma unroll 1
-    for (int j = 0; j < elements; ++j) {
-      const int e = j * 32 + lane;
-      if (e >= from && e < to && e != without && key[j] > top) { top = key[j]; id_of = e; }
+    for (int e = from + lane; e < to; e += 32) {
+      const unsigned long long k = key[e];
+      if (e != without && k > top) { top = k; id_of = e; }
     }
     gate_best(top, id_of);
   };
@@ -106,24 +94,24 @@ __device__ __noinline__ void gate_token(const GateArgs &a, int t, int lane, int 
       rank += other > mine || (other == mine && g < lane);
     }
     const unsigned chosen = __ballot_sync(0xffffffffu, lane < a.groups && rank < a.top_groups);
-#pragma unroll 1
-    for (int j = 0; j < elements; ++j) if (!((chosen >> ((j * 32 + lane) / a.per_group)) & 1u)) key[j] = 0ull;
+    for (int g = 0; g < a.groups; ++g)
+      if (!((chosen >> g) & 1u)) for (int e = g * a.per_group + lane; e < (g + 1) * a.per_group; e += 32) key[e] = 0ull;
+    __syncwarp();
   }
   id = 0; score = 0.0;
 #pragma unroll 1
   for (int r = 0; r < a.k; ++r) {
     best(0, a.E, -1, top, id_of);
-    double v = 0.0;
-    if ((id_of & 31) == lane) { v = s[id_of >> 5]; key[id_of >> 5] = 0ull; }
-    v = __shfl_sync(0xffffffffu, v, id_of & 31);
-    if (lane == r) { id = id_of; score = v; }
+    if (lane == r) { id = id_of; score = s[id_of]; }
+    if (lane == 0) key[id_of] = 0ull;
+    __syncwarp();
   }
 }
 
 // The same in 32 bits, where these are enough.  f32 scores carry errors of a few steps, and the choice is taken for the one that 64 bits would make when every comparison that decides it is clear
 // by more than these: between neighbours among the chosen, between the last of them and the best that is left, between the last chosen group and the next.
 // (Experts with one logit and one bias have one score in either width, and go by their index.)  Choices that are not clear, one token in two thousand over 256 experts with continuous
-// logits, are put in order by the 64-bit scores of these alone.  False: the token is one for gate_token.  Returns the weights' scores in f32; the sum of the chosen is left to the caller.
+// logits, are put in order by the 64-bit scores of these alone.  False: the token needs all its scores in 64 bits.  Returns the weights' scores in f32; the sum of the chosen is left to the caller.
 __device__ __forceinline__ uint32_t gate_key(float c) {      // (no NaN)
   const int b = __float_as_int(c);
   return (uint32_t)(b ^ (b >> 31 | (int)0x80000000));
@@ -267,11 +255,48 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, int t, const f
       const uint32_t other = __shfl_sync(all, mine, g);
       rank += other > mine || (other == mine && g < lane);
     }
-    const unsigned chosen = __ballot_sync(all, lane < a.groups && rank < a.top_groups);
+    unsigned chosen = __ballot_sync(all, lane < a.groups && rank < a.top_groups);
     if (a.top_groups < a.groups) {
-      const int last = __ffs(__ballot_sync(all, lane < a.groups && rank == a.top_groups - 1)) - 1, next = __ffs(__ballot_sync(all, lane < a.groups && rank == a.top_groups)) - 1;
-      const float u = gate_value(__shfl_sync(all, mine, last)), v = gate_value(__shfl_sync(all, mine, next));
-      clear = u - v > 4.f * (off + 1e-7f) * most + 3e-7f * (fabsf(u) + fabsf(v)) + 1e-36f;
+      auto group_at = [&](int r) { return __ffs(__ballot_sync(all, lane < a.groups && rank == r)) - 1; };
+      auto value_of = [&](int g) { return gate_value(__shfl_sync(all, mine, g)); };
+      auto behind = [&](float u, float v) { return u - v > 4.f * (off + 1e-7f) * most + 3e-7f * (fabsf(u) + fabsf(v)) + 1e-36f; };
+      const int last = group_at(a.top_groups - 1), next = group_at(a.top_groups);
+      const float u = value_of(last), v = value_of(next);
+      clear = behind(u, v);
+      if (!clear && (a.sigmoid || !a.bias)) {
+        // The last group that is in and the first that is out are too close (in 16384 tokens of 256 experts two or three times): their scores in 64 bits, from their members', where these two are
+        // clear of the others and the members that count are clear of those that do not.
+        clear = (a.top_groups < 2 || behind(value_of(group_at(a.top_groups - 2)), u)) && (a.top_groups + 1 >= a.groups || behind(v, value_of(group_at(a.top_groups + 1))));
+        double total[2];
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          const int g = i ? next : last;
+          int members[2] = {-1, -1};
+          uint32_t top = 0u, before = 0u;
+#pragma unroll 1
+          for (int r = 0; r <= a.top2 + 1; ++r) {
+            uint32_t best = 0u; int at = 0;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+              const int e = j * 32 + lane;
+              if ((unsigned)(e - g * (int)per) < per && e != members[0] && e != members[1] && key[j] > best) { best = key[j]; at = e; }
+            }
+            before = top;
+            top = __reduce_max_sync(all, best);
+            const int e = (int)__reduce_min_sync(all, best == top ? (unsigned)at : 0x7fffffffu);
+            if (r <= a.top2 && top != 0u) members[r] = e;
+            // the first that does not count: clearly behind, or there is none
+            if (r == a.top2 + 1 && top != 0u && !behind(gate_value(before), gate_value(top))) clear = false;
+          }
+          double c = 0.0;
+          if (lane < 2 && members[lane] >= 0) {
+            const double x64 = (double)gate_logit(a, t * a.ld + members[lane]), e64 = exp(a.sigmoid ? -x64 : x64 - (double)mx);
+            c = a.sigmoid ? 1.0 / (1.0 + e64) + (a.bias ? (double)a.bias[members[lane]] : 0.0) : e64;
+          }
+          total[i] = __shfl_sync(all, c, 0) + __shfl_sync(all, c, 1);
+        }
+        if (clear && (total[1] > total[0] || (total[1] == total[0] && next < last))) chosen ^= 1u << last | 1u << next;
+      }
 #pragma unroll
       for (int j = 0; j < PER; ++j) if (!((chosen >> ((group_of[j / 4] >> (j % 4 * 8)) & 31u)) & 1u)) key[j] = 0u;
     }
@@ -420,15 +445,15 @@ template <int PER> constexpr int kGateTokenThreads = PER <= 8 ? 1024 : 512;     
 template <int PER>
 __global__ void __launch_bounds__(kGateTokenThreads<PER>) gate_kernel(const GateArgs a, const GateRowsArgs rows) {
   extern __shared__ int sm[];
-  int *hist = sm, *next = sm + gate_pad(a.E);
+  __shared__ int n_slow;
+  int *hist = sm, *next = sm + gate_pad(a.E), *slow = sm + 2 * gate_pad(a.E) + 8 * a.E;      // (between them 32 bytes an expert)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t0 = blockIdx.x * a.chunk, t1 = min(a.T, t0 + a.chunk);
   const bool count = a.counts || rows.expert_counts || rows.slot_to_row;
-  if (count) {
-    for (int i = threadIdx.x; i < a.E; i += blockDim.x) hist[i] = next[i] = 0;
-    __syncthreads();
-  }
+  for (int i = threadIdx.x; i < a.E; i += blockDim.x) hist[i] = next[i] = 0;
+  if (threadIdx.x == 0) n_slow = 0;
+  __syncthreads();
   float bias[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) bias[j] = j * 32 + lane >= a.E ? __int_as_float(0xff800000) : a.bias ? a.bias[j * 32 + lane] : 0.f;
@@ -447,28 +472,59 @@ __global__ void __launch_bounds__(kGateTokenThreads<PER>) gate_kernel(const Gate
       for (int j = 0; j < PER; ++j) x[j] = j * 32 + lane < a.E ? __ldg(p + j * 32) : __int_as_float(0xff800000);
     }
     int id; float w;
-    if (gate_token_f32<PER>(a, t, x, bias, group_of, lane, id, w)) {
-      if (a.renorm) {
-        float sum = lane < a.k ? w : 0.f;
+    if (!gate_token_f32<PER>(a, t, x, bias, group_of, lane, id, w)) {
+      if (lane == 0) slow[atomicAdd(&n_slow, 1)] = t;
+      continue;
+    }
+    if (a.renorm) {
+      float sum = lane < a.k ? w : 0.f;
 #pragma unroll
-        for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        w = __fdiv_rn(w, sum);
-      }
-      w *= a.scale;
-    } else {
-      double score, sum = 0.0;
-      gate_token<PER>(a, t, lane, id, score);
-      for (int r = 0; r < a.k; ++r) sum += __shfl_sync(0xffffffffu, score, r);
-      w = (float)((a.renorm ? score / sum : score) * (double)a.scale);
+      for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      w = __fdiv_rn(w, sum);
     }
     if (lane < a.k) {
       a.ids[(int64_t)t * a.k + lane] = id;
-      if (a.weights) a.weights[(int64_t)t * a.k + lane] = w;
+      if (a.weights) a.weights[(int64_t)t * a.k + lane] = w * a.scale;
       if (count) atomicAdd(&hist[id], 1);
     }
   }
-  if (!count) return;
   __syncthreads();
+  // Tokens that 32 bits do not decide, by all threads: a thread per expert for the scores (an exponential and a quotient in 64 bits are thousands of clocks one after the other: a warp by itself took
+  // 15 us for a token of 256 experts, and everyone waited), a warp for the choice.
+  for (int i = 0; i < n_slow; ++i) {
+    const int t = slow[i];
+    double *s = reinterpret_cast<double *>(sm + 2 * gate_pad(a.E));
+    unsigned long long *key = reinterpret_cast<unsigned long long *>(s + a.E);
+    const float mx = a.sigmoid ? 0.f : gate_largest(a, t, lane);
+    for (int e = threadIdx.x; e < a.E; e += blockDim.x) s[e] = gate_exp(a, t, e, mx);
+    __syncthreads();
+    double sum = 1.0;
+    if (!a.sigmoid) {
+      sum = 0.0;
+      for (int e = lane; e < a.E; e += 32) sum += s[e];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      __syncthreads();
+    }
+    for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
+      double v = s[e];
+      key[e] = gate_score(a, e, sum, v);
+      s[e] = v;
+    }
+    __syncthreads();
+    if (warp == 0) {
+      int id; double score, all = 0.0;
+      gate_choose(a, s, key, lane, id, score);
+      for (int r = 0; r < a.k; ++r) all += __shfl_sync(0xffffffffu, score, r);
+      if (lane < a.k) {
+        a.ids[(int64_t)t * a.k + lane] = id;
+        if (a.weights) a.weights[(int64_t)t * a.k + lane] = (float)((a.renorm ? score / all : score) * (double)a.scale);
+        if (count) atomicAdd(&hist[id], 1);
+      }
+    }
+    __syncthreads();
+  }
+  if (!count) return;
   if (a.counts) {
     for (int i = threadIdx.x; i < gate_pad(a.E); i += blockDim.x) a.counts[(int64_t)blockIdx.x * gate_pad(a.E) + i] = i < a.E ? hist[i] : 0;
     return;
