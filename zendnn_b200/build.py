@@ -49,7 +49,7 @@ def build(force=False, verbose=False):
     if force or _newer(LIB_CUDA, deps):
         cmd = [nvcc_path(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
                "-ccbin", host_cxx(), "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared",
-               "-Xptxas", "-v" if verbose else "-O3",
+               "-Xptxas", "-v" if verbose else "-O3", "--threads", "0",      # (the source files side by side)
                "-I", os.path.join(ROOT, "include"), "-o", LIB_CUDA] + \
               [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(".cu")] + ["-lcudart"]
         subprocess.check_call(cmd)

@@ -87,8 +87,10 @@ int32_t launch_append(const AppendArgs &a, cudaStream_t st) {
 
 // The split form, where rows are 16-byte vectors: false when the call does not fit.
 template <bool S8, int DP, int NT>
-int32_t launch_split(PagedSplitArgs &s, cudaStream_t st) {
-  auto kern = s.a.page_size % 8 == 0 ? paged_split_kernel<S8, DP, NT, true> : paged_split_kernel<S8, DP, NT, false>;
+int32_t launch_split(PagedSplitArgs &s, bool f32, cudaStream_t st) {
+  const bool p8 = s.a.page_size % 8 == 0;
+  auto kern = f32 ? (p8 ? paged_split_kernel<S8, DP, NT, true, true> : paged_split_kernel<S8, DP, NT, false, true>)
+                  : (p8 ? paged_split_kernel<S8, DP, NT, true, false> : paged_split_kernel<S8, DP, NT, false, false>);
   constexpr size_t smem = paged_smem<S8, DP, NT>();
   const int resident = (int)std::min<size_t>(DP <= 128 ? 3 : 1, (size_t)(227 * 1024) / (smem + 2048));
   constexpr int unit = PagedRing<S8, DP>::KS * kPagedWarps;
@@ -102,14 +104,14 @@ int32_t launch_split(PagedSplitArgs &s, cudaStream_t st) {
   return launch(kern, grid, 32 * kPagedWarps, smem, st, s);
 }
 template <bool S8, int DP>
-int32_t launch_split_heads(PagedSplitArgs &s, cudaStream_t st) {
+int32_t launch_split_heads(PagedSplitArgs &s, bool f32, cudaStream_t st) {
   const bool two = s.a.group > 8;
   s.tiles = (s.a.group + (two ? 16 : 8) - 1) / (two ? 16 : 8);
   s.rows = s.a.kv_heads * s.tiles;
-  return two ? launch_split<S8, DP, 2>(s, st) : launch_split<S8, DP, 1>(s, st);
+  return two ? launch_split<S8, DP, 2>(s, f32, st) : launch_split<S8, DP, 1>(s, f32, st);
 }
 template <bool S8>
-int32_t paged_split(const PagedArgs &a, int out_f32, cudaStream_t st) {
+int32_t paged_split(const PagedArgs &a, bool out_f32, cudaStream_t st) {
   const int vec = S8 ? 16 : 8;          // elements of 16 bytes
   auto rows_vec = [&](const void *p, const int64_t (&s)[3]) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s[0] % vec == 0 && (a.page_size == 1 || s[1] % vec == 0) && (a.kv_heads == 1 || s[2] % vec == 0);
@@ -117,15 +119,13 @@ int32_t paged_split(const PagedArgs &a, int out_f32, cudaStream_t st) {
   if (a.dim % vec != 0 || !rows_vec(a.key, a.ck) || !rows_vec(a.value, a.cv)) return B200DNN_UNIMPLEMENTED;
   PagedSplitArgs s{};
   s.a = a;
-  s.out_f32 = out_f32;
   s.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.qs[0] % 8 == 0 && a.qs[1] % 8 == 0;
   const int ov = out_f32 ? 4 : 8;
   s.out_vec = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.os[0] % ov == 0 && a.os[1] % ov == 0;
   s.min_units = 1;
-  if (a.dim <= 64) return launch_split_heads<S8, 64>(s, st);
-  if (a.dim <= 128) return launch_split_heads<S8, 128>(s, st);
-  if (a.dim <= 192) return launch_split_heads<S8, 192>(s, st);
-  return launch_split_heads<S8, 256>(s, st);
+  if (a.dim <= 64) return launch_split_heads<S8, 64>(s, out_f32, st);
+  if (a.dim <= 128) return launch_split_heads<S8, 128>(s, out_f32, st);
+  return launch_split_heads<S8, 256>(s, out_f32, st);
 }
 
 }  // namespace

@@ -110,8 +110,8 @@ __global__ void __launch_bounds__(32 * kPagedRowWarps) paged_rows_kernel(const P
 // P^T comes from S^T by transposing 8 x 8 blocks (movmatrix).  Statistics of heads 2c and 2c + 1 and their columns of O^T are in the same lanes.
 // Tensor work is a fifth of what the memory leaves time for, so bf16 tiles of 16 x 8 serve: the call is bound by the bytes of the cache.
 //
-// Probabilities enter the second product as the sum of two bf16 (2^-17 relative): one alone would cost as much again as the rounding of a bf16 output, and an f32
-// output most of its digits.  The row sum has them unrounded.  s8 codes are exact in bf16; a key's scale multiplies its scores, a value's scale its probability.
+// Probabilities enter the second product as the sum of two bf16 (2^-17 relative): one alone would cost as much again as the rounding of a bf16 output.  For an f32 output it is three
+// (2^-25).  The row sum has them unrounded.  s8 codes are exact in bf16; a key's scale multiplies its scores, a value's scale its probability.
 // The running maximum moves only when a score passes it by more than 2^8: probabilities are then at most 256, and few steps meet the exchange.
 
 constexpr float kPagedLog2e = 1.44269504088896340736f;
@@ -122,7 +122,7 @@ struct PagedSplitArgs {
   PagedArgs a;
   int tiles;                       // head tiles of a key head
   int rows;                        // rows of a sequence: kv_heads * tiles
-  int out_f32, q_vec, out_vec;     // 16-byte rows of q and out
+  int q_vec, out_vec;              // 16-byte rows of q and out
   int min_units;                   // fewest units of a CTA
   float *part_o; float2 *part_ml;  // partial results: two slots a CTA
   uint32_t *counters;              // one a CTA, zero between launches
@@ -234,9 +234,9 @@ template <bool S8, int DP, int NT> struct PagedJoin {
 };
 template <bool S8, int DP, int NT> constexpr size_t paged_smem() { return PagedRing<S8, DP>::kBytes + PagedJoin<S8, DP, NT>::kBytes; }
 
-// P8: pages of a multiple of eight keys.  Units then begin at a multiple of eight, the eight keys of half a step lie on one page, and their places need no lane's
+// F32: of the output.  P8: pages of a multiple of eight keys.  Units then begin at a multiple of eight, the eight keys of half a step lie on one page, and their places need no lane's
 // table entry but two that the whole warp knows; otherwise every lane looks up the key lane % 16.
-template <bool S8, int DP, int NT, bool P8>
+template <bool S8, int DP, int NT, bool P8, bool F32>
 __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 : 2) paged_split_kernel(const PagedSplitArgs s) {
   using Ring = PagedRing<S8, DP>;
   constexpr int KS = Ring::KS, MT = KS / 16, kPagedUnit = KS * kPagedWarps;
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     for (int x = tid; x < a.q_heads * a.dim; x += 32 * kPagedWarps) {
       const int h = x / a.dim, d = x - h * a.dim;
       const int64_t at = i * a.os[0] + h * a.os[1] + d;
-      if (s.out_f32) reinterpret_cast<float *>(a.out)[at] = 0.f; else reinterpret_cast<uint16_t *>(a.out)[at] = 0;
+      if (F32) reinterpret_cast<float *>(a.out)[at] = 0.f; else reinterpret_cast<uint16_t *>(a.out)[at] = 0;
     }
     if (a.lse) for (int h = tid; h < a.q_heads; h += 32 * kPagedWarps) a.lse[(int64_t)i * a.q_heads + h] = ninf;
   }
@@ -527,7 +527,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
             for (int t = 0; t < DP / 16; ++t) { o[n][t][e] *= keep; o[n][t][e + 2] *= keep; }
           }
       }
-      uint32_t p[MT][NT][2], pl[MT][NT][2];
+      uint32_t p[MT][NT][2], pl[MT][NT][2], pr[F32 ? MT : 1][NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float f0 = m[n][0] == ninf ? 0.f : m[n][0], f1 = m[n][1] == ninf ? 0.f : m[n][1];
@@ -543,7 +543,10 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
           for (int e = 0; e < 2; ++e) {
             const uint32_t hi = paged_pack(y[2 * e], y[2 * e + 1]);
             p[i][n][e] = paged_transpose(hi);
-            pl[i][n][e] = paged_transpose(paged_pack(y[2 * e] - __uint_as_float(hi << 16), y[2 * e + 1] - __uint_as_float(hi & 0xffff0000u)));
+            const float r0 = y[2 * e] - __uint_as_float(hi << 16), r1 = y[2 * e + 1] - __uint_as_float(hi & 0xffff0000u);
+            const uint32_t lo = paged_pack(r0, r1);
+            pl[i][n][e] = paged_transpose(lo);
+            if constexpr (F32) pr[i][n][e] = paged_transpose(paged_pack(r0 - __uint_as_float(lo << 16), r1 - __uint_as_float(lo & 0xffff0000u)));
           }
         }
       }
@@ -560,6 +563,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
             for (int n = 0; n < NT; ++n) {
               paged_mma(o[n][d], a0, a1, a2, a3, p[j][n][0], p[j][n][1]);
               paged_mma(o[n][d], a0, a1, a2, a3, pl[j][n][0], pl[j][n][1]);
+              if constexpr (F32) paged_mma(o[n][d], a0, a1, a2, a3, pr[j][n][0], pr[j][n][1]);
             }
           };
           uint32_t v[4][W];
@@ -681,7 +685,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
             float y[2 * TILES];
 #pragma unroll
             for (int w = 0; w < TILES; ++w) { y[2 * w] = o[n][t + w][e] * by; y[2 * w + 1] = o[n][t + w][e + 2] * by; }
-            if (s.out_f32) {
+            if constexpr (F32) {
               float *out = reinterpret_cast<float *>(a.out) + to;
 #pragma unroll
               for (int w = 0; w < TILES / 2; ++w) {
