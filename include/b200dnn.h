@@ -267,6 +267,13 @@ B200DNN_API int32_t b200dnn_moe_layer(const void *x, int64_t ldx, const float *l
                           int32_t K, int32_t I, int32_t H, int32_t transB, int32_t act, void *out,
                           int64_t ld_out, void *stream);
 
+/* The same layer with the routing done by the caller (b200dnn_moe_gate): ids [T][topk] and weights [T][topk], taken as they are; an
+ * id outside 0 .. E - 1 is taken as the nearest that is not.  No counterpart in the reference. */
+B200DNN_API int32_t b200dnn_moe_layer_routed(const void *x, int64_t ldx, const int32_t *ids, const float *weights, int32_t T, int32_t E,
+                          int32_t num_shared, int32_t topk, const b200dnn_moe_expert_t *experts,
+                          int32_t K, int32_t I, int32_t H, int32_t transB, int32_t act, void *out,
+                          int64_t ld_out, void *stream);
+
 /* ---- Building blocks of the expert-parallel MoE (experts sharded over GPUs).  No counterpart in the
  * reference, which is a single-process CPU library; the exchange of tokens between GPUs (NCCL
  * all-to-all) happens in the caller between these calls.  Device pointers only. ---- */
@@ -503,7 +510,8 @@ B200DNN_API int32_t b200dnn_paged_attention(const b200dnn_paged_attention_t *des
  *   weights = s of the chosen, divided by their sum with renorm, times scale.
  * Ties go to the lower index; scores are told apart as 64-bit values are.  A NaN ranks behind everything else (ids stay distinct
  * and in range) and makes the token's weights NaN where it enters them.  ids [T][topk] (required) and weights as
- * b200dnn_moe_route's, expert_counts and slot_to_row too. */
+ * b200dnn_moe_route's, expert_counts and slot_to_row too: b200dnn_moe_layer_routed takes the first two, the building blocks of
+ * the MoE the others. */
 enum { B200DNN_GATE_SOFTMAX = 0, B200DNN_GATE_SIGMOID = 1 };
 enum { B200DNN_GROUP_MAX = 0, B200DNN_GROUP_TOP2 = 1 };
 typedef struct b200dnn_moe_gate_t {

@@ -171,6 +171,36 @@ def test_routing_drives_the_expert_blocks(capi, oracle):
     assert_bf16_close(out.view(torch.int16).cpu().numpy().view(np.uint16), ref, max_ulp=1, what="experts", row_atol_frac=2.0 ** -7)
 
 
+@pytest.mark.parametrize("T,E,S,k", [(1, 4, 0, 2), (32, 64, 2, 6), (64, 255, 1, 3), (300, 16, 1, 4), (200, 300, 0, 5)])
+def test_a_layer_routed_by_the_caller(capi, T, E, S, k):
+    """b200dnn_moe_layer_routed on the ids and weights of b200dnn_moe_route is b200dnn_moe_layer bit for bit (in all forms of the routing); ids out of range meet the nearest expert."""
+    H, I = 128, 64
+    rng = np.random.default_rng(E)
+    x = torch.randn(T, H, generator=torch.Generator(device="cuda").manual_seed(0), device="cuda").to(torch.bfloat16)
+    logits = torch.from_numpy(rng.standard_normal((T, E)).astype(np.float32)).cuda()
+    w13, w2 = (torch.from_numpy(rng.integers(-127, 128, (E + S, *s), dtype=np.int8)).cuda() for s in ((H, 2 * I), (I, H)))
+    s13, s2 = torch.full((2 * I,), 1e-3, device="cuda"), torch.full((H,), 1e-3, device="cuda")
+    ex = (capi.MoeExpert * (E + S))()
+    for e in range(E + S):
+        ex[e].w13, ex[e].ldb13, ex[e].w13_scale, ex[e].w2, ex[e].ldb2, ex[e].w2_scale = w13[e].data_ptr(), 2 * I, s13.data_ptr(), w2[e].data_ptr(), H, s2.data_ptr()
+    st = stream()
+    ids, w = torch.zeros(T, k, dtype=torch.int32, device="cuda"), torch.zeros(T, k, device="cuda")
+    capi.check(capi.lib.b200dnn_moe_route(logits.data_ptr(), T, E, k, 1, ids.data_ptr(), w.data_ptr(), None, None, st))
+    outs = [torch.zeros(T, H, dtype=torch.bfloat16, device="cuda") for _ in range(3)]
+    tail = lambda o: (T, E, S, k, ex, H, I, H, 0, capi.ACT["silu_and_mul"], o.data_ptr(), H, st)
+    capi.check(capi.lib.b200dnn_moe_layer(x.data_ptr(), H, logits.data_ptr(), *tail(outs[0])))
+    capi.check(capi.lib.b200dnn_moe_layer_routed(x.data_ptr(), H, ids.data_ptr(), w.data_ptr(), *tail(outs[1])))
+    capi.check(capi.lib.b200dnn_stream_status(st))
+    assert torch.equal(outs[0], outs[1])
+    far = ids.clone()
+    far[ids == E - 1], far[ids == 0] = E + 1000, -5
+    capi.check(capi.lib.b200dnn_moe_layer_routed(x.data_ptr(), H, far.data_ptr(), w.data_ptr(), *tail(outs[2])))
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[2])
+    assert capi.lib.b200dnn_moe_layer_routed(x.data_ptr(), H, None, w.data_ptr(), *tail(outs[2])) == capi.FAILURE and "null" in capi.last_error()
+    capi.lib.b200dnn_clear_caches()
+
+
 def test_two_streams_at_once(capi):
     """Calls on streams of their own share no workspace: long and short batches side by side, many times, give what each gives alone."""
     from test_paged_attention_gpu import filled, queries

@@ -128,7 +128,7 @@ EXPORTS = ["b200dnn_last_error", "b200dnn_version", "b200dnn_device_count", "b20
            "b200dnn_ep_set_experts", "b200dnn_ep_nccl_unique_id", "b200dnn_ep_connect_nccl", "b200dnn_ep_connect_local",
            "b200dnn_moe_layer_ep", "b200dnn_moe_layer_ep_local", "b200dnn_ep_rows_per_rank", "b200dnn_ep_status",
            "b200dnn_phase_timing", "b200dnn_phase_times", "b200dnn_measure_int8_peak", "b200dnn_normalization", "b200dnn_sdpa",
-           "b200dnn_kv_append", "b200dnn_paged_attention", "b200dnn_moe_gate"]
+           "b200dnn_kv_append", "b200dnn_paged_attention", "b200dnn_moe_gate", "b200dnn_moe_layer_routed"]
 
 if not os.path.exists(LIB_PATH):
     raise ImportError(
@@ -166,6 +166,7 @@ lib.b200dnn_matmul_nshard.argtypes = [vp, C.POINTER(MatmulDesc), i32, vp]
 lib.b200dnn_group_matmul.argtypes = [i32, C.POINTER(MatmulDesc), vp]
 lib.b200dnn_fused_moe.argtypes = [i32, C.POINTER(MoeExpert), i32, i32, i32, i32, i32, i32, vp, vp, i32, i32, vp, i64, vp]
 lib.b200dnn_moe_route.argtypes = [vp, i32, i32, i32, i32, vp, vp, vp, vp, vp]
+lib.b200dnn_moe_layer_routed.argtypes = [vp, i64, vp, vp, i32, i32, i32, i32, C.POINTER(MoeExpert), i32, i32, i32, i32, i32, vp, i64, vp]
 lib.b200dnn_moe_layer.argtypes = [vp, i64, vp, i32, i32, i32, i32, C.POINTER(MoeExpert), i32, i32, i32, i32, i32, vp, i64, vp]
 
 

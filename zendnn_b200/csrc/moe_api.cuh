@@ -425,17 +425,23 @@ extern "C" int32_t b200dnn_fused_moe(int32_t G, const b200dnn_moe_expert_t *ex, 
   return B200DNN_SUCCESS;
 }
 
-extern "C" int32_t b200dnn_moe_layer(const void *x, int64_t ldx, const float *logits, int32_t T, int32_t E, int32_t S,
-                                     int32_t topk, const b200dnn_moe_expert_t *ex, int32_t K, int32_t I, int32_t H,
-                                     int32_t transB, int32_t act, void *out, int64_t ld_out, void *stream) {
+namespace {
+// One layer, routed by logits or (logits null) by the caller's ids and weights.
+int32_t moe_layer(const void *x, int64_t ldx, const float *logits, const int32_t *given, const float *given_w, int32_t T, int32_t E, int32_t S, int32_t topk,
+                  const b200dnn_moe_expert_t *ex, int32_t K, int32_t I, int32_t H, int32_t transB, int32_t act, void *out, int64_t ld_out, void *stream) {
   B2_ENTER(stream);
   Runtime &Rt = rt();
-  B2_CHECK(x && logits && ex && out && T > 0 && E > 0 && S >= 0 && topk > 0 && topk <= E && topk <= kMaxTopk, B200DNN_FAILURE, "bad argument");
+  B2_CHECK(x && (logits || (given && given_w)) && ex && out && T > 0 && E > 0 && S >= 0 && topk > 0 && topk <= E && topk <= kMaxTopk, B200DNN_FAILURE, "bad argument");
   B2_CHECK(ldx >= K && ld_out >= H, B200DNN_FAILURE, "leading dimension too small");
   const int G = E + S, ns = topk + S, R = T * ns;
-  const void *x_dev, *l_dev;
+  const void *x_dev, *l_dev = nullptr, *g_dev = nullptr, *gw_dev = nullptr;
   B2_TRY(stage_in(x, span_bytes(T, K, ldx, B200DNN_BF16), st, &x_dev));
-  B2_TRY(stage_in(logits, (size_t)T * E * 4, st, &l_dev));
+  if (logits) B2_TRY(stage_in(logits, (size_t)T * E * 4, st, &l_dev));
+  else {
+    B2_TRY(stage_in(given, (size_t)T * topk * 4, st, &g_dev));
+    B2_TRY(stage_in(given_w, (size_t)T * topk * 4, st, &gw_dev));
+  }
+  const int32_t *g_ids = (const int32_t *)g_dev; const float *g_w = (const float *)gw_dev;
   int32_t *ids = (int32_t *)Rt.ws.alloc((size_t)T * topk * 4);
   float *w = (float *)Rt.ws.alloc((size_t)T * topk * 4);
   int32_t *rank = (int32_t *)Rt.ws.alloc((size_t)T * topk * 4);
@@ -463,7 +469,7 @@ extern "C" int32_t b200dnn_moe_layer(const void *x, int64_t ldx, const float *lo
   if (T <= kRouteSmallT && T * topk <= kRouteSmallSlots && G <= kRouteSmallGroups) {
     zmax = (uint32_t *)Rt.ws.alloc((size_t)R * 4);
     B2_CHECK(zmax, B200DNN_FAILURE, "workspace allocation failed");
-#define B2_RS(PER) launch_pdl(route_small_kernel<PER>, 1u, 1024u, 0, st, true, (const float *)l_dev, T, E, topk, S, route_rows, row_off, tile_prefix, slot_rows, slot_w, row_token, zmax)
+#define B2_RS(PER) launch_pdl(route_small_kernel<PER>, 1u, 1024u, 0, st, true, (const float *)l_dev, g_ids, g_w, T, E, topk, S, route_rows, row_off, tile_prefix, slot_rows, slot_w, row_token, zmax)
     B2_TRY(E <= 32 ? B2_RS(1) : E <= 64 ? B2_RS(2) : E <= 128 ? B2_RS(4) : B2_RS(8));
 #undef B2_RS
     B2_LAUNCHED();
@@ -473,7 +479,7 @@ extern "C" int32_t b200dnn_moe_layer(const void *x, int64_t ldx, const float *lo
     zmax = (uint32_t *)Rt.ws.alloc((size_t)R * 4);
     int32_t *counts = (int32_t *)Rt.ws.alloc((size_t)chunks * E * 4);
     B2_CHECK(zmax && counts, B200DNN_FAILURE, "workspace allocation failed");
-#define B2_RC(PER) launch_pdl(route_count_kernel<PER>, chunks, (unsigned)kRouteChunkThreads, 0, st, true, (const float *)l_dev, T, E, topk, S, chunk, ids, w, counts, zmax)
+#define B2_RC(PER) launch_pdl(route_count_kernel<PER>, chunks, (unsigned)kRouteChunkThreads, 0, st, true, (const float *)l_dev, g_ids, g_w, T, E, topk, S, chunk, ids, w, counts, zmax)
     B2_TRY(E <= 32 ? B2_RC(1) : E <= 64 ? B2_RC(2) : E <= 128 ? B2_RC(4) : B2_RC(8));
 #undef B2_RC
     B2_LAUNCHED();
@@ -481,7 +487,11 @@ extern "C" int32_t b200dnn_moe_layer(const void *x, int64_t ldx, const float *lo
                       row_token));
     B2_LAUNCHED();
   } else {
-    B2_TRY(launch_route_topk((const float *)l_dev, T, E, topk, 1, ids, w, st));
+    if (logits) B2_TRY(launch_route_topk((const float *)l_dev, T, E, topk, 1, ids, w, st));
+    else {
+      route_given_kernel<<<(unsigned)(((int64_t)T * topk + 255) / 256), 256, 0, st>>>(g_ids, g_w, (int64_t)T * topk, E, ids, w);
+      B2_LAUNCHED();
+    }
     B2_TRY(launch_expert_rank(ids, T * topk, E, rank, cnt, st));
     expert_offsets_kernel<<<1, 32, 0, st>>>(cnt, E, S, T, row_off, tile_prefix, route_rows);
     B2_LAUNCHED();
@@ -514,6 +524,21 @@ extern "C" int32_t b200dnn_moe_layer(const void *x, int64_t ldx, const float *lo
   B2_CUDA(cudaGetLastError());
   rt().mark(8);
   return finish_out({&o_out}, st);
+}
+}  // namespace
+
+extern "C" int32_t b200dnn_moe_layer(const void *x, int64_t ldx, const float *logits, int32_t T, int32_t E, int32_t S,
+                                     int32_t topk, const b200dnn_moe_expert_t *ex, int32_t K, int32_t I, int32_t H,
+                                     int32_t transB, int32_t act, void *out, int64_t ld_out, void *stream) {
+  B2_CHECK(logits, B200DNN_FAILURE, "bad argument");
+  return moe_layer(x, ldx, logits, nullptr, nullptr, T, E, S, topk, ex, K, I, H, transB, act, out, ld_out, stream);
+}
+
+extern "C" int32_t b200dnn_moe_layer_routed(const void *x, int64_t ldx, const int32_t *ids, const float *weights, int32_t T, int32_t E, int32_t S,
+                                            int32_t topk, const b200dnn_moe_expert_t *ex, int32_t K, int32_t I, int32_t H,
+                                            int32_t transB, int32_t act, void *out, int64_t ld_out, void *stream) {
+  B2_CHECK(ids && weights, B200DNN_FAILURE, "moe layer: ids or weights is null");
+  return moe_layer(x, ldx, nullptr, ids, weights, T, E, S, topk, ex, K, I, H, transB, act, out, ld_out, stream);
 }
 
 // ------------------------------------------------------------------------------------------------

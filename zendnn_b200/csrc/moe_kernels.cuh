@@ -214,6 +214,17 @@ __device__ __forceinline__ void route_topk_warp(const float *l, int E, int k, in
   *id = min(my_id, E - 1);
   *weight = renorm ? __fdiv_rn(my_p, tot) : my_p;
 }
+// The same where the caller has chosen (b200dnn_moe_layer_routed): its ids, kept inside their range, and weights.
+__device__ __forceinline__ void route_given(const int32_t *ids, const float *w, int64_t t, int E, int k, int lane, int32_t *id, float *weight) {
+  *id = lane < k ? min(max(ids[t * k + lane], 0), E - 1) : 0;
+  *weight = lane < k ? w[t * k + lane] : 0.f;
+}
+__global__ void __launch_bounds__(256) route_given_kernel(const int32_t *given, const float *given_w, int64_t n, int E, int32_t *ids, float *w) {
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  ids[i] = min(max(given[i], 0), E - 1);
+  w[i] = given_w[i];
+}
 template <int PER>
 __global__ void __launch_bounds__(256) route_topk_warp_kernel(const float *logits, int T, int E, int k, int renorm, int32_t *ids, float *w) {
   const int t = (int)((blockIdx.x * (unsigned)blockDim.x + threadIdx.x) >> 5), lane = threadIdx.x & 31;
@@ -232,7 +243,7 @@ __global__ void __launch_bounds__(256) route_topk_warp_kernel(const float *logit
 // 2048 x 1408, top-6, went from 117 to 98 us.  Larger batches spread over the device instead: one CTA would walk several tokens per warp.
 constexpr int kRouteSmallT = 64, kRouteSmallSlots = 1024, kRouteSmallGroups = 256;
 template <int PER>
-__global__ void __launch_bounds__(1024) route_small_kernel(const float *logits, int T, int E, int k, int S, int tile_rows, int32_t *row_off,
+__global__ void __launch_bounds__(1024) route_small_kernel(const float *logits, const int32_t *given, const float *given_w, int T, int E, int k, int S, int tile_rows, int32_t *row_off,
                                                            int32_t *tile_prefix, int32_t *slot_rows, float *slot_w, int32_t *row_token, uint32_t *row_max) {
   __shared__ int32_t s_id[kRouteSmallSlots];
   __shared__ float s_w[kRouteSmallSlots];
@@ -245,7 +256,8 @@ __global__ void __launch_bounds__(1024) route_small_kernel(const float *logits, 
   for (int i = lane; i < E; i += 32) s_cnt[warp][i] = 0;
   for (int t = warp; t < T; t += 32) {
     int32_t id; float weight;
-    route_topk_warp<PER>(logits + (int64_t)t * E, E, k, 1, lane, &id, &weight);
+    if (given) route_given(given, given_w, t, E, k, lane, &id, &weight);
+    else route_topk_warp<PER>(logits + (int64_t)t * E, E, k, 1, lane, &id, &weight);
     if (lane < k) { s_id[t * k + lane] = id; s_w[t * k + lane] = weight; }
   }
   __syncthreads();
@@ -296,7 +308,7 @@ __global__ void __launch_bounds__(1024) route_small_kernel(const float *logits, 
 constexpr int kRouteChunkThreads = 1024, kRouteMaxChunks = 256;
 inline int route_chunk_tokens(int T) { return 32 * (int)((T + 32LL * kRouteMaxChunks - 1) / (32LL * kRouteMaxChunks)); }
 template <int PER>
-__global__ void __launch_bounds__(kRouteChunkThreads) route_count_kernel(const float *logits, int T, int E, int k, int S, int chunk, int32_t *ids, float *w, int32_t *counts,
+__global__ void __launch_bounds__(kRouteChunkThreads) route_count_kernel(const float *logits, const int32_t *given, const float *given_w, int T, int E, int k, int S, int chunk, int32_t *ids, float *w, int32_t *counts,
                                                                          uint32_t *row_max) {
   __shared__ int hist[PER * 32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -307,7 +319,8 @@ __global__ void __launch_bounds__(kRouteChunkThreads) route_count_kernel(const f
   __syncthreads();
   for (int t = t0 + warp; t < t1; t += kRouteChunkThreads / 32) {
     int32_t id; float weight;
-    route_topk_warp<PER>(logits + (int64_t)t * E, E, k, 1, lane, &id, &weight);
+    if (given) route_given(given, given_w, t, E, k, lane, &id, &weight);
+    else route_topk_warp<PER>(logits + (int64_t)t * E, E, k, 1, lane, &id, &weight);
     if (lane < k) { ids[t * k + lane] = id; w[t * k + lane] = weight; atomicAdd(&hist[id], 1); }
   }
   __syncthreads();
