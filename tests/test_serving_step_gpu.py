@@ -223,3 +223,52 @@ def test_two_streams_at_once(capi):
         torch.cuda.synchronize()
         for _, _, alone, out in jobs:
             assert torch.equal(alone, out)
+
+
+def test_graphs_captured_on_one_stream_run_side_by_side(capi):
+    """Graphs have scratch of their own: two captured one after the other on a stream, replayed on two streams at once and beside a call on the stream they were captured on, give
+    what each call gives alone; a graph's scratch serves later ones when it is gone."""
+    from test_paged_attention_gpu import filled, queries
+    g = torch.Generator(device="cuda").manual_seed(2)
+    home = torch.cuda.Stream()
+    jobs = []
+    for lens in ([20000, 5], [15000, 100, 9000], [12345]):
+        cache, table = filled(g, lens, 2, 64, "bf16", 16)
+        q, dev = queries(g, len(lens), 8, 64), torch.tensor(lens, dtype=torch.int32, device="cuda")
+        x = torch.randn(2000, 64, generator=g, device="cuda")
+        alone, out = torch.zeros_like(q), torch.zeros_like(q)
+        gates = []
+        for _ in range(2):
+            t = [torch.zeros(2000, 4, dtype=torch.int32, device="cuda"), torch.zeros(64, dtype=torch.int32, device="cuda"), torch.zeros(2000, 4, dtype=torch.int32, device="cuda")]
+            gates.append((capi.make_moe_gate(x, 4, t[0], expert_counts=t[1], slot_to_row=t[2]), t))
+        capi.check(run(capi, capi.lib.b200dnn_paged_attention, capi.make_paged_attention(cache.desc(capi), q, alone, table, dev)))
+        capi.check(run(capi, capi.lib.b200dnn_moe_gate, gates[0][0]))
+        jobs.append((capi.make_paged_attention(cache.desc(capi), q, out, table, dev), gates[1][0], (alone, *gates[0][1]), (out, *gates[1][1])))
+
+    def calls(job, st):
+        capi.check(capi.lib.b200dnn_paged_attention(C.byref(job[0]), st))
+        capi.check(capi.lib.b200dnn_moe_gate(C.byref(job[1]), st))
+
+    for round_ in range(3):
+        torch.cuda.synchronize()
+        graphs, streams = [], [torch.cuda.Stream() for _ in range(2)]
+        for job in jobs[:2]:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=home):
+                calls(job, home.cuda_stream)
+                calls(job, home.cuda_stream)
+            graphs.append(graph)
+        for _ in range(10):
+            for job in jobs:
+                for t in job[3]:
+                    t.zero_()
+            torch.cuda.synchronize()
+            for _ in range(2):
+                for s, graph in zip(streams, graphs):
+                    with torch.cuda.stream(s):
+                        graph.replay()
+                calls(jobs[2], home.cuda_stream)
+            torch.cuda.synchronize()
+            for job in jobs:
+                assert all(torch.equal(a, b) for a, b in zip(job[2], job[3]))
+        del graphs, graph

@@ -1361,6 +1361,7 @@ int32_t b200dnn_clear_caches(void) {
       D->host_packed.clear();
       D->packed_registry.clear();
     }
+    D->capture_blocks.release();
     std::lock_guard<std::mutex> lk(D->ctx_mu);
     for (auto &kv : D->ctxs) { std::lock_guard<std::mutex> lk2(kv.second->mu); kv.second->release_buffers(); }
   }

@@ -80,8 +80,9 @@ extern "C" int32_t b200dnn_moe_gate(const b200dnn_moe_gate_t *d, void *stream) {
   GateRowsArgs r{a.ids, nullptr, T, E, k, a.chunk, (int32_t *)counts.dev, (int32_t *)rows.dev};
   const bool second = grid > 1 && (d->expert_counts || d->slot_to_row);
   if (second) {
-    a.counts = (int32_t *)rt().ws.alloc((size_t)grid * gate_pad(E) * 4);
-    B2_CHECK(a.counts, B200DNN_FAILURE, "workspace allocation failed");
+    uint32_t *zeros; uint8_t *scratch = nullptr;
+    B2_TRY(call_scratch(0, (size_t)grid * gate_pad(E) * 4, st, &zeros, &scratch));
+    a.counts = (int32_t *)scratch;
     r.counts = a.counts;
   }
   B2_TRY(launch_gate(a, grid > 1 ? GateRowsArgs{} : r, grid, st));

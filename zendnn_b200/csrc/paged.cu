@@ -97,10 +97,11 @@ int32_t launch_split(PagedSplitArgs &s, bool f32, cudaStream_t st) {
   const int64_t most = (int64_t)s.a.B * s.rows * ((s.a.n_keys + unit - 1) / unit + 1);      // (a window may begin inside a unit)
   if (most >= (1ll << 31)) return B200DNN_UNIMPLEMENTED;
   const unsigned grid = (unsigned)std::min<int64_t>(most, (int64_t)resident * rt().sm_count);
-  s.part_o = (float *)rt().ws.alloc((size_t)grid * 2 * 8 * NT * DP * 4);
-  s.part_ml = (float2 *)rt().ws.alloc((size_t)grid * 2 * 8 * NT * 8);
-  B2_CHECK(s.part_o && s.part_ml, B200DNN_FAILURE, "workspace allocation failed");
-  s.counters = rt().counters;
+  const size_t part_o = (size_t)grid * 2 * 8 * NT * DP * 4, part_ml = (size_t)grid * 2 * 8 * NT * 8;
+  uint8_t *scratch = nullptr;
+  B2_TRY(call_scratch(grid, part_o + part_ml, st, &s.counters, &scratch));
+  s.part_o = (float *)scratch;
+  s.part_ml = (float2 *)(scratch + part_o);
   return launch(kern, grid, 32 * kPagedWarps, smem, st, s);
 }
 template <bool S8, int DP>

@@ -160,6 +160,26 @@ struct SmallBatch {
   }
 };
 
+// Workspace of calls that are captured into a graph: blocks of the graph's own, so that graphs captured on one stream may be replayed side by side, and beside calls on that
+// stream.  A block lives as long as a graph that was made with it (the graph holds a user object, whose destructor may not call CUDA and gives the block back
+// here), and is then used for the next capture.  Its first kCaptureZeros bytes are zero between launches.
+struct CaptureBlocks {
+  static constexpr size_t kCaptureZeros = 32 << 10;
+  struct Block { uint8_t *p; size_t cap; CaptureBlocks *home; };
+  std::mutex mu;
+  std::vector<Block> free_blocks;
+  static void CUDART_CB give_back(void *arg) {
+    Block *b = static_cast<Block *>(arg);
+    { std::lock_guard<std::mutex> lk(b->home->mu); b->home->free_blocks.push_back(*b); }
+    delete b;
+  }
+  void release() {
+    std::lock_guard<std::mutex> lk(mu);
+    for (Block &b : free_blocks) cudaFree(b.p);
+    free_blocks.clear();
+  }
+};
+
 struct Runtime;
 
 // State shared by every stream of one device: the weight caches (mutex-protected, as the reference's are:
@@ -175,6 +195,7 @@ struct DeviceShared {
   std::map<const void *, PackedWeight> host_packed;       // host-resident prepacked buffers uploaded once
   std::mutex ctx_mu;
   std::map<cudaStream_t, Runtime *> ctxs;
+  CaptureBlocks capture_blocks;
   std::mutex attr_mu;
   std::map<const void *, int> smem_limit;                 // kernels whose dynamic shared-memory limit was raised
   std::atomic<int> split_room[5] = {}, skinny_room[9] = {}, gs_tc_room[9] = {};   // by cluster size: see cluster_room
@@ -210,6 +231,7 @@ struct Runtime {
   Workspace ws;
   SmallBatch small;
   BlobCache blobs;
+  unsigned long long capture_id = 0; uint8_t *capture_block = nullptr; size_t capture_cap = 0;   // of the capture under way on this stream
   uint8_t *slab = nullptr; size_t slab_cap = 0;           // pinned staging for large gathered host inputs
   uint32_t *counters = nullptr; size_t n_counters = 0;   // split-K tile counters, kept zero between launches
   int32_t *status = nullptr;                              // status word the kernels write: device view of mapped pinned memory
@@ -314,6 +336,54 @@ inline int32_t ensure_max_smem(const void *fn, int bytes = 227 * 1024) {
     B2_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     have = bytes;
   }
+  return B200DNN_SUCCESS;
+}
+
+// Scratch of one call: `zeros` words that are zero and that the call's kernels leave zero, and `bytes` more.  From the stream's workspace, or from a block of the graph that is being captured
+// (calls captured one after the other on a stream share it, as they share the workspace).
+inline int32_t call_scratch(size_t zeros, size_t bytes, cudaStream_t st, uint32_t **z, uint8_t **p) {
+  Runtime &R = rt();
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  cudaGraph_t graph = nullptr;
+  if (cudaStreamGetCaptureInfo(st, &status, &id, &graph) != cudaSuccess) { cudaGetLastError(); status = cudaStreamCaptureStatusNone; }
+  B2_CHECK(zeros * 4 <= CaptureBlocks::kCaptureZeros && zeros <= R.n_counters, B200DNN_FAILURE, "too many counters");
+  if (status != cudaStreamCaptureStatusActive || !graph) {
+    *z = R.counters;
+    *p = (uint8_t *)R.ws.alloc(bytes);
+    B2_CHECK(*p, B200DNN_FAILURE, "workspace allocation of %zu bytes failed", bytes);
+    return B200DNN_SUCCESS;
+  }
+  const size_t need = CaptureBlocks::kCaptureZeros + bytes;
+  if (R.capture_id != id || R.capture_cap < need) {
+    CaptureBlocks &home = R.shared->capture_blocks;
+    CaptureBlocks::Block b{nullptr, 0, &home};
+    {
+      std::lock_guard<std::mutex> lk(home.mu);
+      for (size_t i = 0; i < home.free_blocks.size(); ++i)
+        if (home.free_blocks[i].cap >= need) { b = home.free_blocks[i]; home.free_blocks.erase(home.free_blocks.begin() + i); break; }
+    }
+    if (!b.p) {
+      RelaxedCapture relaxed;
+      b.cap = need > (size_t(4) << 20) ? need : (size_t(4) << 20);
+      B2_CUDA(cudaMalloc((void **)&b.p, b.cap));
+      cudaStream_t tmp = nullptr;
+      cudaError_t e = cudaStreamCreateWithFlags(&tmp, cudaStreamNonBlocking);
+      if (e == cudaSuccess) e = cudaMemsetAsync(b.p, 0, CaptureBlocks::kCaptureZeros, tmp);
+      if (e == cudaSuccess) e = cudaStreamSynchronize(tmp);
+      if (tmp) cudaStreamDestroy(tmp);
+      if (e != cudaSuccess) { cudaFree(b.p); return fail(B200DNN_FAILURE, "scratch of a captured call: %s", cudaGetErrorString(e)); }
+    }
+    CaptureBlocks::Block *held = new CaptureBlocks::Block(b);
+    cudaUserObject_t obj = nullptr;
+    cudaError_t e = cudaUserObjectCreate(&obj, held, CaptureBlocks::give_back, 1, cudaUserObjectNoDestructorSync);
+    if (e != cudaSuccess) CaptureBlocks::give_back(held);
+    else if ((e = cudaGraphRetainUserObject(graph, obj, 1, cudaGraphUserObjectMove)) != cudaSuccess) cudaUserObjectRelease(obj, 1);
+    if (e != cudaSuccess) return fail(B200DNN_FAILURE, "scratch of a captured call: %s", cudaGetErrorString(e));
+    R.capture_id = id; R.capture_block = b.p; R.capture_cap = b.cap;
+  }
+  *z = (uint32_t *)R.capture_block;
+  *p = R.capture_block + CaptureBlocks::kCaptureZeros;
   return B200DNN_SUCCESS;
 }
 
