@@ -517,7 +517,7 @@ enum { B200DNN_GROUP_MAX = 0, B200DNN_GROUP_TOP2 = 1 };
 typedef struct b200dnn_moe_gate_t {
   int32_t num_tokens;             /* 0 allowed: the counts are zero */
   int32_t num_experts;            /* <= 1024 */
-  int32_t topk;                   /* <= 32 and <= the experts of topk_groups groups */
+  int32_t topk;                   /* <= 16 and <= the experts of topk_groups groups */
   int32_t score;                  /* B200DNN_GATE_* */
   int32_t num_groups, topk_groups;   /* 1, 1: no groups; num_groups <= 32 divides num_experts */
   int32_t group_score;            /* B200DNN_GROUP_* */

@@ -106,6 +106,25 @@ def test_biases_of_minus_infinity(capi, E, k, groups, top):
         check(capi, x, k, np.full(E, -np.inf, np.float32), score, groups, top, "max", False, 1.0)
 
 
+def test_weights_of_scores_that_32_bits_do_not_hold(capi):
+    """The chosen scores are zero in 32 bits, all of them equal or told apart by 64: divided by their sum they are ordinary numbers."""
+    x = torch.full((40, 64), -200.0)
+    x[20:] += torch.randn(20, 64, generator=torch.Generator().manual_seed(3))
+    for groups in (1, 4):
+        check(capi, x, 6, None, "sigmoid", groups, groups, "max", True, 1.0)
+    # a softmax whose bias chooses experts far below the largest logit
+    bias = np.zeros(64, np.float32)
+    bias[10:20] = 2.0
+    y = logits(40, 64, seed=6)
+    y[:, 10:20] -= 150.0
+    check(capi, y, 6, bias, "softmax", 1, 1, "max", True, 1.0)
+    y[:, 10:20] = y[0, 10]
+    check(capi, y, 6, bias, "softmax", 1, 1, "max", True, 2.5)
+    # of minus infinity: zero
+    y[:, 10:20] = -np.inf
+    check(capi, y, 6, bias, "softmax", 1, 1, "max", False, 1.0)
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("groups", [1, 4])
 def test_nans_rank_last(capi, score, groups):

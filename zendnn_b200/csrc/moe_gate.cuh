@@ -347,9 +347,9 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, int t, const f
     }
     if (a.sigmoid) score = __fdiv_rn(1.0f, __fadd_rn(1.0f, expf(-my_x)));
     else {
-      // the difference, and what its rounding left out
+      // the difference, and what its rounding left out (of minus infinity: nothing)
       const float d = __fsub_rn(my_x, mx), back = __fsub_rn(d, my_x), rest = __fsub_rn(__fsub_rn(my_x, __fsub_rn(d, back)), __fadd_rn(mx, back));
-      score = __fdiv_rn(expf(d) * (1.0f + rest), sum);
+      score = d < -1e30f ? 0.f : __fdiv_rn(expf(d) * (1.0f + rest), sum);
     }
   };
   // is this lane's choice before the next lane's in 64 bits too?
@@ -472,15 +472,17 @@ __global__ void __launch_bounds__(kGateTokenThreads<PER>) gate_kernel(const Gate
       for (int j = 0; j < PER; ++j) x[j] = j * 32 + lane < a.E ? __ldg(p + j * 32) : __int_as_float(0xff800000);
     }
     int id; float w;
-    if (!gate_token_f32<PER>(a, t, x, bias, group_of, lane, id, w)) {
-      if (lane == 0) slow[atomicAdd(&n_slow, 1)] = t;
-      continue;
-    }
-    if (a.renorm) {
+    bool done = gate_token_f32<PER>(a, t, x, bias, group_of, lane, id, w);
+    if (a.renorm && done) {
       float sum = lane < a.k ? w : 0.f;
 #pragma unroll
       for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       w = __fdiv_rn(w, sum);
+      done = __shfl_sync(0xffffffffu, sum, 0) >= 1e-30f;      // (else the scores of the chosen are zero in 32 bits, or not whole)
+    }
+    if (!done) {
+      if (lane == 0) slow[atomicAdd(&n_slow, 1)] = t;
+      continue;
     }
     if (lane < a.k) {
       a.ids[(int64_t)t * a.k + lane] = id;

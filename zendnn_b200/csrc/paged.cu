@@ -69,7 +69,7 @@ int32_t launch_append(const AppendArgs &a, cudaStream_t st) {
   auto cache = [&](const void *p, const int64_t (&s)[3]) {
     return apart(p, cb, ct, 2, s[0], a.page_size, s[1]) && apart(p, cb, ct, a.kv_heads, s[2], 1, 0);
   };
-  const bool vec = a.dim % 8 == 0 && a.rot % 16 == 0 && (!a.interleaved || a.rot == 0 || a.rot % 16 == 0) && cache(a.key, a.ck) && cache(a.value, a.cv) &&
+  const bool vec = a.dim % 8 == 0 && a.rot % 16 == 0 && cache(a.key, a.ck) && cache(a.value, a.cv) &&
                    apart(a.k, 16, it, a.T, a.ks[0], a.kv_heads, a.ks[1]) && apart(a.v, 16, it, a.T, a.vs[0], a.kv_heads, a.vs[1]) &&
                    (a.q_heads == 0 || (apart(a.q, 16, it, a.T, a.qs[0], a.q_heads, a.qs[1]) && apart(a.q_out, 16, it, a.T, a.os[0], a.q_heads, a.os[1]))) &&
                    (a.rot == 0 || (apart(a.cos_t, 16, 4, a.table_rows, a.table_ld, 1, 0) && apart(a.sin_t, 16, 4, a.table_rows, a.table_ld, 1, 0)));
@@ -85,7 +85,7 @@ int32_t launch_append(const AppendArgs &a, cudaStream_t st) {
   }
 }
 
-// The split form, where rows are 16-byte vectors: false when the call does not fit.
+// The split form, where rows are 16-byte vectors: B200DNN_UNIMPLEMENTED when the call does not fit.
 template <bool S8, int DP, int NT>
 int32_t launch_split(PagedSplitArgs &s, bool f32, cudaStream_t st) {
   const bool p8 = s.a.page_size % 8 == 0;
@@ -123,7 +123,6 @@ int32_t paged_split(const PagedArgs &a, bool out_f32, cudaStream_t st) {
   s.q_vec = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.qs[0] % 8 == 0 && a.qs[1] % 8 == 0;
   const int ov = out_f32 ? 4 : 8;
   s.out_vec = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.os[0] % ov == 0 && a.os[1] % ov == 0;
-  s.min_units = 1;
   if (a.dim <= 64) return launch_split_heads<S8, 64>(s, out_f32, st);
   if (a.dim <= 128) return launch_split_heads<S8, 128>(s, out_f32, st);
   return launch_split_heads<S8, 256>(s, out_f32, st);

@@ -123,7 +123,6 @@ struct PagedSplitArgs {
   int tiles;                       // head tiles of a key head
   int rows;                        // rows of a sequence: kv_heads * tiles
   int q_vec, out_vec;              // 16-byte rows of q and out
-  int min_units;                   // fewest units of a CTA
   float *part_o; float2 *part_ml;  // partial results: two slots a CTA
   uint32_t *counters;              // one a CTA, zero between launches
 };
@@ -182,19 +181,19 @@ __device__ __forceinline__ uint32_t paged_codes(uint32_t e) {
 }
 
 // What a CTA works on, one piece of a row after the other.
-template <bool P8, int kPagedUnit> struct PagedPieces {
+template <bool P8, int UNIT> struct PagedPieces {
   int seq, row, off, n;            // sequence, row of it, first unit in the row, units of the row
   int left;                        // units that the CTA still has, this piece included
   int lo, hi, base;                // visible keys of the sequence; where its units begin
   __device__ __forceinline__ int units() const { return min(n - off, left); }
-  __device__ __forceinline__ int first_key() const { return base + off * kPagedUnit; }
-  __device__ __forceinline__ int end_key() const { return min(hi, base + (off + units()) * kPagedUnit); }
+  __device__ __forceinline__ int first_key() const { return base + off * UNIT; }
+  __device__ __forceinline__ int end_key() const { return min(hi, base + (off + units()) * UNIT); }
   __device__ __forceinline__ void sequence(const PagedArgs &a) {
     int64_t l, h;
     if (!paged_range(a, seq, l, h)) l = h = 0;
     lo = (int)l; hi = (int)h;
     base = P8 ? lo & ~7 : lo;
-    n = hi > lo ? (hi - base + kPagedUnit - 1) / kPagedUnit : 0;
+    n = hi > lo ? (hi - base + UNIT - 1) / UNIT : 0;
   }
   __device__ __forceinline__ void next(const PagedSplitArgs &s) {
     const int u = units();
@@ -239,7 +238,7 @@ template <bool S8, int DP, int NT> constexpr size_t paged_smem() { return PagedR
 template <bool S8, int DP, int NT, bool P8, bool F32>
 __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 : 2) paged_split_kernel(const PagedSplitArgs s) {
   using Ring = PagedRing<S8, DP>;
-  constexpr int KS = Ring::KS, MT = KS / 16, kPagedUnit = KS * kPagedWarps;
+  constexpr int KS = Ring::KS, MT = KS / 16, UNIT = KS * kPagedWarps;
   constexpr int ST = Ring::ST, CH = Ring::CH, RI = Ring::RI, IN = Ring::IN, KP = Ring::kPieceK, VP = Ring::kPieceV, VB = Ring::kWideV, REGS = PagedJoin<S8, DP, NT>::kRegs;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float s_m[kPagedWarps][8 * NT], s_l[kPagedWarps][8 * NT];
@@ -265,7 +264,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
   }
 
   // ---- this CTA's units: every thread adds up the sequences of its stretch
-  PagedPieces<P8, kPagedUnit> ahead;
+  PagedPieces<P8, UNIT> ahead;
   int per, first;
   {
     const int stretch = (a.B + 32 * kPagedWarps - 1) / (32 * kPagedWarps), b0 = min(a.B, tid * stretch), b1 = min(a.B, b0 + stretch);
@@ -280,7 +279,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     int total = 0;
 #pragma unroll
     for (int w = 0; w < kPagedWarps; ++w) total += s_scan[w];
-    per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, s.min_units);
+    per = (total + (int)gridDim.x - 1) / (int)gridDim.x;
     first = min(total, (int)blockIdx.x * per);
     const int count = min(per, total - first);
     if (count <= 0) return;
@@ -296,7 +295,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     ahead.off = (first - before) - ahead.row * ahead.n;
     ahead.left = count;
   }
-  PagedPieces<P8, kPagedUnit> now = ahead;
+  PagedPieces<P8, UNIT> now = ahead;
 
   // ---- copies, ST steps ahead
   const uint32_t ring = smem_u32(smem) + (uint32_t)warp * (ST * Ring::kStep);
@@ -325,7 +324,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
       end_in = ahead.end_key();
       lo_in = ahead.lo;
     }
-    const int g = ahead.row / s.tiles, key = step_key + lane / EP * kPagedUnit + lane % EP * GK;
+    const int g = ahead.row / s.tiles, key = step_key + lane / EP * UNIT + lane % EP * GK;
     uint32_t page = 0, off = 0;                // (behind the end: page 0, token 0; nothing of it is used)
     if (key < end_in) {
       const uint32_t column = (uint32_t)key / (uint32_t)a.page_size;
@@ -336,7 +335,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     const uint64_t v = reinterpret_cast<uint64_t>(a.value) + (uint64_t)((int64_t)page * a.cv[0] + (int64_t)off * a.cv[1] + g * a.cv[2]) * ES;
     asm volatile("st.shared.v2.b64 [%0], {%1, %2};" ::"r"(plan + (uint32_t)lane * 16u), "l"(k), "l"(v) : "memory");
     if (S8) asm volatile("st.shared.b64 [%0], %1;" ::"r"(splan + (uint32_t)lane * 8u), "l"((int64_t)page * a.cs[0] + (int64_t)off * a.cs[1] + g * a.cs[2]) : "memory");
-    plan_n = min(SP, (end_in - step_key + kPagedUnit - 1) / kPagedUnit);
+    plan_n = min(SP, (end_in - step_key + UNIT - 1) / UNIT);
     __syncwarp();
   };
   int slot_in = 0, entry = 0;
@@ -349,7 +348,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     entry = plan_at * EP;
     cut_in = step_key + KS > end_in || step_key < lo_in;
     if (cut_in && limit) taken = (0xffffffffu >> max(0, step_key + 32 - end_in)) & (0xffffffffu << max(0, lo_in - step_key));
-    if (limit) { ++plan_at; step_key += kPagedUnit; }
+    if (limit) { ++plan_at; step_key += UNIT; }
   };
   // Copies of whole rows, CH lanes each (a key that the step does not see is zeros: its address is that of a token of the same page, or of page 0).  Measured on their own, 256-byte
   // rows: 6.8 TB/s, with every lane copying the pieces that it multiplies (64 bytes of a row at a time) 4.9.
@@ -450,7 +449,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     const int end = now.end_key();
     const float to_log2 = a.scale * kPagedLog2e, cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f, cap_out = a.softcap * kPagedLog2e;
 #pragma unroll 1
-    for (int key = now.first_key() + warp * KS; key < end; key += kPagedUnit) {
+    for (int key = now.first_key() + warp * KS; key < end; key += UNIT) {
       const uint32_t at = (uint32_t)slot * Ring::kStep;
       slot = slot + 1 == ST ? 0 : slot + 1;
       // ---- scores
