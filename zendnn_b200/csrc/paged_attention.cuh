@@ -98,9 +98,12 @@ __global__ void __launch_bounds__(32 * kPagedRowWarps) paged_rows_kernel(const P
 // ---------------------------------------------------------------------------------------------------------------------------------------------
 // The split form: rows of 16-byte vectors.
 //
-// Work.  A row is one sequence and one tile of up to 8 NT query heads of a key head; its visible keys come in units of 64 or 128.  The units of all rows, one row after the other, are
-// dealt out evenly: CTA c takes units [c per, (c + 1) per) of a grid that fills the device once, whatever the lengths are (they are on the device).  A row that lies in one CTA is finished
-// there; of the others every CTA leaves a partial result (maximum, sum, unnormalised output), and the last one to arrive joins them, in order.
+// Work.  A row is one sequence and one tile of up to 8 NT query heads of a key head; its visible keys come in units of 128 (of 64 where a row of the cache is longer than 256 bytes).
+// The units of all rows, one row after the other, are dealt out evenly: CTA c takes units [c per, (c + 1) per) of a grid that fills the device once, whatever the lengths are (they are on the
+// device).  A row that lies in one CTA is finished there; of the others every CTA leaves a partial result (maximum, sum, unnormalised output), and the last one to arrive joins them, in order.
+// With `side` > 1 it is a set of so many CTAs that takes units of so many rows of a sequence, each CTA its own row: they go through the same tokens at the same time.  Short rows that lie
+// token after token, head beside head, and the scales beside each other then come from L2 (s8, 8 key heads, pages of 32 tokens: 64 sequences of 8192 keys of 64 elements 204 -> 126 us,
+// 105 of 4096 of 128 189 -> 176).
 //
 // A warp takes 32 keys of a unit at a time (16 of more than 256 bytes), by itself: it copies their rows and those of their values into a ring of its own (cp.async, `ST` steps ahead, across the
 // ends of the work's rows), so that no barrier stands between steps.  The products run on mma.m16n8k16 with the keys as the 16 rows:
@@ -111,7 +114,7 @@ __global__ void __launch_bounds__(32 * kPagedRowWarps) paged_rows_kernel(const P
 // Tensor work is a fifth of what the memory leaves time for, so bf16 tiles of 16 x 8 serve: the call is bound by the bytes of the cache.
 //
 // Probabilities enter the second product as the sum of two bf16 (2^-17 relative): one alone would cost as much again as the rounding of a bf16 output.  For an f32 output it is three
-// (2^-25).  The row sum has them unrounded.  s8 codes are exact in bf16; a key's scale multiplies its scores, a value's scale its probability.
+// (2^-25).  The row sum has them unrounded.  s8 codes are exact in bf16 (here as 64ths); a key's scale multiplies its scores, a value's scale its probability.
 // The running maximum moves only when a score passes it by more than 2^8: probabilities are then at most 256, and few steps meet the exchange.
 
 constexpr float kPagedLog2e = 1.44269504088896340736f;
@@ -121,7 +124,7 @@ constexpr float kPagedReach = 8.0f;
 struct PagedSplitArgs {
   PagedArgs a;
   int tiles;                       // head tiles of a key head
-  int rows;                        // rows of a sequence: kv_heads * tiles
+  int blocks, side;                // rows of a sequence, kv_heads * tiles: so many blocks of rows side by side
   int q_vec, out_vec;              // 16-byte rows of q and out
   float *part_o; float2 *part_ml;  // partial results: two slots a CTA
   uint32_t *counters;              // one a CTA, zero between launches
@@ -172,17 +175,20 @@ __device__ __forceinline__ uint32_t paged_pack(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// Two codes (the bytes of e that stand in front of 0x43) as bf16: 0x43bb without its sign bit is 128 + (the low seven bits), with nothing else 128 or 256.
-__device__ __forceinline__ uint32_t paged_codes(uint32_t e) {
-  const uint32_t x = e & 0xff7fff7fu, y = e & 0xff80ff80u;
+// Two of a word's four codes as bf16, divided by 64: of its bytes 0 and 2, or 1 and 3.  A byte u with zeros in front is u 2^-133 as a bf16 (below 128 without the leading one, from there on
+// with it), so of u = code + 128 one multiplication and addition makes u 2^-6 - 2, exactly.
+__device__ __forceinline__ uint32_t paged_codes(uint32_t u) {
   uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(u), "r"(0x7f007f00u), "r"(0xc000c000u));
   return r;
 }
+__device__ __forceinline__ uint32_t paged_codes_even(uint32_t w) { return paged_codes((w ^ 0x80808080u) & 0x00ff00ffu); }
+__device__ __forceinline__ uint32_t paged_codes_odd(uint32_t w) { return paged_codes(__byte_perm(w ^ 0x80808080u, 0u, 0x4341)); }
+constexpr float kPagedCode = 64.0f;
 
 // What a CTA works on, one piece of a row after the other.
 template <bool P8, int UNIT> struct PagedPieces {
-  int seq, row, off, n;            // sequence, row of it, first unit in the row, units of the row
+  int seq, block, off, n;          // sequence, block of its rows, first unit in the row, units of the row
   int left;                        // units that the CTA still has, this piece included
   int lo, hi, base;                // visible keys of the sequence; where its units begin
   __device__ __forceinline__ int units() const { return min(n - off, left); }
@@ -201,8 +207,8 @@ template <bool P8, int UNIT> struct PagedPieces {
     off += u;
     if (off < n || left <= 0) return;
     off = 0;
-    if (++row < s.rows) return;
-    row = 0;
+    if (++block < s.blocks) return;
+    block = 0;
     for (n = 0; n == 0;) {                             // (there are units left, so there is a sequence with some)
       if (++seq >= s.a.B) { left = 0; return; }
       sequence(s.a);
@@ -251,6 +257,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
   const PagedArgs &a = s.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
   const float ninf = __int_as_float(0xff800000);
+  const int beside = (int)blockIdx.x % s.side;
 
   // ---- sequences without keys: zeros
   for (int i = blockIdx.x; i < a.B; i += gridDim.x) {
@@ -269,7 +276,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
   {
     const int stretch = (a.B + 32 * kPagedWarps - 1) / (32 * kPagedWarps), b0 = min(a.B, tid * stretch), b1 = min(a.B, b0 + stretch);
     int mine = 0;
-    for (ahead.seq = b0; ahead.seq < b1; ++ahead.seq) { ahead.sequence(a); mine += ahead.n * s.rows; }
+    for (ahead.seq = b0; ahead.seq < b1; ++ahead.seq) { ahead.sequence(a); mine += ahead.n * s.blocks; }
     int sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += v; }
@@ -279,8 +286,9 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     int total = 0;
 #pragma unroll
     for (int w = 0; w < kPagedWarps; ++w) total += s_scan[w];
-    per = (total + (int)gridDim.x - 1) / (int)gridDim.x;
-    first = min(total, (int)blockIdx.x * per);
+    const int sets = (int)gridDim.x / s.side;
+    per = (total + sets - 1) / sets;
+    first = min(total, (int)blockIdx.x / s.side * per);
     const int count = min(per, total - first);
     if (count <= 0) return;
     // the stretch: the last one that begins at or before the first unit
@@ -290,9 +298,9 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
     const int at = __popc(__ballot_sync(0xffffffffu, before + s_before[w * 32 + lane] <= first)) - 1;
     before += s_before[w * 32 + at];
     ahead.seq = (w * 32 + at) * stretch;
-    for (ahead.sequence(a); before + ahead.n * s.rows <= first && ahead.seq + 1 < a.B; ahead.sequence(a)) { before += ahead.n * s.rows; ++ahead.seq; }
-    ahead.row = (first - before) / ahead.n;
-    ahead.off = (first - before) - ahead.row * ahead.n;
+    for (ahead.sequence(a); before + ahead.n * s.blocks <= first && ahead.seq + 1 < a.B; ahead.sequence(a)) { before += ahead.n * s.blocks; ++ahead.seq; }
+    ahead.block = (first - before) / ahead.n;
+    ahead.off = (first - before) - ahead.block * ahead.n;
     ahead.left = count;
   }
   PagedPieces<P8, UNIT> now = ahead;
@@ -324,7 +332,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
       end_in = ahead.end_key();
       lo_in = ahead.lo;
     }
-    const int g = ahead.row / s.tiles, key = step_key + lane / EP * UNIT + lane % EP * GK;
+    const int g = (ahead.block * s.side + beside) / s.tiles, key = step_key + lane / EP * UNIT + lane % EP * GK;
     uint32_t page = 0, off = 0;                // (behind the end: page 0, token 0; nothing of it is used)
     if (key < end_in) {
       const uint32_t column = (uint32_t)key / (uint32_t)a.page_size;
@@ -415,7 +423,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
   int global = first;                         // its first unit among all
 #pragma unroll 1
   for (; now.left > 0;) {
-    const int units = now.units(), g = now.row / s.tiles, h0 = g * a.group + (now.row - g * s.tiles) * 8 * NT, heads = min(8 * NT, (g + 1) * a.group - h0);
+    const int units = now.units(), row = now.block * s.side + beside, g = row / s.tiles, h0 = g * a.group + (row - g * s.tiles) * 8 * NT, heads = min(8 * NT, (g + 1) * a.group - h0);
     // queries: the pieces that match the keys'
     uint32_t q[NT][DP / 8];
 #pragma unroll
@@ -436,6 +444,8 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
             v = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
+        // (elements of s8 keys are paired as their codes are)
+        if constexpr (S8) v = make_uint4(__byte_perm(v.x, v.y, 0x5410), __byte_perm(v.x, v.y, 0x7632), __byte_perm(v.z, v.w, 0x5410), __byte_perm(v.z, v.w, 0x7632));
         q[n][4 * t] = v.x; q[n][4 * t + 1] = v.y; q[n][4 * t + 2] = v.z; q[n][4 * t + 3] = v.w;
       }
     }
@@ -447,7 +457,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
       for (int t = 0; t < DP / 16; ++t) o[n][t][0] = o[n][t][1] = o[n][t][2] = o[n][t][3] = 0.f;
     }
     const int end = now.end_key();
-    const float to_log2 = a.scale * kPagedLog2e, cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f, cap_out = a.softcap * kPagedLog2e;
+    const float unit = S8 ? kPagedCode : 1.f, to_log2 = a.scale * kPagedLog2e * unit, cap_in = a.softcap > 0.f ? a.scale / a.softcap * unit : 0.f, cap_out = a.softcap * kPagedLog2e;
 #pragma unroll 1
     for (int key = now.first_key() + warp * KS; key < end; key += UNIT) {
       const uint32_t at = (uint32_t)slot * Ring::kStep;
@@ -476,8 +486,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
           if constexpr (S8) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint32_t a0 = paged_codes(__byte_perm(w0[e], 0x43434343u, 0x4140)), a2 = paged_codes(__byte_perm(w0[e], 0x43434343u, 0x4342));
-              const uint32_t a1 = paged_codes(__byte_perm(w1[e], 0x43434343u, 0x4140)), a3 = paged_codes(__byte_perm(w1[e], 0x43434343u, 0x4342));
+              const uint32_t a0 = paged_codes_even(w0[e]), a1 = paged_codes_even(w1[e]), a2 = paged_codes_odd(w0[e]), a3 = paged_codes_odd(w1[e]);
 #pragma unroll
               for (int n = 0; n < NT; ++n) paged_mma(x[i][n], a0, a1, a2, a3, q[n][8 * t + 2 * e], q[n][8 * t + 2 * e + 1]);
             }
@@ -578,12 +587,10 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
 #pragma unroll
           for (int w = 0; w < W; ++w) {
             if constexpr (S8) {
-              const uint32_t x01 = __byte_perm(v[0][w], v[1][w], 0x5140), x23 = __byte_perm(v[0][w], v[1][w], 0x7362);
-              const uint32_t y01 = __byte_perm(v[2][w], v[3][w], 0x5140), y23 = __byte_perm(v[2][w], v[3][w], 0x7362);
-              product((t * W + w) * 2, paged_codes(__byte_perm(x01, 0x43434343u, 0x4140)), paged_codes(__byte_perm(x01, 0x43434343u, 0x4342)),
-                      paged_codes(__byte_perm(y01, 0x43434343u, 0x4140)), paged_codes(__byte_perm(y01, 0x43434343u, 0x4342)));
-              product((t * W + w) * 2 + 1, paged_codes(__byte_perm(x23, 0x43434343u, 0x4140)), paged_codes(__byte_perm(x23, 0x43434343u, 0x4342)),
-                      paged_codes(__byte_perm(y23, 0x43434343u, 0x4140)), paged_codes(__byte_perm(y23, 0x43434343u, 0x4342)));
+              const uint32_t x = __byte_perm(v[0][w], v[1][w], 0x5410), y = __byte_perm(v[2][w], v[3][w], 0x5410);
+              const uint32_t x2 = __byte_perm(v[0][w], v[1][w], 0x7632), y2 = __byte_perm(v[2][w], v[3][w], 0x7632);
+              product((t * W + w) * 2, paged_codes_even(x), paged_codes_odd(x), paged_codes_even(y), paged_codes_odd(y));
+              product((t * W + w) * 2 + 1, paged_codes_even(x2), paged_codes_odd(x2), paged_codes_even(y2), paged_codes_odd(y2));
             } else {
               product(t * W + w, __byte_perm(v[0][w], v[1][w], 0x5410), __byte_perm(v[0][w], v[1][w], 0x7632), __byte_perm(v[2][w], v[3][w], 0x5410),
                       __byte_perm(v[2][w], v[3][w], 0x7632));
@@ -672,7 +679,7 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
             sum = sum * keep + paged_exp2(sink - f);
             top = to;
           }
-          const float by = sum == 0.f ? 0.f : keep / sum;
+          const float by = sum == 0.f ? 0.f : (S8 ? kPagedCode : 1.f) * keep / sum;
           if (a.lse && r == 0) a.lse[(int64_t)now.seq * a.q_heads + h] = sum == 0.f ? ninf : (top + log2f(sum)) * 0.693147180559945309417f;
 #pragma unroll
           for (int t = 0; t < DP / 16; t += (S8 && VB == 16 ? 8 : 4)) {
@@ -713,25 +720,26 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
       if (warp == 0) finish();
     } else {
       // a part of a row: slot 1 of the CTA in which the row begins, slot 0 of the others
-      const int begin = global - now.off, c0 = begin / per, c1 = (begin + now.n - 1) / per;
-      auto part = [&](int cta) { return (int64_t)cta * 2 + (cta == c0 ? 1 : 0); };
+      const int begin = global - now.off, c0 = begin / per, c1 = (begin + now.n - 1) / per;      // sets
+      auto part = [&](int set) { return (int64_t)(set * s.side + beside) * 2 + (set == c0 ? 1 : 0); };
+      const int my_set = (int)blockIdx.x / s.side;
       if (warp == 0) {
-        float4 *to = reinterpret_cast<float4 *>(s.part_o) + part(blockIdx.x) * (REGS / 4) * 32;
+        float4 *to = reinterpret_cast<float4 *>(s.part_o) + part(my_set) * (REGS / 4) * 32;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int t = 0; t < DP / 16; ++t) __stcg(to + (n * (DP / 16) + t) * 32 + lane, make_float4(o[n][t][0], o[n][t][1], o[n][t][2], o[n][t][3]));
 #pragma unroll
-          for (int e = 0; e < 2; ++e) if (r == 0) __stcg(s.part_ml + part(blockIdx.x) * 8 * NT + n * 8 + 2 * c + e, make_float2(m[n][e], l[n][e]));
+          for (int e = 0; e < 2; ++e) if (r == 0) __stcg(s.part_ml + part(my_set) * 8 * NT + n * 8 + 2 * c + e, make_float2(m[n][e], l[n][e]));
         }
         __threadfence();
         __syncwarp();
-        if (lane == 0) s_last = atomicAdd(s.counters + c0, 1u) == (uint32_t)(c1 - c0);
+        if (lane == 0) s_last = atomicAdd(s.counters + c0 * s.side + beside, 1u) == (uint32_t)(c1 - c0);
       }
       __syncthreads();
       if (s_last) {
         __threadfence();
-        if (tid == 0) s.counters[c0] = 0u;
+        if (tid == 0) s.counters[c0 * s.side + beside] = 0u;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           m[n][0] = m[n][1] = ninf; l[n][0] = l[n][1] = 0.f;
