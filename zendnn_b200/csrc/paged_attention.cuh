@@ -39,7 +39,8 @@ __device__ __forceinline__ int64_t paged_page(const PagedArgs &a, int i, int64_t
   return page;
 }
 
-// Any sizes, strides and alignment: a CTA per sequence and query head, a warp per key, the head dimension over the lanes, in f32 throughout.
+// Any sizes, strides and alignment: a CTA per sequence and query head, a warp per key, the head dimension over the lanes, in f32 throughout.  Every query head reads its key head again, from
+// L2: 32 sequences of up to 4096 keys, 32 / 8 heads of 128, 835 us.
 constexpr int kPagedRowWarps = 8;
 template <bool S8>
 __global__ void __launch_bounds__(32 * kPagedRowWarps) paged_rows_kernel(const PagedArgs a, int out_f32) {
@@ -111,7 +112,8 @@ __global__ void __launch_bounds__(32 * kPagedRowWarps) paged_rows_kernel(const P
 //                              of the product does not matter as long as Q agrees, so a piece of 8 elements is the operand of two products as it lies
 //   O^T[dim][head] = V^T P^T   lane (r, c) holds the same 8 (s8: 16) dims of the keys 2c, 2c + 1, 2c + 8, 2c + 9: a byte permutation pairs two keys of one dim
 // P^T comes from S^T by transposing 8 x 8 blocks (movmatrix).  Statistics of heads 2c and 2c + 1 and their columns of O^T are in the same lanes.
-// Tensor work is a fifth of what the memory leaves time for, so bf16 tiles of 16 x 8 serve: the call is bound by the bytes of the cache.
+// Tensor work is a fifth of what the memory leaves time for, so bf16 tiles of 16 x 8 serve: the call is bound by the bytes of the cache.  bf16, 32 / 8 heads of 128: the same 32 sequences 59 us
+// (10 of them start and join, 6.8 TB/s between), two of 131072 keys 171 us (0.96 of the copy rate).
 //
 // Probabilities enter the second product as the sum of two bf16 (2^-17 relative): one alone would cost as much again as the rounding of a bf16 output.  For an f32 output it is three
 // (2^-25).  The row sum has them unrounded.  s8 codes are exact in bf16 (here as 64ths); a key's scale multiplies its scores, a value's scale its probability.
