@@ -96,6 +96,16 @@ def test_lengths(capi, dt, lens):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "s8"])
+@pytest.mark.parametrize("heads,kv_heads", [(3, 3), (10, 5), (22, 11), (32, 16), (20, 20), (72, 6)])
+@pytest.mark.parametrize("lens", [[900] * 40, [3, 20000, 0, 64, 129], list(range(0, 3000, 37))])
+def test_numbers_of_rows(capi, dt, heads, kv_heads, lens):
+    """Rows of a sequence that go side by side, eight at a time and where eight do not divide them, with sequences that begin and end inside every share of the work."""
+    g = torch.Generator(device="cuda").manual_seed(kv_heads)
+    cache, table = filled(g, lens, kv_heads, 64, dt, 16)
+    check(capi, cache, table, lens, queries(g, len(lens), heads, 64))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "s8"])
 @pytest.mark.parametrize("spread", [0.0, 8.0, 40.0])
 def test_peaked_and_flat_softmax(capi, dt, spread):
     """Scores far apart (the running maximum moves again and again), and all equal."""
