@@ -177,6 +177,11 @@ __device__ __forceinline__ uint32_t paged_pack(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+__device__ __forceinline__ uint32_t paged_arrive(uint32_t *p) {
+  uint32_t n;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(n) : "l"(p) : "memory");
+  return n;
+}
 // Two of a word's four codes as bf16, divided by 64: of its bytes 0 and 2, or 1 and 3.  A byte u with zeros in front is u 2^-133 as a bf16 (below 128 without the leading one, from there on
 // with it), so of u = code + 128 one multiplication and addition makes u 2^-6 - 2, exactly.
 __device__ __forceinline__ uint32_t paged_codes(uint32_t u) {
@@ -734,13 +739,12 @@ __global__ void __launch_bounds__(32 * kPagedWarps, DP > 128 ? 1 : NT == 1 ? 3 :
 #pragma unroll
           for (int e = 0; e < 2; ++e) if (r == 0) __stcg(s.part_ml + part(my_set) * 8 * NT + n * 8 + 2 * c + e, make_float2(m[n][e], l[n][e]));
         }
-        __threadfence();
         __syncwarp();
-        if (lane == 0) s_last = atomicAdd(s.counters + c0 * s.side + beside, 1u) == (uint32_t)(c1 - c0);
+        // (the warp's stores in front of it, and the barrier behind it, are ordered by the one atomic; with fences 0.4 us more: one user, 500 keys 9.5 -> 9.05 us)
+        if (lane == 0) s_last = paged_arrive(s.counters + c0 * s.side + beside) == (uint32_t)(c1 - c0);
       }
       __syncthreads();
       if (s_last) {
-        __threadfence();
         if (tid == 0) s.counters[c0 * s.side + beside] = 0u;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
