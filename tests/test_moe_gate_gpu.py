@@ -106,6 +106,26 @@ def test_biases_of_minus_infinity(capi, E, k, groups, top):
         check(capi, x, k, np.full(E, -np.inf, np.float32), score, groups, top, "max", False, 1.0)
 
 
+@pytest.mark.parametrize("E,k,groups,top_groups", [(8, 1, 1, 1), (64, 1, 1, 1), (64, 6, 8, 3), (34, 1, 2, 2), (200, 8, 1, 1), (300, 3, 4, 4)])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_equal_experts_in_front_of_a_better_one(capi, E, k, groups, top_groups, dt):
+    """The last choice and the next expert have one logit, and one behind them is better by less than 32 bits tell: scores that are one in 32 bits, and neighbouring floats."""
+    g = torch.Generator().manual_seed(E + k)
+    values = torch.tensor([18.0, 20.0, 24.0, 30.0, 45.0])
+    x = values[torch.randint(0, 5, (300, E), generator=g)]
+    x[:40] = 20.0
+    x[torch.arange(40), torch.randint(2, E, (40,), generator=g)] = 25.0
+    x[40] = 20.0
+    near = torch.full((100, E), 1.0)
+    near[torch.arange(100), torch.randint(2, E, (100,), generator=g)] = 1.0 + 2.0 ** -23
+    bias = (np.random.default_rng(E).integers(0, 2, E) * 2.0 ** -24).astype(np.float32)
+    for score in ("sigmoid", "softmax"):
+        for b in (None, bias):
+            check(capi, x.to(torch.float32 if dt == "f32" else torch.bfloat16), k, b, score, groups, top_groups, "max", False, 1.0)
+            if dt == "f32":
+                check(capi, near, k, b, score, groups, top_groups, "top2", False, 1.0)
+
+
 def test_weights_of_scores_that_32_bits_do_not_hold(capi):
     """The chosen scores are zero in 32 bits, all of them equal or told apart by 64: divided by their sum they are ordinary numbers."""
     x = torch.full((40, 64), -200.0)

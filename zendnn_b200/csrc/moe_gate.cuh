@@ -110,7 +110,7 @@ __device__ __noinline__ void gate_choose(const GateArgs &a, const double *s, uns
 
 // The same in 32 bits, where these are enough.  f32 scores carry errors of a few steps, and the choice is taken for the one that 64 bits would make when every comparison that decides it is clear
 // by more than these: between neighbours among the chosen, between the last of them and the best that is left, between the last chosen group and the next.
-// (Experts with one logit and one bias have one score in either width, and go by their index.)  Choices that are not clear, one token in two thousand over 256 experts with continuous
+// (Experts with one logit and one bias have one score in either width, and go by their index; where the last choice is one of several such, it is all of these that the next has to be behind.)  Choices that are not clear, one token in two thousand over 256 experts with continuous
 // logits, are put in order by the 64-bit scores of these alone.  False: the token needs all its scores in 64 bits.  Returns the weights' scores in f32; the sum of the chosen is left to the caller.
 __device__ __forceinline__ uint32_t gate_key(float c) {      // (no NaN)
   const int b = __float_as_int(c);
@@ -363,7 +363,22 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, int t, const f
   look(rounds);
   const bool apart = before_next();
   id = my_id;
-  if (__all_sync(all, clear && (lane + 1 >= rounds || apart || same))) return true;
+  bool past = true;
+  if (rounds > a.k && __shfl_sync(all, (int)(same && !apart), a.k - 1)) {
+    // The last choice and the best that is left are one in logit and bias: what has to lie clearly behind is the best expert that is not.  (Its error: of a score below the last choice's,
+    // or, with a bias, of any.)
+    const float x1 = __shfl_sync(all, my_x, a.k - 1), b1 = __shfl_sync(all, my_b, a.k - 1), c1 = gate_value(__shfl_sync(all, my_key, a.k - 1)), s1 = __shfl_sync(all, score, a.k - 1);
+    uint32_t best = 0u;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const int e = j * 32 + lane;
+      if (key[j] > best && (gate_logit(a, t * a.ld + e) != x1 || (a.bias && a.bias[e] != b1))) best = key[j];
+    }
+    best = __reduce_max_sync(all, best);
+    const float c2 = gate_value(best), err = off + (a.sigmoid ? 6e-8f * fmaxf(fabsf(x1), 16.f) : 1.2e-7f * fmaxf(mx - x1, 1.f));
+    past = best == 0u || c1 - c2 > 2.f * err * (a.bias ? most : s1) + 3e-7f * (fabsf(c1) + fabsf(c2)) + 1e-36f;
+  }
+  if (__all_sync(all, clear && past && (lane + 1 >= rounds || apart || same))) return true;
   // Some neighbours are too close.  Choices up to one that is clearly behind its predecessor, at the k-th or later, hold the right ones: these are put in order by 64-bit scores.
   if (!__all_sync(all, clear) || (!a.sigmoid && a.bias)) return false;
   const int candidates = a.top_groups * a.per_group, more = min(min(32, candidates), a.k + 8);
