@@ -272,3 +272,33 @@ def test_graphs_captured_on_one_stream_run_side_by_side(capi):
             for job in jobs:
                 assert all(torch.equal(a, b) for a, b in zip(job[2], job[3]))
         del graphs, graph
+
+
+@pytest.mark.parametrize("dt,dim,page", [("bf16", 64, 16), ("s8", 64, 16), ("bf16", 64, 12), ("bf16", 50, 16)])
+def test_offsets_beyond_32_bits(capi, dt, dim, page):
+    """Pages that lie 1.3 billion elements apart hold and give what adjacent ones do: appended to, read, bit for bit."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    T, kv_heads, heads, pages, apart = 4 * page - 3, 2, 6, 4, 1_300_000_000
+    shape, kind = (pages, page, kv_heads, dim), torch.int8 if dt == "s8" else torch.bfloat16
+    far = torch.empty((pages - 1) * apart + 2 * page * kv_heads * dim, dtype=kind, device="cuda")
+    k, v = (torch.randn(T, kv_heads, dim, generator=g, device="cuda").to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(1, heads, dim, generator=g, device="cuda").to(torch.bfloat16)
+    table = torch.tensor([[3, 0, 2, 1]], dtype=torch.int32, device="cuda")
+    at = torch.arange(T, device="cuda")
+    slots = table[0].long()[at // page] * page + at % page
+    got = []
+    for wide in (False, True):
+        row = (kv_heads * dim, dim, 1)
+        kv = [far.as_strided(shape, (apart, *row), n * page * kv_heads * dim) for n in (0, 1)] if wide else [torch.zeros(shape, dtype=kind, device="cuda") for _ in range(2)]
+        scales = [torch.zeros(shape[:3], device="cuda") for _ in range(2)] if dt == "s8" else []
+        cache = capi.make_kv_cache(*kv, *scales)
+        out = torch.zeros(1, heads, dim, device="cuda")
+        capi.check(run(capi, capi.lib.b200dnn_kv_append, capi.make_kv_append(cache, k, v, slots)))
+        capi.check(run(capi, capi.lib.b200dnn_paged_attention, capi.make_paged_attention(cache, q, out, table, torch.tensor([T], dtype=torch.int32, device="cuda"))))
+        got.append((out, *(t.clone() for t in kv), *scales))
+    # (of the last page, three tokens were never written)
+    written = torch.ones(pages * page, dtype=torch.bool, device="cuda")
+    written[table[0, -1].long() * page + torch.arange(page - 3, page, device="cuda")] = False
+    assert torch.equal(got[0][0], got[1][0])
+    for a, b in zip(got[0][1:], got[1][1:]):
+        assert torch.equal(a.flatten(0, 1)[written], b.flatten(0, 1)[written])
