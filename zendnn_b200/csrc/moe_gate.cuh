@@ -109,7 +109,7 @@ __device__ __noinline__ void gate_choose(const GateArgs &a, const double *s, uns
 }
 
 // The same in 32 bits, where these are enough.  f32 scores carry errors of a few steps, and the choice is taken for the one that 64 bits would make when every comparison that decides it is clear
-// by more than these: between neighbours among the chosen, between the last of them and the best that is left, between the last chosen group and the next.
+// by more than these: between neighbours among the chosen, between the last of them and all that is left (of which the best stands for the others; their errors are bounded with it), between the last chosen group and the next.
 // (Experts with one logit and one bias have one score in either width, and go by their index; where the last choice is one of several such, it is all of these that the next has to be behind.)  Choices that are not clear, one token in two thousand over 256 experts with continuous
 // logits, are put in order by the 64-bit scores of these alone.  False: the token needs all its scores in 64 bits.  Returns the weights' scores in f32; the sum of the chosen is left to the caller.
 __device__ __forceinline__ uint32_t gate_key(float c) {      // (no NaN)
@@ -352,21 +352,22 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, int t, const f
       score = d < -1e30f ? 0.f : __fdiv_rn(expf(d) * (1.0f + rest), sum);
     }
   };
-  // is this lane's choice before the next lane's in 64 bits too?
+  // Is this lane's choice before the next lane's in 64 bits too?  By the errors of these two; behind every expert that is not in front of the next one (cut: the choices end here), too.  Without a
+  // bias these have smaller scores, and smaller errors; with one, any expert's score may lie behind a tiny one, and it is the error of the largest that counts.
+  const float most_err = 2.f * (off + 1.2e-7f) * most;      // (an exponential's argument adds |x| exp(-|x|) < 0.4 of its rounding)
   bool same = false;                           // one logit and one bias
-  auto before_next = [&]() {
+  auto before_next = [&](bool cut) {
     const float c = gate_value(my_key), c2 = __shfl_down_sync(all, c, 1), x2 = __shfl_down_sync(all, my_x, 1), b2 = __shfl_down_sync(all, my_b, 1), s2 = __shfl_down_sync(all, score, 1);
     const float err = off + (a.sigmoid ? 6e-8f * fmaxf(fabsf(my_x), fabsf(x2)) : 1.2e-7f * fmaxf(mx - my_x, mx - x2));
     same = my_x == x2 && my_b == b2;
-    return c - c2 > 2.f * err * fmaxf(score, s2) + 3e-7f * (fabsf(c) + fabsf(c2)) + 1e-36f;
+    return c - c2 > (cut && a.bias ? most_err : 2.f * err * fmaxf(score, s2)) + 3e-7f * (fabsf(c) + fabsf(c2)) + 1e-36f;
   };
   look(rounds);
-  const bool apart = before_next();
+  const bool apart = before_next(lane == a.k - 1);
   id = my_id;
   bool past = true;
   if (rounds > a.k && __shfl_sync(all, (int)(same && !apart), a.k - 1)) {
-    // The last choice and the best that is left are one in logit and bias: what has to lie clearly behind is the best expert that is not.  (Its error: of a score below the last choice's,
-    // or, with a bias, of any.)
+    // The last choice and the best that is left are one in logit and bias: what has to lie clearly behind is the best expert that is not.
     const float x1 = __shfl_sync(all, my_x, a.k - 1), b1 = __shfl_sync(all, my_b, a.k - 1), c1 = gate_value(__shfl_sync(all, my_key, a.k - 1)), s1 = __shfl_sync(all, score, a.k - 1);
     uint32_t best = 0u;
 #pragma unroll
@@ -376,7 +377,7 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, int t, const f
     }
     best = __reduce_max_sync(all, best);
     const float c2 = gate_value(best), err = off + (a.sigmoid ? 6e-8f * fmaxf(fabsf(x1), 16.f) : 1.2e-7f * fmaxf(mx - x1, 1.f));
-    past = best == 0u || c1 - c2 > 2.f * err * (a.bias ? most : s1) + 3e-7f * (fabsf(c1) + fabsf(c2)) + 1e-36f;
+    past = best == 0u || c1 - c2 > (a.bias ? most_err : 2.f * err * s1) + 3e-7f * (fabsf(c1) + fabsf(c2)) + 1e-36f;
   }
   if (__all_sync(all, clear && past && (lane + 1 >= rounds || apart || same))) return true;
   // Some neighbours are too close.  Choices up to one that is clearly behind its predecessor, at the k-th or later, hold the right ones: these are put in order by 64-bit scores.
@@ -384,7 +385,7 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, int t, const f
   const int candidates = a.top_groups * a.per_group, more = min(min(32, candidates), a.k + 8);
   choose(equal ? rounds : 0, more);
   look(more);
-  const unsigned ends = __ballot_sync(all, before_next() && lane + 1 >= a.k && lane + 1 < more) | (more == candidates ? 1u << (more - 1) : 0u);
+  const unsigned ends = __ballot_sync(all, before_next(true) && lane + 1 >= a.k && lane + 1 < more) | (more == candidates ? 1u << (more - 1) : 0u);
   if (ends == 0u) return false;
   const int p = __ffs(ends);                   // so many of them
   const double e64 = exp(a.sigmoid ? -(double)my_x : (double)my_x - (double)mx), c64 = a.sigmoid ? 1.0 / (1.0 + e64) + (double)my_b : e64;
