@@ -191,7 +191,7 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, int t, const f
     }
   }
   // Errors, relative: the exponential (ex2.approx, 2^-22) with the rounding of its argument, 6e-8 for every unit of it, twice for a softmax (its difference is rounded too); a sum and a quotient: 7e-7 together;
-  // a softmax's denominator up to 4e-6.  A group's two scores, each at most `most`: 1.2e-7 |d| exp(-|d|) of it, which 1e-7 covers.
+  // a softmax's denominator up to 4e-6.  A group's two scores, each at most `most`: 1.2e-7 |d| exp(-|d|) of it, which 1e-7 covers (and the rounding of its sum, see sum_err).
   const float off = a.sigmoid ? 8e-7f : 5e-6f;
   bool clear = true;
   if (a.groups > 1) {
@@ -250,6 +250,13 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, int t, const f
     if (!a.top2) second = 0u;
     // (a group of one expert has no second)
     const uint32_t mine = lane >= a.groups ? 0u : second ? gate_key(gate_value(first) + gate_value(second)) : first;
+    // A bias can make the two of a sum large and their sum small, of any group: its roundings go by the largest pair (an infinite one has no error, a sum that overflows is clear of nothing).
+    float sum_err = 0.f;
+    if (a.top2 && a.bias) {
+      const float v1 = fabsf(gate_value(first)), v2 = fabsf(gate_value(second));
+      const bool pair = lane < a.groups && second != 0u && finite_f32(v1) && finite_f32(v2);
+      sum_err = 3e-7f * __uint_as_float(__reduce_max_sync(all, pair ? __float_as_uint(v1 + v2) : 0u));
+    }
     int rank = 0;
     for (int g = 0; g < a.groups; ++g) {
       const uint32_t other = __shfl_sync(all, mine, g);
@@ -259,14 +266,14 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, int t, const f
     if (a.top_groups < a.groups) {
       auto group_at = [&](int r) { return __ffs(__ballot_sync(all, lane < a.groups && rank == r)) - 1; };
       auto value_of = [&](int g) { return gate_value(__shfl_sync(all, mine, g)); };
-      auto behind = [&](float u, float v) { return u - v > 4.f * (off + 1e-7f) * most + 3e-7f * (fabsf(u) + fabsf(v)) + 1e-36f; };
+      auto behind = [&](float u, float v, float more) { return u - v > 4.f * (off + 1e-7f) * most + 3e-7f * (fabsf(u) + fabsf(v)) + more + 1e-36f; };
       const int last = group_at(a.top_groups - 1), next = group_at(a.top_groups);
       const float u = value_of(last), v = value_of(next);
-      clear = behind(u, v);
+      clear = behind(u, v, sum_err);
       if (!clear && (a.sigmoid || !a.bias)) {
         // The last group that is in and the first that is out are too close (in 16384 tokens of 256 experts two or three times): their scores in 64 bits, from their members', where these two are
         // clear of the others and the members that count are clear of those that do not.
-        clear = (a.top_groups < 2 || behind(value_of(group_at(a.top_groups - 2)), u)) && (a.top_groups + 1 >= a.groups || behind(v, value_of(group_at(a.top_groups + 1))));
+        clear = (a.top_groups < 2 || behind(value_of(group_at(a.top_groups - 2)), u, sum_err)) && (a.top_groups + 1 >= a.groups || behind(v, value_of(group_at(a.top_groups + 1)), sum_err));
         double total[2];
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
@@ -286,7 +293,7 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, int t, const f
             const int e = (int)__reduce_min_sync(all, best == top ? (unsigned)at : 0x7fffffffu);
             if (r <= a.top2 && top != 0u) members[r] = e;
             // the first that does not count: clearly behind, or there is none
-            if (r == a.top2 + 1 && top != 0u && !behind(gate_value(before), gate_value(top))) clear = false;
+            if (r == a.top2 + 1 && top != 0u && !behind(gate_value(before), gate_value(top), 0.f)) clear = false;
           }
           double c = 0.0;
           if (lane < 2 && members[lane] >= 0) {
