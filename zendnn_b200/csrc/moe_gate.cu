@@ -52,7 +52,8 @@ extern "C" int32_t b200dnn_moe_gate(const b200dnn_moe_gate_t *d, void *stream) {
   B2_CHECK(k <= kGateMaxTopk, B200DNN_UNIMPLEMENTED, "%s: topk up to %d (%d)", who, kGateMaxTopk, k);
   B2_CHECK(std::isfinite(d->scale), B200DNN_FAILURE, "%s: scale must be finite", who);
   B2_CHECK(d->logits_dt == B200DNN_F32 || d->logits_dt == B200DNN_BF16, B200DNN_UNIMPLEMENTED, "%s: logits are f32 or bf16 (dt %d)", who, d->logits_dt);
-  B2_CHECK((int64_t)T * k < (1ll << 31), B200DNN_UNIMPLEMENTED, "%s: too many slots in one call", who);
+  // (the last block's tokens, and a step of the loop behind them, are counted in 32 bits)
+  B2_CHECK((int64_t)T * k < (1ll << 31) - 2 * kGateMostTokens, B200DNN_UNIMPLEMENTED, "%s: too many slots in one call", who);
   B2_CHECK(T == 0 || (d->logits && d->ids), B200DNN_FAILURE, "%s: logits or ids is null", who);
   B2_CHECK(T == 0 || d->ld >= E, B200DNN_FAILURE, "%s: ld (%lld) must be at least num_experts", who, (long long)d->ld);
   if (T == 0 && !d->expert_counts) return B200DNN_SUCCESS;
