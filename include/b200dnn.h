@@ -502,8 +502,8 @@ typedef struct b200dnn_paged_attention_t {
   int32_t window;                 /* 0: all keys */
   const int32_t *seq_lens;        /* [num_seqs], including the new token */
   const float *sinks;             /* [q_heads], may be NULL */
-  double scale;                   /* 0 = 1 / sqrt(head_dim) */
-  float softcap;                  /* 0: off */
+  double scale;                   /* 0 = 1 / sqrt(head_dim); up to 2^120 */
+  float softcap;                  /* 0: off; up to 2^120, and scale / softcap up to 2^121 */
   int32_t device;
 } b200dnn_paged_attention_t;
 B200DNN_API int32_t b200dnn_paged_attention(const b200dnn_paged_attention_t *desc, void *stream);

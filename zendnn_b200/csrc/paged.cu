@@ -205,6 +205,11 @@ extern "C" int32_t b200dnn_paged_attention(const b200dnn_paged_attention_t *d, v
   B2_CHECK(d->window >= 0, B200DNN_FAILURE, "%s: window must be >= 0", who);
   B2_CHECK(d->softcap >= 0.f && std::isfinite(d->softcap), B200DNN_FAILURE, "%s: softcap must be finite and >= 0", who);
   B2_CHECK(std::isfinite(d->scale), B200DNN_FAILURE, "%s: scale must be finite", who);
+  // (times 64 and log2(e), and one over the other, they are finite in f32: an infinity, times a product of zero, is a NaN)
+  B2_CHECK(std::fabs(d->scale) <= 0x1p120, B200DNN_UNIMPLEMENTED, "%s: scale up to 2^120", who);
+  B2_CHECK(d->softcap <= 0x1p120f, B200DNN_UNIMPLEMENTED, "%s: softcap up to 2^120", who);
+  const double scale = d->scale == 0.0 ? 1.0 / std::sqrt((double)c.head_dim) : d->scale;
+  B2_CHECK(d->softcap == 0.f || 64.0 * std::fabs(scale) <= 0x1p127 * d->softcap, B200DNN_UNIMPLEMENTED, "%s: scale / softcap up to 2^121", who);
   if (d->num_seqs == 0) return B200DNN_SUCCESS;
   B2_CHECK(d->max_pages > 0 && d->page_table_ld >= d->max_pages && d->page_table_ld < (1ll << 31), B200DNN_FAILURE, "%s: page_table_ld must be at least max_pages > 0", who);
   B2_CHECK(d->q && d->out && d->page_table && d->seq_lens, B200DNN_FAILURE, "%s: q, out, page_table or seq_lens is null", who);
