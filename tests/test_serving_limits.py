@@ -35,3 +35,12 @@ def test_caps_and_scales_within_32_bits_are_taken(capi):  # noqa: F811
         d = attend(capi)
         d.scale, d.softcap, d.num_seqs = scale, softcap, 0
         assert capi.lib.b200dnn_paged_attention(C.byref(d), None) == capi.SUCCESS, capi.last_error()
+
+
+def test_more_rows_than_a_grid_has(capi):  # noqa: F811
+    """Eight rows a block, and fewer than 2^31 blocks."""
+    d = append(capi)
+    for T, heads in ((1717986918, 6), (1561806289, 7), (572662306, 26), ((1 << 31) - 1, 5)):
+        d.num_tokens, d.q_heads = T, heads
+        assert (T * (heads + 4) + 7) // 8 >= 1 << 31
+        refused(capi, "b200dnn_kv_append", d, "too many", capi.UNIMPLEMENTED)

@@ -149,7 +149,7 @@ extern "C" int32_t b200dnn_kv_append(const b200dnn_kv_append_t *d, void *stream)
   B2_CHECK(d->rotary_dim >= 0 && d->rotary_dim % 2 == 0 && d->rotary_dim <= c.head_dim, B200DNN_FAILURE, "%s: rotary_dim must be even and at most head_dim (%d)", who, d->rotary_dim);
   if (T == 0) return B200DNN_SUCCESS;
   const int R = d->q_heads + 2 * c.kv_heads;
-  B2_CHECK(T < (1ll << 31) && d->q_heads < (1 << 16) && T * R < (1ll << 34), B200DNN_UNIMPLEMENTED, "%s: too many rows in one call", who);
+  B2_CHECK(T < (1ll << 31) && d->q_heads < (1 << 16) && T * R <= (1ll << 34) - 8, B200DNN_UNIMPLEMENTED, "%s: too many rows in one call", who);
   B2_CHECK(d->k && d->v && d->slots, B200DNN_FAILURE, "%s: k, v or slots is null", who);
   B2_CHECK(d->q_heads == 0 || (d->q && d->q_out), B200DNN_FAILURE, "%s: q or q_out is null", who);
   B2_CHECK(rows_apart(T, c.kv_heads, c.head_dim, d->k_stride) && rows_apart(T, c.kv_heads, c.head_dim, d->v_stride) &&
