@@ -367,6 +367,8 @@ def make_kv_append(cache, k, v, slots, q=None, q_out=None, positions=None, cos=N
         setattr(d, name, ptr(buf))
         setattr(d, name + "_stride", (C.c_int64 * 2)(*strides(buf)[:2]))
     d.slots = _index("kv append: slots", slots, "int64", (T,))
+    if positions is None and (cos is not None or sin is not None):
+        raise ValueError("kv append: cos and sin without positions: no row would be rotated")
     if positions is not None:
         if cos is None or sin is None or tuple(cos.shape) != tuple(sin.shape) or strides(cos) != strides(sin) or dt_of(cos) != DT["f32"] or dt_of(sin) != DT["f32"]:
             raise ValueError("kv append: cos and sin must be f32 arrays of one layout")
