@@ -634,17 +634,23 @@ struct Staging {
     return B200DNN_SUCCESS;
   }
   template <typename T> int32_t in(const T *p, size_t bytes, const T **out) const {
-    if (device) { *out = p; return B200DNN_SUCCESS; }
+    *out = p;
+    if (device || !p || bytes == 0) return B200DNN_SUCCESS;
+    bool host;
+    B2_TRY(where(p, &host));
+    if (!host) return B200DNN_SUCCESS;
     const void *d = nullptr;
     B2_TRY(stage_in(p, bytes, st, &d));
     *out = static_cast<const T *>(d);
     return B200DNN_SUCCESS;
   }
   int32_t out(void *p, size_t bytes, Staged *s, bool preload = false) const {
-    if (!device) return stage_out(p, bytes, st, s, preload);
     *s = Staged{};
     s->dev = p;
-    return B200DNN_SUCCESS;
+    if (device || !p || bytes == 0) return B200DNN_SUCCESS;
+    bool host;
+    B2_TRY(where(p, &host));
+    return host ? stage_out(p, bytes, st, s, preload) : B200DNN_SUCCESS;
   }
   // buffers that are used where they lie
   int32_t here(const char *what, const void *p) const {
@@ -653,6 +659,16 @@ struct Staging {
     if (cudaPointerGetAttributes(&at, p) != cudaSuccess) { cudaGetLastError(); at.type = cudaMemoryTypeUnregistered; }
     B2_CHECK(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, B200DNN_UNIMPLEMENTED, "%s: %s must be device memory", who, what);
     B2_CHECK(at.type == cudaMemoryTypeManaged || at.device == rt().shared->dev, B200DNN_FAILURE, "%s: %s lies on device %d, the current one is %d", who, what, at.device, rt().shared->dev);
+    return B200DNN_SUCCESS;
+  }
+  // Is it host memory?  A call with such buffers is synchronous, and what it stages lies in the stream's workspace: neither goes into a graph.
+  int32_t where(const void *p, bool *host) const {
+    *host = !is_device_ptr(p);
+    if (*host) {
+      cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+      if (cudaStreamIsCapturing(st, &status) != cudaSuccess) cudaGetLastError();
+      B2_CHECK(status == cudaStreamCaptureStatusNone, B200DNN_UNIMPLEMENTED, "%s: a captured call takes device memory only", who);
+    }
     return B200DNN_SUCCESS;
   }
 };
