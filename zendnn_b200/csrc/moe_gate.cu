@@ -65,7 +65,7 @@ extern "C" int32_t b200dnn_moe_gate(const b200dnn_moe_gate_t *d, void *stream) {
   B2_TRY(g.out(d->expert_counts, (size_t)E * 4, &counts));
   if (T == 0) {
     B2_CUDA(cudaMemsetAsync(counts.dev, 0, (size_t)E * 4, st));
-    return finish_out({&counts}, st);
+    return g.finish({&counts});
   }
   GateArgs a{};
   B2_TRY(g.in(d->logits, span_bytes(T, E, d->ld, d->logits_dt), &a.logits));
@@ -89,5 +89,5 @@ extern "C" int32_t b200dnn_moe_gate(const b200dnn_moe_gate_t *d, void *stream) {
   }
   B2_TRY(launch_gate(a, grid > 1 ? GateRowsArgs{} : r, grid, st));
   if (second) B2_TRY(launch(gate_rows_kernel, grid, kGateThreads, (size_t)gate_pad(E) * 8 + (size_t)E * 32, st, r));
-  return finish_out({&ids, &weights, &counts, &rows}, st);
+  return g.finish({&ids, &weights, &counts, &rows});
 }

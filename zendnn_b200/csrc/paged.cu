@@ -190,7 +190,7 @@ extern "C" int32_t b200dnn_kv_append(const b200dnn_kv_append_t *d, void *stream)
   const bool f32 = d->dt == B200DNN_F32, s8 = c.dt == B200DNN_S8;
   B2_TRY(f32 ? (s8 ? launch_append<float, true>(a, st) : launch_append<float, false>(a, st))
              : (s8 ? launch_append<__nv_bfloat16, true>(a, st) : launch_append<__nv_bfloat16, false>(a, st)));
-  return finish_out({&q_out}, st);
+  return g.finish({&q_out});
 }
 
 extern "C" int32_t b200dnn_paged_attention(const b200dnn_paged_attention_t *d, void *stream) {
@@ -242,8 +242,8 @@ extern "C" int32_t b200dnn_paged_attention(const b200dnn_paged_attention_t *d, v
   a.status = rt().status;
   const int f32 = d->out_dt == B200DNN_F32;
   const int32_t rc = c.dt == B200DNN_S8 ? paged_split<true>(a, f32, st) : paged_split<false>(a, f32, st);
-  if (rc != B200DNN_UNIMPLEMENTED) { B2_TRY(rc); return finish_out({&out, &lse}, st); }
+  if (rc != B200DNN_UNIMPLEMENTED) { B2_TRY(rc); return g.finish({&out, &lse}); }
   const unsigned grid = (unsigned)(B * d->q_heads);
   B2_TRY(c.dt == B200DNN_S8 ? launch(paged_rows_kernel<true>, grid, 32 * kPagedRowWarps, 0, st, a, f32) : launch(paged_rows_kernel<false>, grid, 32 * kPagedRowWarps, 0, st, a, f32));
-  return finish_out({&out, &lse}, st);
+  return g.finish({&out, &lse});
 }

@@ -628,6 +628,7 @@ inline int32_t finish_out(std::initializer_list<Staged *> outs, cudaStream_t st)
 // The buffers of a call whose caller may vouch for where they lie (`device` of its descriptor: 0, or ordinal + 1).
 struct Staging {
   int32_t device; cudaStream_t st; const char *who;
+  mutable bool staged = false;      // an input lies in host memory
   int32_t check() const {
     B2_CHECK(device >= 0 && (device == 0 || device - 1 == rt().shared->dev), B200DNN_FAILURE, "%s: the descriptor is one of device %d, the current one is %d", who, device - 1,
              rt().shared->dev);
@@ -642,6 +643,7 @@ struct Staging {
     const void *d = nullptr;
     B2_TRY(stage_in(p, bytes, st, &d));
     *out = static_cast<const T *>(d);
+    staged = true;
     return B200DNN_SUCCESS;
   }
   int32_t out(void *p, size_t bytes, Staged *s, bool preload = false) const {
@@ -651,6 +653,11 @@ struct Staging {
     bool host;
     B2_TRY(where(p, &host));
     return host ? stage_out(p, bytes, st, s, preload) : B200DNN_SUCCESS;
+  }
+  // Behind the launches.  A host input may still be read by its copy: the call waits for it as it does for host outputs.
+  int32_t finish(std::initializer_list<Staged *> outs) const {
+    for (Staged *s : outs) if (staged && !s->copy_back) s->sync = true;
+    return finish_out(outs, st);
   }
   // buffers that are used where they lie
   int32_t here(const char *what, const void *p) const {
