@@ -62,17 +62,17 @@ extern "C" int32_t b200dnn_moe_gate(const b200dnn_moe_gate_t *d, void *stream) {
   B2_TRY(g.check());
   const size_t ns = (size_t)T * k;
   Staged ids{}, weights{}, counts{}, rows{};
-  B2_TRY(g.out(d->expert_counts, (size_t)E * 4, &counts));
+  B2_TRY(g.out(d->expert_counts, (size_t)E * 4, 4, &counts));
   if (T == 0) {
     B2_CUDA(cudaMemsetAsync(counts.dev, 0, (size_t)E * 4, st));
     return g.finish({&counts});
   }
   GateArgs a{};
-  B2_TRY(g.in(d->logits, span_bytes(T, E, d->ld, d->logits_dt), &a.logits));
-  if (d->bias) B2_TRY(g.in(d->bias, (size_t)E * 4, &a.bias));
-  B2_TRY(g.out(d->ids, ns * 4, &ids));
-  B2_TRY(g.out(d->weights, ns * 4, &weights));
-  B2_TRY(g.out(d->slot_to_row, ns * 4, &rows));
+  B2_TRY(g.in(d->logits, span_bytes(T, E, d->ld, d->logits_dt), dt_size(d->logits_dt), &a.logits));
+  if (d->bias) B2_TRY(g.in(d->bias, (size_t)E * 4, 4, &a.bias));
+  B2_TRY(g.out(d->ids, ns * 4, 4, &ids));
+  B2_TRY(g.out(d->weights, ns * 4, 4, &weights));
+  B2_TRY(g.out(d->slot_to_row, ns * 4, 4, &rows));
   a.ld = d->ld; a.logits_bf16 = d->logits_dt == B200DNN_BF16;
   a.T = T; a.E = E; a.k = k; a.sigmoid = d->score == B200DNN_GATE_SIGMOID; a.groups = G; a.top_groups = d->topk_groups; a.per_group = E / G;
   a.top2 = d->group_score == B200DNN_GROUP_TOP2; a.renorm = d->renorm ? 1 : 0; a.scale = d->scale;

@@ -49,11 +49,11 @@ int32_t check_cache(const char *who, const b200dnn_kv_cache_t &c) {
 
 // The kernels use the cache where it lies.
 int32_t check_cache_here(const Staging &g, const b200dnn_kv_cache_t &c) {
-  B2_TRY(g.here("the cache", c.key));
-  B2_TRY(g.here("the cache", c.value));
+  B2_TRY(g.here("the cache", c.key, dt_size(c.dt)));
+  B2_TRY(g.here("the cache", c.value, dt_size(c.dt)));
   if (c.dt == B200DNN_S8) {
-    B2_TRY(g.here("the cache's scales", c.key_scale));
-    B2_TRY(g.here("the cache's scales", c.value_scale));
+    B2_TRY(g.here("the cache's scales", c.key_scale, 4));
+    B2_TRY(g.here("the cache's scales", c.value_scale, 4));
   }
   return B200DNN_SUCCESS;
 }
@@ -167,18 +167,18 @@ extern "C" int32_t b200dnn_kv_append(const b200dnn_kv_append_t *d, void *stream)
   AppendArgs a{};
   const size_t table_bytes = d->rotary_dim ? (size_t)((d->table_rows - 1) * d->table_ld + d->rotary_dim / 2) * 4 : 0;
   Staged q_out{};
-  B2_TRY(g.in(d->k, span2(T, c.kv_heads, c.head_dim, d->k_stride, d->dt), &a.k));
-  B2_TRY(g.in(d->v, span2(T, c.kv_heads, c.head_dim, d->v_stride, d->dt), &a.v));
-  B2_TRY(g.in(d->slots, (size_t)T * 8, &a.slots));
+  B2_TRY(g.in(d->k, span2(T, c.kv_heads, c.head_dim, d->k_stride, d->dt), dt_size(d->dt), &a.k));
+  B2_TRY(g.in(d->v, span2(T, c.kv_heads, c.head_dim, d->v_stride, d->dt), dt_size(d->dt), &a.v));
+  B2_TRY(g.in(d->slots, (size_t)T * 8, 8, &a.slots));
   if (d->q_heads) {
-    B2_TRY(g.in(d->q, span2(T, d->q_heads, c.head_dim, d->q_stride, d->dt), &a.q));
-    B2_TRY(g.out(d->q_out, span2(T, d->q_heads, c.head_dim, d->q_out_stride, d->dt), &q_out, true));
+    B2_TRY(g.in(d->q, span2(T, d->q_heads, c.head_dim, d->q_stride, d->dt), dt_size(d->dt), &a.q));
+    B2_TRY(g.out(d->q_out, span2(T, d->q_heads, c.head_dim, d->q_out_stride, d->dt), dt_size(d->dt), &q_out, true));
     a.q_out = q_out.dev;
   }
   if (d->rotary_dim) {
-    B2_TRY(g.in(d->positions, (size_t)T * 4, &a.positions));
-    B2_TRY(g.in(d->cos_table, table_bytes, &a.cos_t));
-    B2_TRY(g.in(d->sin_table, table_bytes, &a.sin_t));
+    B2_TRY(g.in(d->positions, (size_t)T * 4, 4, &a.positions));
+    B2_TRY(g.in(d->cos_table, table_bytes, 4, &a.cos_t));
+    B2_TRY(g.in(d->sin_table, table_bytes, 4, &a.sin_t));
   }
   for (int i = 0; i < 2; ++i) { a.qs[i] = d->q_stride[i]; a.ks[i] = d->k_stride[i]; a.vs[i] = d->v_stride[i]; a.os[i] = d->q_out_stride[i]; }
   for (int i = 0; i < 3; ++i) { a.ck[i] = c.key_stride[i]; a.cv[i] = c.value_stride[i]; a.cs[i] = c.scale_stride[i]; }
@@ -225,12 +225,12 @@ extern "C" int32_t b200dnn_paged_attention(const b200dnn_paged_attention_t *d, v
   B2_TRY(check_cache_here(g, c));
   PagedArgs a{};
   Staged out{}, lse{};
-  B2_TRY(g.in((const uint16_t *)d->q, span2(B, d->q_heads, c.head_dim, d->q_stride, d->q_dt), &a.q));
-  B2_TRY(g.in(d->page_table, (size_t)((B - 1) * d->page_table_ld + d->max_pages) * 4, &a.table));
-  B2_TRY(g.in(d->seq_lens, (size_t)B * 4, &a.lens));
-  if (d->sinks) B2_TRY(g.in(d->sinks, (size_t)d->q_heads * 4, &a.sinks));
-  B2_TRY(g.out(d->out, span2(B, d->q_heads, c.head_dim, d->out_stride, d->out_dt), &out, true));
-  if (d->lse) B2_TRY(g.out(d->lse, (size_t)B * d->q_heads * 4, &lse, true));
+  B2_TRY(g.in((const uint16_t *)d->q, span2(B, d->q_heads, c.head_dim, d->q_stride, d->q_dt), dt_size(d->q_dt), &a.q));
+  B2_TRY(g.in(d->page_table, (size_t)((B - 1) * d->page_table_ld + d->max_pages) * 4, 4, &a.table));
+  B2_TRY(g.in(d->seq_lens, (size_t)B * 4, 4, &a.lens));
+  if (d->sinks) B2_TRY(g.in(d->sinks, (size_t)d->q_heads * 4, 4, &a.sinks));
+  B2_TRY(g.out(d->out, span2(B, d->q_heads, c.head_dim, d->out_stride, d->out_dt), dt_size(d->out_dt), &out, true));
+  if (d->lse) B2_TRY(g.out(d->lse, (size_t)B * d->q_heads * 4, 4, &lse, true));
   a.out = out.dev; a.lse = d->lse ? (float *)lse.dev : nullptr;
   for (int i = 0; i < 2; ++i) { a.qs[i] = d->q_stride[i]; a.os[i] = d->out_stride[i]; }
   for (int i = 0; i < 3; ++i) { a.ck[i] = c.key_stride[i]; a.cv[i] = c.value_stride[i]; a.cs[i] = c.scale_stride[i]; }

@@ -634,25 +634,26 @@ struct Staging {
              rt().shared->dev);
     return B200DNN_SUCCESS;
   }
-  template <typename T> int32_t in(const T *p, size_t bytes, const T **out) const {
+  // size: of an element; a device address that is no multiple of it would fault
+  template <typename T> int32_t in(const T *p, size_t bytes, size_t size, const T **out) const {
     *out = p;
-    if (device || !p || bytes == 0) return B200DNN_SUCCESS;
-    bool host;
-    B2_TRY(where(p, &host));
-    if (!host) return B200DNN_SUCCESS;
+    if (!p || bytes == 0) return B200DNN_SUCCESS;
+    bool host = false;
+    if (!device) B2_TRY(where(p, &host));
+    if (!host) return aligned(p, size);
     const void *d = nullptr;
     B2_TRY(stage_in(p, bytes, st, &d));
     *out = static_cast<const T *>(d);
     staged = true;
     return B200DNN_SUCCESS;
   }
-  int32_t out(void *p, size_t bytes, Staged *s, bool preload = false) const {
+  int32_t out(void *p, size_t bytes, size_t size, Staged *s, bool preload = false) const {
     *s = Staged{};
     s->dev = p;
-    if (device || !p || bytes == 0) return B200DNN_SUCCESS;
-    bool host;
-    B2_TRY(where(p, &host));
-    return host ? stage_out(p, bytes, st, s, preload) : B200DNN_SUCCESS;
+    if (!p || bytes == 0) return B200DNN_SUCCESS;
+    bool host = false;
+    if (!device) B2_TRY(where(p, &host));
+    return host ? stage_out(p, bytes, st, s, preload) : aligned(p, size);
   }
   // Behind the launches.  A host input may still be read by its copy: the call waits for it as it does for host outputs.
   int32_t finish(std::initializer_list<Staged *> outs) const {
@@ -660,12 +661,17 @@ struct Staging {
     return finish_out(outs, st);
   }
   // buffers that are used where they lie
-  int32_t here(const char *what, const void *p) const {
+  int32_t here(const char *what, const void *p, size_t size) const {
+    B2_TRY(aligned(p, size));
     if (device) return B200DNN_SUCCESS;
     cudaPointerAttributes at;
     if (cudaPointerGetAttributes(&at, p) != cudaSuccess) { cudaGetLastError(); at.type = cudaMemoryTypeUnregistered; }
     B2_CHECK(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, B200DNN_UNIMPLEMENTED, "%s: %s must be device memory", who, what);
     B2_CHECK(at.type == cudaMemoryTypeManaged || at.device == rt().shared->dev, B200DNN_FAILURE, "%s: %s lies on device %d, the current one is %d", who, what, at.device, rt().shared->dev);
+    return B200DNN_SUCCESS;
+  }
+  int32_t aligned(const void *p, size_t size) const {
+    B2_CHECK(reinterpret_cast<uintptr_t>(p) % size == 0, B200DNN_FAILURE, "%s: an address (%p) is no multiple of its elements' %zu bytes", who, p, size);
     return B200DNN_SUCCESS;
   }
   // Is it host memory?  A call with such buffers is synchronous, and what it stages lies in the stream's workspace: neither goes into a graph.
