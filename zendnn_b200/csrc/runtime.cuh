@@ -664,10 +664,17 @@ struct Staging {
   int32_t here(const char *what, const void *p, size_t size) const {
     B2_TRY(aligned(p, size));
     if (device) return B200DNN_SUCCESS;
+    bool host;
+    B2_TRY(place(what, p, &host));
+    B2_CHECK(!host, B200DNN_UNIMPLEMENTED, "%s: %s must be device memory", who, what);
+    return B200DNN_SUCCESS;
+  }
+  // Host memory, or this device's?  (Another's is not mapped here: the kernels would fault.)
+  int32_t place(const char *what, const void *p, bool *host) const {
     cudaPointerAttributes at;
     if (cudaPointerGetAttributes(&at, p) != cudaSuccess) { cudaGetLastError(); at.type = cudaMemoryTypeUnregistered; }
-    B2_CHECK(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged, B200DNN_UNIMPLEMENTED, "%s: %s must be device memory", who, what);
-    B2_CHECK(at.type == cudaMemoryTypeManaged || at.device == rt().shared->dev, B200DNN_FAILURE, "%s: %s lies on device %d, the current one is %d", who, what, at.device, rt().shared->dev);
+    *host = at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged;
+    B2_CHECK(at.type != cudaMemoryTypeDevice || at.device == rt().shared->dev, B200DNN_FAILURE, "%s: %s lies on device %d, the current one is %d", who, what, at.device, rt().shared->dev);
     return B200DNN_SUCCESS;
   }
   int32_t aligned(const void *p, size_t size) const {
@@ -676,7 +683,7 @@ struct Staging {
   }
   // Is it host memory?  A call with such buffers is synchronous, and what it stages lies in the stream's workspace: neither goes into a graph.
   int32_t where(const void *p, bool *host) const {
-    *host = !is_device_ptr(p);
+    B2_TRY(place("a buffer", p, host));
     if (*host) {
       cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
       if (cudaStreamIsCapturing(st, &status) != cudaSuccess) cudaGetLastError();
