@@ -15,6 +15,9 @@ __device__ __forceinline__ void report_status(int32_t *status, int32_t code) {
   __threadfence_system();
 }
 
+// The same for an index out of range (its word: kIndexWord in runtime.cuh).
+__device__ __forceinline__ void report_index(int32_t *word) { report_status(word, 1); }
+
 __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));

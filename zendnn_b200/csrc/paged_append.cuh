@@ -20,7 +20,7 @@ struct AppendArgs {
   const int64_t *slots; int64_t n_slots;            // page * page_size + token, below n_slots
   int64_t T;
   int page_size, q_heads, kv_heads, dim, rot, interleaved;
-  int32_t *status;
+  int32_t *bad_index;
 };
 
 template <typename T> __device__ __forceinline__ float append_load(const void *p, int64_t i) {
@@ -36,7 +36,7 @@ template <typename T> __device__ __forceinline__ void append_store(void *p, int6
 __device__ __forceinline__ bool append_place(const AppendArgs &a, int64_t slot, int64_t pos, int64_t &page, int &off) {
   if (slot < 0) return false;
   if (slot >= a.n_slots || pos < 0 || (a.rot && pos >= a.table_rows)) {
-    report_status(a.status, kStatusIndex);
+    report_index(a.bad_index);
     return false;
   }
   page = slot / a.page_size;

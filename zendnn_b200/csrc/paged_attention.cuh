@@ -21,7 +21,7 @@ struct PagedArgs {
   int64_t n_pages, n_keys;                           // pages of the cache; most keys that a row of the table has room for
   int B, q_heads, kv_heads, group, dim, page_size, window;
   float scale, softcap;
-  int32_t *status;
+  int32_t *bad_index;
 };
 
 // A sequence's visible keys [lo, hi).  False: padding.  Lengths beyond the table's room are cut, and reported.
@@ -29,13 +29,13 @@ __device__ __forceinline__ bool paged_range(const PagedArgs &a, int i, int64_t &
   hi = a.lens[i];
   lo = 0;
   if (hi < 0) return false;
-  if (hi > a.n_keys) { report_status(a.status, kStatusIndex); hi = a.n_keys; }
+  if (hi > a.n_keys) { report_index(a.bad_index); hi = a.n_keys; }
   if (a.window > 0 && hi > a.window) lo = hi - a.window;
   return true;
 }
 __device__ __forceinline__ int64_t paged_page(const PagedArgs &a, int i, int64_t column) {
   int32_t page = a.table[i * a.table_ld + column];
-  if (page < 0 || page >= a.n_pages) { report_status(a.status, kStatusIndex); page = 0; }
+  if (page < 0 || page >= a.n_pages) { report_index(a.bad_index); page = 0; }
   return page;
 }
 

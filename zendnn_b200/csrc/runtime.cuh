@@ -446,18 +446,22 @@ struct CallGuard {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream_ptr);    \
   B2_TRY(guard__.enter(st))
 
-// Not a wait: a slot, position, page or length that a kernel of the paged cache met and made no access with.
-constexpr int32_t kStatusIndex = 41;
+// Behind the word of the bounded waits' codes, a word of its own: set when a kernel of the paged cache met a slot, position, page or length out of range and made no access with it.
+constexpr int kIndexWord = 1;
 
 // After the stream has been drained: did a kernel of this context give up on one of its bounded waits since the last
-// check?  The kernels write the code into mapped pinned memory, so the check is one host load.
+// check, or meet an index out of range?  The kernels write to mapped pinned memory, so the check is a host load or two.  Where both happened the wait is told
+// first, and the index by the next check.
 inline int32_t read_status() {
   Runtime &R = rt();
   const int32_t code = *R.status_host;
   if (code != 0) {
     *R.status_host = 0;
-    if (code == kStatusIndex) return fail(B200DNN_FAILURE, "an index array on the device held an entry out of range (code %d)", code);
     return fail(B200DNN_FAILURE, "a GEMM kernel gave up waiting on a barrier (code %d)", code);
+  }
+  if (R.status_host[kIndexWord] != 0) {
+    R.status_host[kIndexWord] = 0;
+    return fail(B200DNN_FAILURE, "an index array on the device held an entry out of range");
   }
   return B200DNN_SUCCESS;
 }
