@@ -436,7 +436,8 @@ B200DNN_API int32_t b200dnn_sdpa(const b200dnn_sdpa_t *desc, void *stream);
  * has a length and pages of its own, and query heads may share a key head.
  * Index arrays (slots, positions, page tables, lengths) are read on the device.  An entry that is out of range is met by no
  * access: the call leaves that token out (kv_append) or reads page 0 in its place (paged_attention: that sequence's output is
- * unspecified), and b200dnn_stream_status reports it.
+ * unspecified), and b200dnn_stream_status reports it: of calls on the stream, and of captured ones, on whichever stream of the
+ * device their graphs have run.
  * Buffers other than the cache may be host memory (staged, the call is then synchronous; not in a capture).  `device` of a descriptor: 0, or the
  * current device's ordinal + 1 where the caller vouches that all buffers are that device's (no look at the pointers).
  * Calls captured into a CUDA graph have scratch of that graph's own: such graphs may run side by side. ---- */

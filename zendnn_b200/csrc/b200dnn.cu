@@ -1311,7 +1311,13 @@ int32_t b200dnn_matmul(const b200dnn_matmul_t *d, void *stream) {
 int32_t b200dnn_stream_status(void *stream) {
   B2_ENTER(stream);
   B2_CUDA(cudaStreamSynchronize(st));
-  return read_status();
+  B2_TRY(read_status());
+  volatile int32_t *graph_index = rt().shared->graph_index_host;
+  if (*graph_index != 0) {
+    *graph_index = 0;
+    return fail(B200DNN_FAILURE, "an index array of a captured call held an entry out of range");
+  }
+  return B200DNN_SUCCESS;
 }
 
 int32_t b200dnn_phase_timing(void *stream, int32_t enable) {

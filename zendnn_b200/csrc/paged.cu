@@ -186,7 +186,7 @@ extern "C" int32_t b200dnn_kv_append(const b200dnn_kv_append_t *d, void *stream)
   a.table_rows = d->table_rows; a.table_ld = d->table_ld;
   a.n_slots = c.num_pages * c.page_size; a.T = T;
   a.page_size = c.page_size; a.q_heads = d->q_heads; a.kv_heads = c.kv_heads; a.dim = c.head_dim; a.rot = d->rotary_dim; a.interleaved = d->interleaved ? 1 : 0;
-  a.bad_index = rt().status + kIndexWord;
+  a.bad_index = index_word(st);
   const bool f32 = d->dt == B200DNN_F32, s8 = c.dt == B200DNN_S8;
   B2_TRY(f32 ? (s8 ? launch_append<float, true>(a, st) : launch_append<float, false>(a, st))
              : (s8 ? launch_append<__nv_bfloat16, true>(a, st) : launch_append<__nv_bfloat16, false>(a, st)));
@@ -239,7 +239,7 @@ extern "C" int32_t b200dnn_paged_attention(const b200dnn_paged_attention_t *d, v
   a.B = (int)B; a.q_heads = d->q_heads; a.kv_heads = c.kv_heads; a.group = d->q_heads / c.kv_heads; a.dim = c.head_dim; a.page_size = c.page_size; a.window = d->window;
   a.scale = d->scale == 0.0 ? 1.0f / std::sqrt((float)c.head_dim) : (float)d->scale;
   a.softcap = d->softcap;
-  a.bad_index = rt().status + kIndexWord;
+  a.bad_index = index_word(st);
   const int f32 = d->out_dt == B200DNN_F32;
   const int32_t rc = c.dt == B200DNN_S8 ? paged_split<true>(a, f32, st) : paged_split<false>(a, f32, st);
   if (rc != B200DNN_UNIMPLEMENTED) { B2_TRY(rc); return g.finish({&out, &lse}); }

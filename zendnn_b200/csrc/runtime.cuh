@@ -196,6 +196,7 @@ struct DeviceShared {
   std::mutex ctx_mu;
   std::map<cudaStream_t, Runtime *> ctxs;
   CaptureBlocks capture_blocks;
+  int32_t *graph_index = nullptr; volatile int32_t *graph_index_host = nullptr;      // see index_word
   std::mutex attr_mu;
   std::map<const void *, int> smem_limit;                 // kernels whose dynamic shared-memory limit was raised
   std::atomic<int> split_room[5] = {}, skinny_room[9] = {}, gs_tc_room[9] = {};   // by cluster size: see cluster_room
@@ -273,6 +274,13 @@ struct Runtime {
     memset(h, 0, 256);
     B2_CUDA(cudaHostGetDevicePointer(&d, h, 0));
     status_host = (volatile int32_t *)h; status = (int32_t *)d;
+    if (!sh->graph_index_host) {      // (contexts are made one at a time, under ctx_mu)
+      void *w = nullptr, *w_dev = nullptr;
+      B2_CUDA(cudaHostAlloc(&w, 64, cudaHostAllocMapped));
+      memset(w, 0, 64);
+      B2_CUDA(cudaHostGetDevicePointer(&w_dev, w, 0));
+      sh->graph_index = (int32_t *)w_dev; sh->graph_index_host = (volatile int32_t *)w;
+    }
     B2_CUDA(cudaMallocHost(&small.pinned, SmallBatch::kCap));
     B2_CUDA(cudaMalloc(&small.dev, SmallBatch::kCap));
     B2_CUDA(cudaEventCreateWithFlags(&small.ev, cudaEventDisableTiming));
@@ -448,6 +456,14 @@ struct CallGuard {
 
 // Behind the word of the bounded waits' codes, a word of its own: set when a kernel of the paged cache met a slot, position, page or length out of range and made no access with it.
 constexpr int kIndexWord = 1;
+
+// Where a call's kernels report such an index.  Those of a captured call run on whichever streams its graph is replayed on: they have one word of the device, which b200dnn_stream_status of any
+// stream reads, and calls that check themselves do not.
+inline int32_t *index_word(cudaStream_t st) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &status) != cudaSuccess) cudaGetLastError();
+  return status == cudaStreamCaptureStatusActive ? rt().shared->graph_index : rt().status + kIndexWord;
+}
 
 // After the stream has been drained: did a kernel of this context give up on one of its bounded waits since the last
 // check, or meet an index out of range?  The kernels write to mapped pinned memory, so the check is a host load or two.  Where both happened the wait is told
