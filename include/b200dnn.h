@@ -440,7 +440,8 @@ B200DNN_API int32_t b200dnn_sdpa(const b200dnn_sdpa_t *desc, void *stream);
  * device their graphs have run.
  * Buffers other than the cache may be host memory (staged, the call is then synchronous; not in a capture).  `device` of a descriptor: 0, or the
  * current device's ordinal + 1 where the caller vouches that all buffers are that device's (no look at the pointers).
- * Calls captured into a CUDA graph have scratch of that graph's own: such graphs may run side by side. ---- */
+ * Calls captured into a CUDA graph have scratch of that graph's own: such graphs may run side by side, but no two executables of
+ * one graph (nor one in two places of a larger graph), which share it. ---- */
 
 /* A cache of num_pages pages of page_size tokens.  Element (page, token, head, d) of the keys lies at key[page * key_stride[0] +
  * token * key_stride[1] + head * key_stride[2] + d], of the values likewise: [page][token][head][dim] and [page][head][token][dim]

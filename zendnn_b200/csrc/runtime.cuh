@@ -162,7 +162,7 @@ struct SmallBatch {
 
 // Workspace of calls that are captured into a graph: blocks of the graph's own, so that graphs captured on one stream may be replayed side by side, and beside calls on that
 // stream.  A block lives as long as a graph that was made with it (the graph holds a user object, whose destructor may not call CUDA and gives the block back
-// here), and is then used for the next capture.  Its first kCaptureZeros bytes are zero between launches.
+// here), and is then used for the next capture.  Its first kCaptureZeros bytes are zero between launches.  All executables of one graph have the same block: they are not to run at one time.
 struct CaptureBlocks {
   static constexpr size_t kCaptureZeros = 32 << 10;
   struct Block { uint8_t *p; size_t cap; CaptureBlocks *home; };
@@ -371,10 +371,13 @@ inline int32_t call_scratch(size_t zeros, size_t bytes, cudaStream_t st, uint32_
       for (size_t i = 0; i < home.free_blocks.size(); ++i)
         if (home.free_blocks[i].cap >= need) { b = home.free_blocks[i]; home.free_blocks.erase(home.free_blocks.begin() + i); break; }
     }
-    if (!b.p) {
+    {
+      // (zeroed again where it has served a graph before: what runs of two executables of that one at a time may have left there)
       RelaxedCapture relaxed;
-      b.cap = need > (size_t(4) << 20) ? need : (size_t(4) << 20);
-      B2_CUDA(cudaMalloc((void **)&b.p, b.cap));
+      if (!b.p) {
+        b.cap = need > (size_t(4) << 20) ? need : (size_t(4) << 20);
+        B2_CUDA(cudaMalloc((void **)&b.p, b.cap));
+      }
       cudaStream_t tmp = nullptr;
       cudaError_t e = cudaStreamCreateWithFlags(&tmp, cudaStreamNonBlocking);
       if (e == cudaSuccess) e = cudaMemsetAsync(b.p, 0, CaptureBlocks::kCaptureZeros, tmp);
