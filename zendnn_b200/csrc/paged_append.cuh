@@ -126,11 +126,12 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const AppendArgs a) {
 struct Append8 { float v[8]; };
 // eight elements as they lie in memory
 template <typename T> struct AppendRaw { uint4 w[sizeof(T) / 2]; };
-template <typename T> __device__ __forceinline__ AppendRaw<T> append_raw(const void *p, int64_t i) {
+// (KEPT: what the kernel does not write.  Queries may be rotated in place, and are not to be read through the read-only path.)
+template <typename T, bool KEPT> __device__ __forceinline__ AppendRaw<T> append_raw(const void *p, int64_t i) {
   const uint4 *q = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(p) + i * (int64_t)sizeof(T));
   AppendRaw<T> x;
 #pragma unroll
-  for (int e = 0; e < (int)sizeof(T) / 2; ++e) x.w[e] = __ldg(q + e);
+  for (int e = 0; e < (int)sizeof(T) / 2; ++e) x.w[e] = KEPT ? __ldg(q + e) : q[e];
   return x;
 }
 template <typename T> __device__ __forceinline__ Append8 append_floats(const AppendRaw<T> &x) {
@@ -193,14 +194,14 @@ __global__ void __launch_bounds__(256, 3) append_token_kernel(const AppendArgs a
       const void *p; int64_t at;
       source(row, p, at);
       const int o0 = row < a.q_heads + a.kv_heads ? c0 : 16 * j, o1 = row < a.q_heads + a.kv_heads ? c1 : 16 * j + 8;
-      if (o0 < a.dim) x[i][0] = append_raw<T>(p, at + o0);
-      if (o1 < a.dim) x[i][1] = append_raw<T>(p, at + o1);
+      if (o0 < a.dim) x[i][0] = append_raw<T, false>(p, at + o0);
+      if (o1 < a.dim) x[i][1] = append_raw<T, false>(p, at + o1);
     }
     if (!placed) {
       if (!append_place(a, slot, pos, page, off)) return;
       if (turns) {
-        cs = append_floats<float>(append_raw<float>(a.cos_t, pos * a.table_ld + 8 * j));
-        sn = append_floats<float>(append_raw<float>(a.sin_t, pos * a.table_ld + 8 * j));
+        cs = append_floats<float>(append_raw<float, true>(a.cos_t, pos * a.table_ld + 8 * j));
+        sn = append_floats<float>(append_raw<float, true>(a.sin_t, pos * a.table_ld + 8 * j));
       }
       placed = true;
     }
