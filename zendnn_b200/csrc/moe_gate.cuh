@@ -359,20 +359,40 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, int t, const f
       score = d < -1e30f ? 0.f : __fdiv_rn(expf(d) * (1.0f + rest), sum);
     }
   };
-  // Is this lane's choice before the next lane's in 64 bits too?  By the errors of these two; behind every expert that is not in front of the next one (cut: the choices end here), too.  Without a
-  // bias these have smaller scores, and smaller errors; with one, any expert's score may lie behind a tiny one, and it is the error of the largest that counts.
+  // Is this lane's choice before the next lane's in 64 bits too?  By the errors of these two; where the choices end, those that are not in front of the next one have to lie behind as well (all_behind).
+  // Without a bias these have smaller scores, and smaller errors; with one, any expert's score may lie behind a tiny one, and it is the error of the largest that counts.
   const float most_err = 2.f * (off + 1.2e-7f) * most;      // (an exponential's argument adds |x| exp(-|x|) < 0.4 of its rounding)
-  bool same = false;                           // one logit and one bias
-  auto before_next = [&](bool cut) {
+  bool same = false, all_behind = false;       // same: one logit and one bias
+  auto before_next = [&]() {
     const float c = gate_value(my_key), c2 = __shfl_down_sync(all, c, 1), x2 = __shfl_down_sync(all, my_x, 1), b2 = __shfl_down_sync(all, my_b, 1), s2 = __shfl_down_sync(all, score, 1);
     const float err = off + (a.sigmoid ? 6e-8f * fmaxf(fabsf(my_x), fabsf(x2)) : 1.2e-7f * fmaxf(mx - my_x, mx - x2));
     same = my_x == x2 && my_b == b2;
-    return c - c2 > (cut && a.bias ? most_err : 2.f * err * fmaxf(score, s2)) + 3e-7f * (fabsf(c) + fabsf(c2)) + 1e-36f;
+    const float clear_by = c - c2 - (3e-7f * (fabsf(c) + fabsf(c2)) + 1e-36f), own = 2.f * err * fmaxf(score, s2);
+    all_behind = clear_by > (a.bias ? most_err : own);
+    return clear_by > own;
   };
   look(rounds);
-  const bool apart = before_next(lane == a.k - 1);
+  bool apart = before_next();
   id = my_id;
   bool past = true;
+  if (rounds > a.k && a.bias) {
+    // The cut: the largest error that can lie behind it, or, where that is too much, every expert's own (one token in some thousands: the keys below the last choice's are those that are left).
+    if (__shfl_sync(all, (int)(apart && !all_behind), a.k - 1)) {
+      const uint32_t key1 = __shfl_sync(all, my_key, a.k - 1);
+      const float x1 = __shfl_sync(all, my_x, a.k - 1), c1 = gate_value(key1), err1 = (off + (a.sigmoid ? 6e-8f * fabsf(x1) : 1.2e-7f * (mx - x1))) * __shfl_sync(all, score, a.k - 1);
+      const float ninf = __int_as_float(0xff800000);
+      bool behind = true;
+#pragma unroll
+      for (int j = 0; j < PER; ++j)
+        if (key[j] != 0u && key[j] < key1) {
+          const float x2 = gate_logit(a, t * a.ld + j * 32 + lane), c2 = gate_value(key[j]);
+          const float s2 = a.sigmoid ? gate_rcp(1.0f + __expf(-x2)) : __expf(x2 - mx) * most, err2 = (off + (a.sigmoid ? 6e-8f * fabsf(x2) : 1.2e-7f * (mx - x2))) * s2;
+          behind &= c2 == ninf || c1 - c2 > err1 + err2 + 3e-7f * (fabsf(c1) + fabsf(c2)) + 1e-36f;      // (a bias of minus infinity: no error)
+        }
+      behind = __all_sync(all, behind);
+      if (lane == a.k - 1) apart = behind;
+    }
+  }
   if (rounds > a.k && __shfl_sync(all, (int)(same && !apart), a.k - 1)) {
     // The last choice and the best that is left are one in logit and bias: what has to lie clearly behind is the best expert that is not.
     const float x1 = __shfl_sync(all, my_x, a.k - 1), b1 = __shfl_sync(all, my_b, a.k - 1), c1 = gate_value(__shfl_sync(all, my_key, a.k - 1)), s1 = __shfl_sync(all, score, a.k - 1);
@@ -392,7 +412,8 @@ __device__ __forceinline__ bool gate_token_f32(const GateArgs &a, int t, const f
   const int candidates = a.top_groups * a.per_group, more = min(min(32, candidates), a.k + 8);
   choose(equal ? rounds : 0, more);
   look(more);
-  const unsigned ends = __ballot_sync(all, before_next(true) && lane + 1 >= a.k && lane + 1 < more) | (more == candidates ? 1u << (more - 1) : 0u);
+  before_next();
+  const unsigned ends = __ballot_sync(all, all_behind && lane + 1 >= a.k && lane + 1 < more) | (more == candidates ? 1u << (more - 1) : 0u);
   if (ends == 0u) return false;
   const int p = __ffs(ends);                   // so many of them
   const double e64 = exp(a.sigmoid ? -(double)my_x : (double)my_x - (double)mx), c64 = a.sigmoid ? 1.0 / (1.0 + e64) + (double)my_b : e64;
