@@ -92,6 +92,8 @@ int32_t launch_split(PagedSplitArgs &s, bool f32, cudaStream_t st) {
   auto kern = f32 ? (p8 ? paged_split_kernel<S8, DP, NT, true, true> : paged_split_kernel<S8, DP, NT, false, true>)
                   : (p8 ? paged_split_kernel<S8, DP, NT, true, false> : paged_split_kernel<S8, DP, NT, false, false>);
   constexpr size_t smem = paged_smem<S8, DP, NT>();
+  // CTAs an SM, by shared memory (2848 to 4128 bytes of a CTA's own and 1 KB of the system's beside the dynamic part: three fit where this says three).  DP 256: one (of bf16 no more
+  // fit; of s8 two would by shared memory and registers, not measured).
   const int resident = (int)std::min<size_t>(DP <= 128 ? 3 : 1, (size_t)(227 * 1024) / (smem + 2048));
   constexpr int unit = PagedRing<S8, DP>::KS * kPagedWarps;
   const int64_t most = (int64_t)s.a.B * s.blocks * s.side * ((s.a.n_keys + unit - 1) / unit + 1);      // (a window may begin inside a unit)

@@ -101,7 +101,8 @@ __global__ void __launch_bounds__(32 * kPagedRowWarps) paged_rows_kernel(const P
 //
 // Work.  A row is one sequence and one tile of up to 8 NT query heads of a key head; its visible keys come in units of 128 (of 64 where a row of the cache is longer than 256 bytes).
 // The units of all rows, one row after the other, are dealt out evenly: CTA c takes units [c per, (c + 1) per) of a grid that fills the device once, whatever the lengths are (they are on the
-// device).  A row that lies in one CTA is finished there; of the others every CTA leaves a partial result (maximum, sum, unnormalised output), and the last one to arrive joins them, in order.
+// device).  (Except for more than eight heads a key head of up to 64 elements: the grid counts three CTAs an SM by their shared memory, 190 to 218 registers a thread leave two, and the last third
+// of the work comes behind; 32 sequences of 8192 keys, 64 / 4 heads of 64, 64 us, 0.64 of the copy rate.)  A row that lies in one CTA is finished there; of the others every CTA leaves a partial result (maximum, sum, unnormalised output), and the last one to arrive joins them, in order.
 // With `side` > 1 it is a set of so many CTAs that takes units of so many rows of a sequence, each CTA its own row: they go through the same tokens at the same time.  Short rows that lie
 // token after token, head beside head, and the scales beside each other then come from L2 (s8, 8 key heads, pages of 32 tokens: 64 sequences of 8192 keys of 64 elements 204 -> 126 us,
 // 105 of 4096 of 128 189 -> 176).
@@ -113,7 +114,8 @@ __global__ void __launch_bounds__(32 * kPagedRowWarps) paged_rows_kernel(const P
 //   O^T[dim][head] = V^T P^T   lane (r, c) holds the same 8 (s8: 16) dims of the keys 2c, 2c + 1, 2c + 8, 2c + 9: a byte permutation pairs two keys of one dim
 // P^T comes from S^T by transposing 8 x 8 blocks (movmatrix).  Statistics of heads 2c and 2c + 1 and their columns of O^T are in the same lanes.
 // Tensor work is a fifth of what the memory leaves time for, so bf16 tiles of 16 x 8 serve: the call is bound by the bytes of the cache.  bf16, 32 / 8 heads of 128: the same 32 sequences 59 us
-// (10 of them start and join, 6.8 TB/s between), two of 131072 keys 171 us (0.96 of the copy rate).
+// (10 of them start and join, 6.8 TB/s between), two of 131072 keys 171 to 177 us (0.93 to 0.96 of the copy rate).  Head sizes are those of the next form, 64, 128 or 256: of 80 elements a row
+// of the ring and the products are those of 128 (32 sequences of 4096 keys 94 us, as long as with 128).
 //
 // Probabilities enter the second product as the sum of two bf16 (2^-17 relative): one alone would cost as much again as the rounding of a bf16 output.  For an f32 output it is three
 // (2^-25).  The row sum has them unrounded.  s8 codes are exact in bf16 (here as 64ths); a key's scale multiplies its scores, a value's scale its probability.
