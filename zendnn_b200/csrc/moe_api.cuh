@@ -523,6 +523,12 @@ int32_t moe_layer(const void *x, int64_t ldx, const float *logits, const int32_t
   B2_LAUNCHED();
   B2_CUDA(cudaGetLastError());
   rt().mark(8);
+  // (a routing in pinned memory may still be on its way: the caller is free to change it when the call returns; in a capture the copy is the graph's)
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (g_dev != given || gw_dev != given_w) {
+    if (cudaStreamIsCapturing(st, &capture) != cudaSuccess) cudaGetLastError();
+    if (capture == cudaStreamCaptureStatusNone && !o_out.copy_back) o_out.sync = true;
+  }
   return finish_out({&o_out}, st);
 }
 }  // namespace
